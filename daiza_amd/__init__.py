@@ -25,6 +25,7 @@ _f32p = ctypes.POINTER(ctypes.c_float)
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _vp = ctypes.c_void_p
+_i64 = ctypes.c_int64
 
 
 class DaizaError(RuntimeError):
@@ -167,6 +168,19 @@ _MODEL_PROTOS = {
     "dz_leviathan_check": ([_f32p, _f32p, ctypes.c_int, ctypes.c_uint32, _vp, ctypes.POINTER(ctypes.c_uint64),
                             ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "dz_sample_bonus": ([_f32p, _f32p, ctypes.c_int, _vp, ctypes.POINTER(ctypes.c_uint64), _u32p], ctypes.c_int),
+    "dz_kv4_create": ([ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)], ctypes.c_int),
+    "dz_kv4_free": ([_vp], ctypes.c_int),
+    "dz_kv4_len": ([_vp], ctypes.c_int),
+    "dz_kv4_truncate": ([_vp, ctypes.c_int], ctypes.c_int),
+    "dz_kv4_append_dev": ([_vp, _vp, _i64, _vp, _i64, ctypes.c_int, ctypes.c_int, _vp], ctypes.c_int),
+    "dz_kv4_read_dev": ([_vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp], ctypes.c_int),
+    "dz_kv4_attend_work_bytes": ([_vp, ctypes.c_int, ctypes.c_int], ctypes.c_size_t),
+    "dz_kv4_attend_dev": ([_vp, _vp, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp, _i64, _vp, _i64, _vp,
+                           _vp], ctypes.c_int),
+    "dz_kv4_evict_dev": ([_vp, _vp, _i64, ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, _vp], ctypes.c_int),
+    "dz_logprobs_work_bytes": ([ctypes.c_int, _i64, ctypes.c_int], ctypes.c_size_t),
+    "dz_logprobs_dev": ([_vp, _i64, ctypes.c_int, ctypes.c_int, _i64, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp],
+                        ctypes.c_int),
     "dz_spec_verify": ([_vp, _u32p, ctypes.c_int, _f32p, _vp, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64),
                         ctypes.POINTER(ctypes.c_int), _u32p], ctypes.c_int),
 }
@@ -275,7 +289,7 @@ class Tensor(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("type", ctypes.c_int32), ("data", _vp), ("n_bytes", ctypes.c_size_t)]
 
 
-GGUF_F32, GGUF_F16, GGUF_Q1_0 = 0, 1, 41
+GGUF_F32, GGUF_F16, GGUF_BF16, GGUF_Q1_0 = 0, 1, 30, 41
 
 
 class Model:
@@ -601,3 +615,139 @@ class Context:
 
     def stream(self):
         return lib().dz_ctx_stream(self._h)
+
+
+# ---------------------------------------------------------------- device arrays
+
+_TYPES = {"torch.float32": GGUF_F32, "torch.float16": GGUF_F16, "torch.bfloat16": GGUF_BF16}
+
+
+def _rows(t, what, shape, types=("torch.float32",)):
+    """(pointer, elements from row to row) of a device tensor of this shape (None: any size) with its rows contiguous."""
+    if str(t.dtype) not in types:
+        raise DaizaError(DZ_ERR_UNSUPPORTED, "%s of %s" % (what, t.dtype))
+    if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
+        raise DaizaError(DZ_ERR_TENSOR, "%s of shape %s, expected %s" % (what, tuple(t.shape), tuple("n" if s is None else s for s in shape)))
+    inner = 1
+    for d, st in zip(t.shape[:0:-1], t.stride()[:0:-1]):
+        if d > 1 and st != inner:
+            raise DaizaError(DZ_ERR_TENSOR, "%s: a row is not contiguous" % what)
+        inner *= d
+    if not t.is_cuda:
+        raise DaizaError(DZ_ERR_TENSOR, "%s is not on a device" % what)
+    return t.data_ptr(), max(t.stride(0), inner) if t.shape[0] < 2 else t.stride(0)
+
+
+def _stream_of(t, stream):
+    """The HIP stream (an int) of a call: the one given, or torch's current one."""
+    import torch
+    return torch.cuda.current_stream(t.device).cuda_stream if stream is None else int(getattr(stream, "cuda_stream", stream))
+
+
+def _work(t, n_bytes, stream):
+    """Device memory for one call, from torch's allocator: it goes back when the call has run on its stream."""
+    import torch
+    w = torch.empty(max(16, n_bytes), dtype=torch.uint8, device=t.device)
+    if stream != torch.cuda.current_stream(t.device).cuda_stream:
+        w.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
+    return w
+
+
+class Kv4Cache:
+    """A key/value cache held in 4 bits (dz_kv4): rows of kv_heads x head_dim keys and values.
+
+    Arrays are torch tensors on the cache's device, [row][head][head_dim] with any stride between rows; calls are enqueued on
+    `stream` (torch's current one if None) and return at once.  One cache's calls must be ordered by the caller.
+    """
+
+    def __init__(self, kv_heads, head_dim, capacity):
+        self.kv_heads, self.head_dim, self.capacity = int(kv_heads), int(head_dim), int(capacity)
+        h = _vp()
+        _check(lib().dz_kv4_create(self.kv_heads, self.head_dim, self.capacity, ctypes.byref(h)))
+        self._h = h
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().dz_kv4_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __len__(self):
+        return max(0, lib().dz_kv4_len(self._h))
+
+    def truncate(self, n):
+        """KvCache::truncate (kv_cache.rs:119-130): keeps the first n rows."""
+        _check(lib().dz_kv4_truncate(self._h, int(n)))
+
+    def append_dev(self, k, v, stream=None):
+        """Writes rows k, v [n][kv_heads][head_dim] (float32, float16 or bfloat16) behind the rows held."""
+        shape = (None, self.kv_heads, self.head_dim)
+        kp, ldk = _rows(k, "k", shape, _TYPES)
+        vp, ldv = _rows(v, "v", (k.shape[0],) + shape[1:], (str(k.dtype),))
+        _check(lib().dz_kv4_append_dev(self._h, kp, ldk, vp, ldv, _TYPES[str(k.dtype)], k.shape[0], _stream_of(k, stream)))
+
+    def read_dev(self, start, k=None, v=None, stream=None):
+        """The float32 values of rows start .. into k and v [kv_heads][n][head_dim] (contiguous; either may be None)."""
+        t = k if k is not None else v
+        if t is None:
+            return
+        for x, what in ((k, "k"), (v, "v")):
+            if x is not None:
+                _rows(x, what, (self.kv_heads, t.shape[1], self.head_dim))
+                if not x.is_contiguous():
+                    raise DaizaError(DZ_ERR_TENSOR, "%s is not contiguous" % what)
+        _check(lib().dz_kv4_read_dev(self._h, int(start), t.shape[1], None if k is None else k.data_ptr(),
+                                     None if v is None else v.data_ptr(), _stream_of(t, stream)))
+
+    def attend_dev(self, q, out, scale=None, weights=None, stream=None):
+        """Causal attention of the newest rows' queries q [n][heads][head_dim] into out (the same shape and type); scale is
+        1/sqrt(head_dim) if None.  weights (float32 [kv_heads][>= rows held]) grow by the attention that each row received."""
+        qp, ldq = _rows(q, "q", (None, None, self.head_dim), _TYPES)
+        op, ldo = _rows(out, "out", q.shape, (str(q.dtype),))
+        wp, ldw = (None, 0) if weights is None else _rows(weights, "weights", (self.kv_heads, None))
+        if weights is not None and weights.shape[1] < len(self):
+            raise DaizaError(DZ_ERR_TENSOR, "weights of %d rows, %d held" % (weights.shape[1], len(self)))
+        s = _stream_of(q, stream)
+        w = _work(q, lib().dz_kv4_attend_work_bytes(self._h, q.shape[1], q.shape[0]), s)
+        _check(lib().dz_kv4_attend_dev(self._h, qp, ldq, _TYPES[str(q.dtype)], q.shape[1], q.shape[0],
+                                       self.head_dim ** -0.5 if scale is None else float(scale), wp, ldw, op, ldo, w.data_ptr(), s))
+
+    def evict_dev(self, dst, keep, recent, weights, dst_weights, kept, stream=None):
+        """Copies the newest `recent` rows and the keep - recent others of the largest weights to dst, in order; kept (int32
+        [kv_heads][m], m = min(keep, rows held)) receives their indices, dst_weights [kv_heads][>= m] (or None) their weights."""
+        m = min(int(keep), len(self))
+        wp, ldw = _rows(weights, "weights", (self.kv_heads, None))
+        dp, ldd = (None, 0) if dst_weights is None else _rows(dst_weights, "dst_weights", (self.kv_heads, None))
+        if weights.shape[1] < len(self) or (dst_weights is not None and dst_weights.shape[1] < m):
+            raise DaizaError(DZ_ERR_TENSOR, "evict: fewer weights than rows")
+        kp, ldk = _rows(kept, "kept", (self.kv_heads, m), ("torch.int32",))
+        if not kept.is_contiguous():
+            raise DaizaError(DZ_ERR_TENSOR, "kept is not contiguous")
+        _check(lib().dz_kv4_evict_dev(self._h, wp, ldw, int(keep), int(recent), dst._h, dp, ldd, kp, _stream_of(weights, stream)))
+
+
+def logprobs_dev(logits, tokens=None, logp=None, entropy=None, top_ids=None, top_logp=None, stream=None):
+    """Of rows of logits [n][vocab] (a torch tensor on the device, float32, float16 or bfloat16, any stride between rows): the
+    log probabilities logp [n] of tokens [n] (int32), the entropies [n] in nats, and the ids (int32) and log probabilities
+    of the top_ids.shape[1] best tokens, larger first, the lower id first among equal ones.  Every output may be None."""
+    lp, ld = _rows(logits, "logits", (None, None), _TYPES)
+    n, vocab = logits.shape
+    top = 0 if top_ids is None else top_ids.shape[1]
+    ptr = {}
+    for what, t, shape, ty in (("tokens", tokens, (n,), "torch.int32"), ("logp", logp, (n,), "torch.float32"),
+                               ("entropy", entropy, (n,), "torch.float32"), ("top_ids", top_ids, (n, top), "torch.int32"),
+                               ("top_logp", top_logp, (n, top), "torch.float32")):
+        if t is not None:
+            _rows(t, what, shape, (ty,))
+            if not t.is_contiguous():
+                raise DaizaError(DZ_ERR_TENSOR, "%s is not contiguous" % what)
+        ptr[what] = None if t is None else t.data_ptr()
+    s = _stream_of(logits, stream)
+    w = _work(logits, lib().dz_logprobs_work_bytes(n, vocab, top), s)
+    _check(lib().dz_logprobs_dev(lp, ld, _TYPES[str(logits.dtype)], n, vocab, ptr["tokens"], top, ptr["logp"], ptr["entropy"],
+                                 ptr["top_ids"], ptr["top_logp"], w.data_ptr(), s))

@@ -135,6 +135,83 @@ int dz_q1_0_ntiles(const dz_mat* m);
  * Replaces dequantize_q1_0_row_into (quant.rs:161-194) / row_into_slice (weights.rs:106). */
 int dz_q1_0_dequant_rows(dz_mat* m, size_t r0, size_t n, float* out);
 
+/* ===================== key/value cache held in 4 bits ===================== */
+
+/* Element types of device arrays (GGUF TensorType codes). */
+#define DZ_F32 0
+#define DZ_F16 1
+#define DZ_BF16 30
+
+/*
+ * A key/value cache whose rows are held in 4 bits: 17/32 byte a value instead of the 4 bytes of a context's f32
+ * cache (KvCache, cache/kv_cache.rs:17-130; the reference has no such form).  A row's head is blocks of 32 values,
+ * each a 4-bit float (a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6; nearest, ties to the even code) times a power of two per
+ * block: the smallest one at which the block's largest value does not round past 6, within [2^-120, 2^125] (a value
+ * past 6 * 2^125 is held as that).  A block with an infinity or a NaN reads back as NaN throughout.  Writing a row that was read back gives the same row.
+ *
+ * The calls below take device pointers and are enqueued on `stream` (a hipStream_t, NULL = default) without a host
+ * synchronisation; their lengths are the host's.  A cache belongs to the device that dz_device_init selected before
+ * dz_kv4_create; arrays elsewhere are refused.  Its calls must be ordered by the caller (one stream, or events).
+ * Every array is [row][head][head_dim] with `ld` elements from row to row (ld >= heads * head_dim); no
+ * alignment beyond the element's own is needed.
+ */
+typedef struct dz_kv4 dz_kv4;
+
+/* An empty cache for `capacity` rows of kv_heads x head_dim (64, 128 or 256) keys and values. */
+int dz_kv4_create(int kv_heads, int head_dim, int capacity, dz_kv4** out);
+int dz_kv4_free(dz_kv4* c);
+/* Rows held, or -1 for a null cache. */
+int dz_kv4_len(const dz_kv4* c);
+/* Keeps the first len rows (KvCache::truncate, kv_cache.rs:119-130: a longer request is a no-op). */
+int dz_kv4_truncate(dz_kv4* c, int len);
+
+/* Writes n rows of keys and values of `type` (DZ_F32, DZ_F16 or DZ_BF16) behind the rows held. */
+int dz_kv4_append_dev(dz_kv4* c, const void* k, int64_t ldk, const void* v, int64_t ldv, int type, int n, void* stream);
+/* The values that rows [start, start + n) stand for, f32: k[kv_heads][n][head_dim] and v (either may be NULL). */
+int dz_kv4_read_dev(const dz_kv4* c, int start, int n, float* k, float* v, void* stream);
+
+/*
+ * Causal attention of n queries over the cache, whose newest n rows are the queries' own: query i sees the rows
+ * [0, len - n + i].  n_head is a multiple of kv_heads, query head h reads key/value head h / (n_head / kv_heads)
+ * (attention.rs:149-203).  out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j]) V[j]; q and out are of `type`, scores,
+ * softmax statistics and sums f32.  What a query does not see (an infinity or a NaN of a later row) does not reach it.
+ * With `weights` (f32 [kv_heads] rows of ldw >= len elements, NULL: none), weights[g][j] += the sum of
+ * query j's softmax weights over all queries and the heads of group g, in a fixed order.
+ * `work` is device memory of dz_kv4_attend_work_bytes(c, n_head, n) bytes, 16-byte aligned, that no other work uses
+ * until the call has run (a captured call: until its last replay has); the size does not depend on the rows held.
+ */
+size_t dz_kv4_attend_work_bytes(const dz_kv4* c, int n_head, int n);
+int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
+                      int64_t ldw, void* out, int64_t ldo, void* work, void* stream);
+
+/*
+ * Eviction by accumulated attention weight: per key/value head the newest `recent` rows and the keep - recent others of
+ * the largest weights[g][j] (ties and zeros of either sign: the lower row first; NaN ranks below every number) are
+ * copied to `dst`, in order.  dst, another cache of the same shape, then holds m = min(keep, rows of c) rows; c is
+ * left as it is.  kept[kv_heads][m] (int32) receives the rows' indices in c and dst_weights (f32, rows of ld_dst >= m
+ * elements, NULL: none) their weights.  Needs 0 <= recent <= keep and room for m rows in dst.
+ */
+int dz_kv4_evict_dev(const dz_kv4* c, const float* weights, int64_t ldw, int keep, int recent, dz_kv4* dst,
+                     float* dst_weights, int64_t ld_dst, int32_t* kept, void* stream);
+
+/* ===================== log probabilities ===================== */
+
+/*
+ * Of n rows of logits [vocab] on the device (`type` DZ_F32, DZ_F16 or DZ_BF16; ld elements from row to row):
+ *   logp[i]      log softmax(row i)[tokens[i]]  (tokens int32; NaN for a token outside [0, vocab))
+ *   entropy[i]   -sum p log p of the row, in nats
+ *   top_ids[i][j], top_logp[i][j]  the j < top largest (top <= 64, <= vocab), larger first, the lower id first among
+ *                equal ones, NaN last
+ * Any of tokens+logp, entropy, top_logp may be NULL; top = 0 takes no alternatives.  Sums are f32; a logit of -inf has
+ * probability 0; a row with a NaN or +inf, or of nothing but -inf, has NaN everywhere but in top_ids.  The
+ * untempered softmax is that of leviathan_check (engine.rs:1791-1819); the reference reports no log probabilities.
+ * `work`: dz_logprobs_work_bytes(n, vocab, top) bytes of device memory, 16-byte aligned, as for dz_kv4_attend_dev.
+ * Runs on the device that dz_device_init selected; arrays elsewhere are refused.
+ */
+size_t dz_logprobs_work_bytes(int n, int64_t vocab, int top);
+int dz_logprobs_dev(const void* logits, int64_t ld, int type, int n, int64_t vocab, const int32_t* tokens, int top, float* logp,
+                    float* entropy, int32_t* top_ids, float* top_logp, void* work, void* stream);
+
 /* ===================== model level: forward_single_token / forward_batch ===================== */
 
 typedef struct dz_model dz_model;
