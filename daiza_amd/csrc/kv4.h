@@ -21,16 +21,20 @@
 namespace dz {
 
 constexpr int kKv4Tile = 32;  // rows of a tile
+constexpr int kKv4MaxChunks = 512;
 constexpr int kKv4MinExp = -120, kKv4MaxExp = 125;  // 6 · 2^125 is the largest f32 of the format
 
 struct Kv4View {
   uint8_t *kc = nullptr, *vc = nullptr;  // codes  [kv head][cap · hd/2]
   uint8_t *ks = nullptr, *vs = nullptr;  // scales [kv head][cap · hd/32]
+  uint8_t* bad = nullptr;                // [kv head][cap/32]: not 0 where a row of the tile has (or had) a scale byte of 255
   int nkv = 0, hd = 0, cap = 0;          // cap: rows, a multiple of 32
   __host__ __device__ size_t code_head() const { return (size_t)cap * (size_t)(hd / 2); }
   __host__ __device__ size_t scale_head() const { return (size_t)cap * (size_t)(hd / 32); }
 };
-inline size_t kv4_bytes(int nkv, int hd, int cap) { return (size_t)nkv * cap * (size_t)(hd / 2 + hd / 32) * 2; }
+inline size_t kv4_bytes(int nkv, int hd, int cap) {
+  return (size_t)nkv * ((size_t)cap * (size_t)(hd / 2 + hd / 32) * 2 + (size_t)(cap / kKv4Tile));
+}
 // A view of kv4_bytes(nkv, hd, cap) bytes at base (16-byte aligned).
 inline Kv4View kv4_carve(uint8_t* base, int nkv, int hd, int cap) {
   Kv4View v;
@@ -41,6 +45,7 @@ inline Kv4View kv4_carve(uint8_t* base, int nkv, int hd, int cap) {
   v.vc = v.kc + nkv * v.code_head();
   v.ks = v.vc + nkv * v.code_head();
   v.vs = v.ks + nkv * v.scale_head();
+  v.bad = v.vs + nkv * v.scale_head();
   return v;
 }
 
@@ -75,7 +80,8 @@ __device__ __forceinline__ float kv4_scale(unsigned byte) {
 // Rows k, v -> rows [row0, row0 + n) of the cache.
 int kv4_append(const Kv4View& c, int row0, const void* k, int64_t ldk, const void* v, int64_t ldv, int type, int n, hipStream_t s);
 int kv4_read(const Kv4View& c, int start, int n, float* k, float* v, hipStream_t s);
-size_t kv4_attend_work(int hd, int n_head, int n);
+int prepare_kv4_kernels();
+size_t kv4_attend_work(const Kv4View& c, int n_head, int n);
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s);
 int kv4_evict(const Kv4View& c, int len, const float* weights, int64_t ldw, int keep, int recent, const Kv4View& dst,

@@ -2,6 +2,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <mutex>
 #include <new>
 
 #include "elem.h"
@@ -45,7 +46,10 @@ __global__ __launch_bounds__(HD) void kv4_append_kernel(Kv4View c, int row0, con
   for (int o = 1; o < 32; o <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, o));
   const int sb = kv4_scale_byte(__uint_as_float(big));
   code[d] = (uint8_t)kv4_code(x, sb);
-  if ((d & 31) == 0) (values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + d / 32] = (uint8_t)sb;
+  if ((d & 31) == 0) {
+    (values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + d / 32] = (uint8_t)sb;
+    if (sb == 255) c.bad[(size_t)g * (c.cap / kKv4Tile) + r / kKv4Tile] = 1;
+  }
   __syncthreads();
   if (!values) {
     if (d < HD / 8) {
@@ -114,111 +118,609 @@ int kv4_read(const Kv4View& c, int start, int n, float* k, float* v, hipStream_t
 
 // ---------------------------------------------------------------- attention
 
-// A (token, query head) per workgroup: tiles of 256 rows, a thread per row for the scores and per dim for the sums.
-template <int HD, class E>
-__global__ __launch_bounds__(256) void kv4_attend_simple_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq,
-                                                                int n, float scale, float2* __restrict__ stats,
-                                                                E* __restrict__ out, int64_t ldo) {
-  constexpr int T = HD / 32;
-  __shared__ float qs[HD], ps[256], red[4];
-  const int i = blockIdx.x, h = blockIdx.y, g = h / (nq / c.nkv), tid = threadIdx.x;
-  if (tid < HD) qs[tid] = to_f32(q[(size_t)i * ldq + (size_t)h * HD + tid]) * scale;
-  const int seen = len - n + i + 1;
-  const size_t ch = g * c.code_head(), sh = g * c.scale_head();
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  __syncthreads();
-  for (int p0 = 0; p0 < seen; p0 += 256) {
-    const int r = p0 + tid;
-    float sc = -INFINITY;
-    if (r < seen) {
-      sc = 0.f;
-      const unsigned* kr = reinterpret_cast<const unsigned*>(c.kc + ch + (size_t)r * (HD / 2));
-      for (int b = 0; b < T; ++b) {
-        float a = 0.f;
-        for (int lk = 0; lk < 4; ++lk) {
-          const unsigned w = kr[lk * T + b];
-          for (int j = 0; j < 8; ++j) a = __builtin_fmaf(kv4_grid((w >> (4 * j)) & 15u), qs[32 * b + 8 * lk + j], a);
-        }
-        sc = __builtin_fmaf(a, kv4_scale(c.ks[sh + (size_t)r * T + b]), sc);
-      }
-    }
-    float bm = sc;
-    for (int x = 1; x < 64; x <<= 1) bm = fmaxf(bm, __shfl_xor(bm, x));
-    if ((tid & 63) == 0) red[tid >> 6] = bm;
-    __syncthreads();
-    const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float al = m == -INFINITY ? 0.f : expf(m - mn);
-    const float p = r < seen ? expf(sc - mn) : 0.f;
-    ps[tid] = p;
-    float sum = wave_sum(p);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = sum;
-    __syncthreads();
-    l = l * al + ((red[0] + red[1]) + (red[2] + red[3]));
-    m = mn;
-    if (tid < HD) {
-      const int t = tid / 32, in = tid % 32;
-      o *= al;
-      for (int j = 0; j < min(256, seen - p0); ++j) {
-        const unsigned byte = c.vc[ch + kv4_value_offset<HD>(p0 + j, in / 2) + t];
-        const float x = kv4_grid((byte >> (4 * (tid & 1))) & 15u) * kv4_scale(c.vs[sh + (size_t)(p0 + j) * T + t]);
-        o = __builtin_fmaf(ps[j], x, o);
-      }
-    }
-    __syncthreads();
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// A query is carried as a sum of bf16 values that holds every bit of its type; a probability as enough of them that what
+// is cut lies beneath the rounding of the output: 24 bits for f32, 16 for the 16-bit types.
+template <class E>
+struct Parts;
+template <>
+struct Parts<float> {
+  static constexpr int q = 3, p = 3;
+};
+template <>
+struct Parts<__half> {
+  static constexpr int q = 2, p = 2;
+};
+template <>
+struct Parts<__hip_bfloat16> {
+  static constexpr int q = 1, p = 2;
+};
+
+// The high halves of two words as one (a in the low half): two bf16 values cut from two f32.
+__device__ __forceinline__ unsigned high_halves(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+// x minus its high 16 bits, exact.
+__device__ __forceinline__ float rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+
+// Eight f32 values as N bf16 operands whose sum they are (cut after 8 N bits).
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[N]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[k][i] = high_halves(r[2 * i], r[2 * i + 1]);
+    if (k + 1 < N)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = rest(r[i]);
   }
-  if (tid < HD) out[(size_t)i * ldo + (size_t)h * HD + tid] = from_f32<E>(o / l);
-  if (stats && tid == 0) stats[(size_t)i * nq + h] = make_float2(m, l);
 }
 
-// weights[g][r] += the softmax weights that row r received, a thread per row, queries and heads in order.
-template <int HD, class E>
-__global__ __launch_bounds__(256) void kv4_weights_simple_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq,
-                                                                 int n, float scale, const float2* __restrict__ stats,
-                                                                 float* __restrict__ weights, int64_t ldw) {
-  constexpr int T = HD / 32;
-  __shared__ float qs[HD];
-  const int g = blockIdx.y, grp = nq / c.nkv, tid = threadIdx.x, r = (int)blockIdx.x * 256 + tid;
-  const size_t ch = g * c.code_head(), sh = g * c.scale_head();
-  float acc = 0.f;
-  for (int i = 0; i < n; ++i)
-    for (int h = g * grp; h < (g + 1) * grp; ++h) {
-      __syncthreads();
-      if (tid < HD) qs[tid] = to_f32(q[(size_t)i * ldq + (size_t)h * HD + tid]) * scale;
-      __syncthreads();
-      if (r <= len - n + i) {
-        float sc = 0.f;
-        const unsigned* kr = reinterpret_cast<const unsigned*>(c.kc + ch + (size_t)r * (HD / 2));
-        for (int b = 0; b < T; ++b) {
-          float a = 0.f;
-          for (int lk = 0; lk < 4; ++lk) {
-            const unsigned w = kr[lk * T + b];
-            for (int j = 0; j < 8; ++j) a = __builtin_fmaf(kv4_grid((w >> (4 * j)) & 15u), qs[32 * b + 8 * lk + j], a);
-          }
-          sc = __builtin_fmaf(a, kv4_scale(c.ks[sh + (size_t)r * T + b]), sc);
-        }
-        const float2 st = stats[(size_t)i * nq + h];
-        acc += expf(sc - st.x) / st.y;
+// Scale byte `i` of a word as the f32 operand of the conversions, which take its exponent bits alone.
+__device__ __forceinline__ float scale_of(unsigned w, int i) {
+  return __uint_as_float(i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1);
+}
+template <int SEL>
+__device__ __forceinline__ unsigned fp4_pair(unsigned w, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+}
+__device__ __forceinline__ unsigned fp4_pair(unsigned w, float scale, int sel) {
+  switch (sel) {
+    case 0: return fp4_pair<0>(w, scale);
+    case 1: return fp4_pair<1>(w, scale);
+    case 2: return fp4_pair<2>(w, scale);
+    default: return fp4_pair<3>(w, scale);
+  }
+}
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// A lane's words of a tile of 32 rows.
+template <int HD>
+struct KeyWords {
+  static constexpr int T = HD / 32;
+  unsigned code[2][T];           // rows 16h + ln: dims 32b + 8lk .. +7
+  unsigned scale[2][(T + 3) / 4];
+  __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ks, int64_t row, int ln, int lk) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t r = row + 16 * h + ln;
+      const unsigned* p = reinterpret_cast<const unsigned*>(kc + (size_t)r * (HD / 2) + 4 * T * lk);
+#pragma unroll
+      for (int b = 0; b < T; ++b) code[h][b] = p[b];
+      if constexpr (T >= 4) {
+        const unsigned* q = reinterpret_cast<const unsigned*>(ks + (size_t)r * T);
+#pragma unroll
+        for (int b = 0; b < T / 4; ++b) scale[h][b] = q[b];
+      } else {
+        scale[h][0] = *reinterpret_cast<const unsigned short*>(ks + (size_t)r * T);
       }
     }
-  if (r < len) weights[(size_t)g * ldw + r] += acc;
+  }
+  // The matrix operand of block b of rows 16h + ln.
+  __device__ __forceinline__ u32x4 operand(int h, int b) const {
+    const float s = scale_of(scale[h][b / 4], b % 4);
+    const unsigned w = code[h][b];
+    return u32x4{fp4_pair<0>(w, s), fp4_pair<1>(w, s), fp4_pair<2>(w, s), fp4_pair<3>(w, s)};
+  }
+  // Bit r of the result: row 16h + r has a block that is not a number.
+  __device__ __forceinline__ unsigned bad_rows(int h) const {
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < T; ++b) bad |= ((scale[h][b / 4] >> (8 * (b % 4))) & 255u) == 255u;
+    return (unsigned)__ballot(bad) & 0xFFFFu;  // the four lanes of a row agree
+  }
+};
+template <int HD>
+struct ValueWords {
+  static constexpr int T = HD / 32;
+  unsigned code[2 * T];      // byte j·T + t
+  unsigned scale[2][T];      // rows 16h + 4lk + i: byte i·T + t
+  __device__ __forceinline__ void load(const uint8_t* vc, const uint8_t* vs, int64_t row, int lane) {
+    const uint8_t* p = vc + (size_t)row * (HD / 2) + 16 * lane;
+#pragma unroll
+    for (int c = 0; c < T / 2; ++c) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(p + 1024 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) code[4 * c + i] = w[i];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned* q = reinterpret_cast<const unsigned*>(vs + (size_t)(row + 16 * h + 4 * (lane >> 4)) * T);
+#pragma unroll
+      for (int i = 0; i < T; ++i) scale[h][i] = q[i];
+    }
+  }
+  // Dims 32t + 2ln and + 1 of slot j's row.
+  __device__ __forceinline__ unsigned pair(int j, int t) const {
+    const int o = j * T + t, s = (j & 3) * T + t;
+    return fp4_pair(code[o / 4], scale_of(scale[j >> 2][s / 4], s % 4), o % 4);
+  }
+  // The operands of dims 32t + 2ln (lo) and 32t + 2ln + 1 (hi) over the lane's eight slots.
+  __device__ __forceinline__ void operands(int t, u32x4& lo, u32x4& hi) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned a = pair(2 * i, t), b = pair(2 * i + 1, t);
+      lo[i] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+      hi[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    }
+  }
+  // Blocks that are not numbers count as zeros from here on (their codes are zeros); first[t] becomes the first row of
+  // the tile, at `row`, with such a block t, if that is earlier.
+  __device__ __forceinline__ void take_bad(int64_t row, int lk, int (&first)[T]) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int j = 7; j >= 0; --j) {
+        const int s = (j & 3) * T + t;
+        unsigned& w = scale[j >> 2][s / 4];
+        const bool bad = ((w >> (8 * (s % 4))) & 255u) == 255u;
+        const unsigned long long m = __ballot(bad);
+        if (bad) w ^= 0x80u << (8 * (s % 4));  // 127
+        if (m) first[t] = min(first[t], (int)row + 16 * (j >> 2) + 4 * (__builtin_ctzll(m) >> 4) + (j & 3));
+      }
+  }
+};
+
+// The query rows of a workgroup, row ρ = token · grp + head of the group, as operands in LDS: [row tile][block][part]
+// [lane][16 B], lane 16·lk + ln holding dims 32b + 8lk .. +7 of the tile's row ln.
+template <int HD, class E>
+__device__ __forceinline__ void stage_queries(u32x4* lds, int tiles, const E* __restrict__ q, int64_t ldq, int head0, int grp,
+                                              int row0, int rows, unsigned tid, unsigned nt) {
+  constexpr int T = HD / 32, QP = Parts<E>::q;
+  for (unsigned u = tid; u < (unsigned)(tiles * T * 64); u += nt) {
+    const int lane = (int)(u & 63u), b = (int)((u >> 6) % T), tile = (int)((u >> 6) / T);
+    const int rho = row0 + 16 * tile + (lane & 15);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (rho < rows) {
+      const E* p = q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD + 32 * b + 8 * (lane >> 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+    }
+    u32x4 part[QP];
+    split8<QP>(x, part);
+#pragma unroll
+    for (int k = 0; k < QP; ++k) lds[((tile * T + b) * QP + k) * 64 + lane] = part[k];
+  }
 }
 
-size_t kv4_attend_work(int hd, int n_head, int n) { return (size_t)n * n_head * sizeof(float2); }
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Where a call's results go: the output itself (nch = 1) or a record (m, l, o[HD]) per row and chunk of positions.
+struct AttendOut {
+  float* rec;     // [n][nq][nch][2 + HD]
+  float2* stats;  // [n][nq] (m, l), or null
+};
+
+// Causal attention of the n·grp query rows of a key/value head on the matrix cores.  Scores as S^T = K · Q^T: the operand
+// of the keys is the dequantised block itself (a block of 32 dims is one 16x16x32 instruction), that of the queries comes from LDS;
+// lane (ln, lk) gets the scores of row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that order, its
+// part of the operand P of O += P · V.  Dequantising is exact, queries and probabilities are sums of bf16 operands
+// (Parts), so products are those of f32 values and the sums f32.
+//
+// ROWS16: up to 16 rows; the workgroup's four waves take the chunk's tiles of 32 positions in turn and their results meet in
+// LDS.  Otherwise a workgroup has 64 rows, 16 a wave, and every wave all of the chunk's tiles.
+// Grid: (row tiles x key/value heads x chunks), 256 threads.
+template <int HD, class E, bool ROWS16>
+__global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq, int n,
+                                                            float scale, int csz, int nch, AttendOut dst, E* __restrict__ out,
+                                                            int64_t ldo) {
+  constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p;
+  extern __shared__ __align__(16) uint8_t smem[];
+  u32x4* qs = reinterpret_cast<u32x4*>(smem);
+  const int grp = nq / c.nkv, rows = n * grp, ntile = ROWS16 ? 1 : (rows + 63) / 64;
+  const int pairs = c.nkv * nch, pair = (int)blockIdx.x % pairs;
+  const int tile = ntile - 1 - (int)blockIdx.x / pairs, g = pair % c.nkv, z = pair / c.nkv;
+  const unsigned tid = threadIdx.x, lane = tid & 63u, w = tid >> 6;
+  const int ln = (int)(lane & 15u), lk = (int)(lane >> 4);
+  const int row0 = ROWS16 ? 0 : 64 * tile, wrow = ROWS16 ? 0 : row0 + 16 * (int)w;
+  const int before = len - n;
+  // the positions that any row of the workgroup (of the wave) sees in the chunk
+  const int last_row = min(ROWS16 ? rows : row0 + 64, rows) - 1, wlast = min(wrow + 16, rows) - 1;
+  const int pbeg = z * csz, pend = min(min((z + 1) * csz, len), before + last_row / grp + 1);
+  const int wend = wrow < rows ? min(pend, before + wlast / grp + 1) : pbeg;
+  const int wmin = wrow < rows ? before + wrow / grp + 1 : 0;  // what the wave's first row sees
+  const int rho = wrow + ln;
+  const int ctx = rho < rows ? before + rho / grp + 1 : 0;
+  if (pbeg < pend) stage_queries<HD, E>(qs, ROWS16 ? 1 : 4, q, ldq, g * grp, grp, row0, rows, tid, 256);
+  __syncthreads();
+  const u32x4* qw = qs + (ROWS16 ? 0 : (int)w * T * QP * 64) + lane;
+  f32x4 o[2 * T];
+#pragma unroll
+  for (int t = 0; t < 2 * T; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  int first[T];  // first position seen whose value block t is not a number
+#pragma unroll
+  for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
+  const uint8_t *kc = c.kc + g * c.code_head(), *vc = c.vc + g * c.code_head();
+  const uint8_t *ks = c.ks + g * c.scale_head(), *vs = c.vs + g * c.scale_head();
+  const uint8_t* bad = c.bad + (size_t)g * (c.cap / kKv4Tile);
+  const int step = ROWS16 ? 128 : 32;
+  int p0 = pbeg + (ROWS16 ? 32 * (int)w : 0);
+  KeyWords<HD> kw;
+  ValueWords<HD> vw;
+  if (p0 < wend) {
+    kw.load(kc, ks, p0, ln, lk);
+    vw.load(vc, vs, p0, (int)lane);
+  }
+  for (; p0 < wend; p0 += step) {
+    const bool odd = bad[p0 >> 5] != 0;
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int b = 0; b < T; ++b) {
+      const u32x4 k0 = kw.operand(0, b), k1 = kw.operand(1, b);
+#pragma unroll
+      for (int k = 0; k < QP; ++k) {
+        const u32x4 qq = qw[(b * QP + k) * 64];
+        s[0] = mfma(k0, qq, s[0]);
+        s[1] = mfma(k1, qq, s[1]);
+      }
+    }
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * scale;
+    if (odd) {
+      const unsigned b0 = kw.bad_rows(0), b1 = kw.bad_rows(1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (((j < 4 ? b0 : b1) >> (4 * lk + (j & 3))) & 1u) x[j] = __builtin_nanf("");
+    }
+    const int pn = p0 + step < wend ? p0 + step : p0;
+    kw.load(kc, ks, pn, ln, lk);
+    if (p0 + 32 > wmin) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
+    }
+    float bm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    bm = fmaxf(bm, __shfl_xor(bm, 16));
+    bm = fmaxf(bm, __shfl_xor(bm, 32));
+    const float mn = fmaxf(m, bm);
+    // a row that has seen nothing keeps m = -inf: its factor is 1 by definition, and its probabilities 0
+    const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    float p[8], ps = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
+      ps += p[j];
+    }
+    ps += __shfl_xor(ps, 16);
+    ps += __shfl_xor(ps, 32);
+    l = l * al + ps;
+    m = mn;
+    // the O rows of this lane are 4lk + i: their factors live in lanes 4lk + i
+    if (__ballot(al != 1.f)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = __shfl(al, 4 * lk + i);
+#pragma unroll
+        for (int t = 0; t < 2 * T; ++t) o[t][i] *= a;
+      }
+    }
+    u32x4 pp[PP];
+    split8<PP>(p, pp);
+    if (odd) vw.take_bad(p0, lk, first);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      u32x4 lo, hi;
+      vw.operands(t, lo, hi);
+#pragma unroll
+      for (int k = 0; k < PP; ++k) {
+        o[2 * t] = mfma(pp[k], lo, o[2 * t]);
+        o[2 * t + 1] = mfma(pp[k], hi, o[2 * t + 1]);
+      }
+    }
+    vw.load(vc, vs, pn, (int)lane);
+  }
+  // rows that see a value which is not a number
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int ci = __shfl(ctx, 4 * lk + i);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      if (first[t] < ci) o[2 * t][i] = o[2 * t + 1][i] = __builtin_nanf("");
+  }
+  if constexpr (ROWS16) {
+    // the four waves' results: each row's largest maximum, then the sums at it
+    float* ms = reinterpret_cast<float*>(smem);  // [wave][16], over the queries, which every wave has read
+    float* os = ms + 128;                        // [wave][row][HD]
+    __syncthreads();
+    if (lk == 0) {
+      ms[16 * w + ln] = m;
+      ms[64 + 16 * w + ln] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        *reinterpret_cast<float2*>(os + ((size_t)w * 16 + 4 * lk + i) * HD + 32 * t + 2 * ln) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
+    __syncthreads();
+    for (unsigned u = tid; u < (unsigned)(rows * (HD / 4)); u += 256) {
+      const int r = (int)(u / (HD / 4)), d = 4 * (int)(u % (HD / 4));
+      const float M = fmaxf(fmaxf(ms[r], ms[16 + r]), fmaxf(ms[32 + r], ms[48 + r]));
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float mk = ms[16 * k + r], e = mk == -INFINITY && M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * kLog2e);
+        const float4 v = *reinterpret_cast<const float4*>(os + ((size_t)k * 16 + r) * HD + d);
+        L = __builtin_fmaf(ms[64 + 16 * k + r], e, L);
+        O.x = __builtin_fmaf(v.x, e, O.x);
+        O.y = __builtin_fmaf(v.y, e, O.y);
+        O.z = __builtin_fmaf(v.z, e, O.z);
+        O.w = __builtin_fmaf(v.w, e, O.w);
+      }
+      const size_t row = (size_t)(r / grp) * nq + g * grp + r % grp;
+      if (nch == 1) {
+        E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + d;
+        y[0] = from_f32<E>(O.x / L);
+        y[1] = from_f32<E>(O.y / L);
+        y[2] = from_f32<E>(O.z / L);
+        y[3] = from_f32<E>(O.w / L);
+        if (dst.stats && d == 0) dst.stats[row] = make_float2(M, L);
+      } else {
+        float* rr = dst.rec + (row * nch + z) * (2 + HD);
+        if (d == 0) *reinterpret_cast<float2*>(rr) = make_float2(M, L);
+        *reinterpret_cast<float2*>(rr + 2 + d) = make_float2(O.x, O.y);
+        *reinterpret_cast<float2*>(rr + 4 + d) = make_float2(O.z, O.w);
+      }
+    }
+    return;
+  }
+  if (lk == 0 && rho < rows) {
+    const size_t row = (size_t)(rho / grp) * nq + g * grp + rho % grp;
+    if (nch > 1) *reinterpret_cast<float2*>(dst.rec + (row * nch + z) * (2 + HD)) = make_float2(m, l);
+    else if (dst.stats) dst.stats[row] = make_float2(m, l);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = wrow + 4 * lk + i;
+    const float li = __shfl(l, 4 * lk + i);
+    if (r >= rows) continue;
+    if (nch == 1) {
+      E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + 2 * ln;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        y[32 * t] = from_f32<E>(o[2 * t][i] / li);
+        y[32 * t + 1] = from_f32<E>(o[2 * t + 1][i] / li);
+      }
+    } else {
+      float* rr = dst.rec + (((size_t)(r / grp) * nq + g * grp + r % grp) * nch + z) * (2 + HD) + 2 + 2 * ln;
+#pragma unroll
+      for (int t = 0; t < T; ++t) *reinterpret_cast<float2*>(rr + 32 * t) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
+    }
+  }
+}
+
+// The chunks' records of a row (query blockIdx.x, head blockIdx.y) as its output and statistics: 4 HD threads, the
+// chunks in four quarters.  A chunk whose positions the row does not see has l = 0, m = -inf and zeros.
+template <int HD, class E>
+__global__ __launch_bounds__(4 * HD) void kv4_merge_kernel(AttendOut src, int nch, int nq, E* __restrict__ out, int64_t ldo) {
+  __shared__ float fac[kKv4MaxChunks], red[4][HD + 1], mx[4 * HD / 64];
+  const unsigned tid = threadIdx.x, d = tid % HD, part = tid / HD;
+  const size_t row = (size_t)blockIdx.x * nq + blockIdx.y;
+  const float* rec = src.rec + row * nch * (2 + HD);
+  float m = -INFINITY;
+  for (int z = (int)tid; z < nch; z += 4 * HD) m = fmaxf(m, rec[(size_t)z * (2 + HD)]);
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  if ((tid & 63u) == 0) mx[tid >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4 * HD / 64; ++k) m = fmaxf(m, mx[k]);
+  for (int z = (int)tid; z < nch; z += 4 * HD) {
+    const float mz = rec[(size_t)z * (2 + HD)];
+    fac[z] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mz - m) * kLog2e);
+  }
+  __syncthreads();
+  const int q4 = (nch + 3) / 4, z0 = (int)part * q4, z1 = min(nch, z0 + q4);
+  float O = 0.f, L = 0.f;
+  for (int z = z0; z < z1; z += 8) {
+    float v[8], lv[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float* rr = rec + (size_t)min(z + k, z1 - 1) * (2 + HD);
+      v[k] = rr[2 + d];
+      lv[k] = rr[1];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (z + k < z1) {
+        O = __builtin_fmaf(v[k], fac[z + k], O);
+        L = __builtin_fmaf(lv[k], fac[z + k], L);
+      }
+  }
+  red[part][d] = O;
+  if (d == 0) red[part][HD] = L;
+  __syncthreads();
+  if (part == 0) {
+    O = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
+    L = (red[0][HD] + red[1][HD]) + (red[2][HD] + red[3][HD]);
+    out[(size_t)blockIdx.x * ldo + (size_t)blockIdx.y * HD + d] = from_f32<E>(O / L);
+    if (src.stats && d == 0) src.stats[row] = make_float2(m, L);
+  }
+}
+
+// weights[g][r] += Σ over the group's query rows ρ of exp(s_ρr - m_ρ) / l_ρ: a wave holds the operands of 16·PT rows of keys and
+// walks the query rows 16 at a time (staged for the workgroup's four waves in LDS), a lane adding up its four positions
+// of each 16 over the query rows ln, in order; the sixteen lanes of a position are summed at the end.
+// Grid (ceil(len / 64PT), nkv), 256 threads.
+template <int HD, class E, int PT>
+__global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq, int n,
+                                                             float scale, const float2* __restrict__ stats,
+                                                             float* __restrict__ weights, int64_t ldw) {
+  constexpr int T = HD / 32, QP = Parts<E>::q;
+  __shared__ u32x4 qs[T * QP * 64];
+  const int g = blockIdx.y, grp = nq / c.nkv, rows = n * grp, before = len - n;
+  const unsigned tid = threadIdx.x, lane = tid & 63u, w = tid >> 6;
+  const int ln = (int)(lane & 15u), lk = (int)(lane >> 4);
+  const int pw = (int)blockIdx.x * 64 * PT + 16 * PT * (int)w;  // the wave's first position
+  const int pblk = (int)blockIdx.x * 64 * PT;
+  const uint8_t *kc = c.kc + g * c.code_head(), *ks = c.ks + g * c.scale_head();
+  u32x4 kop[PT][T];
+  unsigned nan[PT];
+#pragma unroll
+  for (int u = 0; u < PT; u += (PT == 1 ? 1 : 2)) {
+    KeyWords<HD> kw;
+    // whole tiles of 32 rows; past the last one (a wave with nothing to do, or half a tile) the first is read instead
+    const int r = pw + 16 * u, base = r < len ? r & ~31 : 0;
+    kw.load(kc, ks, base, ln, lk);
+    const int h0 = r < len ? (r >> 4) & 1 : 0;
+#pragma unroll
+    for (int b = 0; b < T; ++b) {
+      if constexpr (PT == 1) {
+        kop[u][b] = h0 ? kw.operand(1, b) : kw.operand(0, b);
+      } else {
+        kop[u][b] = kw.operand(0, b);
+        kop[u + 1][b] = kw.operand(1, b);
+      }
+    }
+    if constexpr (PT == 1) {
+      nan[u] = h0 ? kw.bad_rows(1) : kw.bad_rows(0);
+    } else {
+      nan[u] = kw.bad_rows(0);
+      nan[u + 1] = kw.bad_rows(1);
+    }
+  }
+  float acc[PT][4];
+#pragma unroll
+  for (int u = 0; u < PT; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[u][i] = 0.f;
+  // the first query row that sees the workgroup's first position
+  const int r0 = max(0, pblk - before) * grp / 16 * 16;
+  for (int row = r0; row < rows; row += 16) {
+    __syncthreads();
+    stage_queries<HD, E>(qs, 1, q, ldq, g * grp, grp, row, rows, tid, 256);
+    __syncthreads();
+    const int rho = row + ln;
+    const bool has = rho < rows;
+    const int ctx = has ? before + rho / grp + 1 : 0;
+    float2 st = make_float2(0.f, 1.f);
+    if (has) st = stats[(size_t)(rho / grp) * nq + g * grp + rho % grp];
+    const float inv = 1.f / st.y;
+    f32x4 s[PT];
+#pragma unroll
+    for (int u = 0; u < PT; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < T; ++b)
+#pragma unroll
+      for (int k = 0; k < QP; ++k) {
+        const u32x4 qq = qs[(b * QP + k) * 64 + lane];
+#pragma unroll
+        for (int u = 0; u < PT; ++u) s[u] = mfma(kop[u][b], qq, s[u]);
+      }
+#pragma unroll
+    for (int u = 0; u < PT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = s[u][i] * scale;
+        if (nan[u] && ((nan[u] >> (4 * lk + i)) & 1u)) x = __builtin_nanf("");
+        const float p = __builtin_amdgcn_exp2f((x - st.x) * kLog2e) * inv;
+        if (pw + 16 * u + 4 * lk + i < ctx) acc[u][i] += p;
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < PT; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a = acc[u][i];
+      a += __shfl_xor(a, 1);
+      a += __shfl_xor(a, 2);
+      a += __shfl_xor(a, 4);
+      a += __shfl_xor(a, 8);
+      const int r = pw + 16 * u + 4 * lk + i;
+      if (ln == 0 && r < len) weights[(size_t)g * ldw + r] += a;
+    }
+}
+
+// Chunks of positions that a call's row tiles are spread over, at most: enough workgroups to fill the device.
+static int attend_max_chunks(int n, int n_head, int nkv) {
+  const int rows = n * (n_head / nkv);
+  const int tiles = (rows <= 16 ? 1 : (rows + 63) / 64) * nkv;
+  return std::max(1, std::min(kKv4MaxChunks, (rows <= 16 ? 512 : 256) / tiles));
+}
+
+size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
+  const size_t rows = (size_t)n * n_head, nch = (size_t)attend_max_chunks(n, n_head, c.nkv);
+  return (rows * sizeof(float2) + 15) / 16 * 16 + (nch > 1 ? rows * nch * (size_t)(2 + c.hd) * sizeof(float) : 0);
+}
+
+template <int HD, class E, bool ROWS16>
+constexpr size_t attend_lds() {
+  constexpr size_t queries = (size_t)(ROWS16 ? 1 : 4) * (HD / 32) * Parts<E>::q * 1024;
+  constexpr size_t merge = ROWS16 ? 512 + 4 * 16 * HD * 4 : 0;
+  return queries > merge ? queries : merge;
+}
+
+// Dynamic-LDS limits, set once before any launch or capture.
+int prepare_kv4_kernels() {
+  static std::mutex mu;
+  static bool done = false;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done) return DZ_OK;
+  for (int hd : {64, 128, 256})
+    for (int type : {DZ_F32, DZ_F16, DZ_BF16}) {
+      const int rc = with_head_dim(hd, [&](auto D) {
+        constexpr int HD = decltype(D)::value;
+        return with_type(type, [&](auto* e) -> int {
+          using E = std::remove_pointer_t<decltype(e)>;
+          DZ_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kv4_attend_kernel<HD, E, true>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, true>()));
+          DZ_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kv4_attend_kernel<HD, E, false>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, false>()));
+          return DZ_OK;
+        });
+      });
+      if (rc) return rc;
+    }
+  done = true;
+  return DZ_OK;
+}
 
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s) {
+  const int rows = n * (n_head / c.nkv), unit = rows <= 16 ? 128 : 32;
+  const int most = attend_max_chunks(n, n_head, c.nkv);
+  const int csz = ((len + most - 1) / most + unit - 1) / unit * unit, nch = (len + csz - 1) / csz;
   return with_head_dim(c.hd, [&](auto D) {
     constexpr int HD = decltype(D)::value;
     return with_type(type, [&](auto* e) -> int {
       using E = std::remove_pointer_t<decltype(e)>;
+      AttendOut dst;
       float2* stats = static_cast<float2*>(work);
-      kv4_attend_simple_kernel<HD, E><<<dim3((unsigned)n, (unsigned)n_head), 256, 0, s>>>(
-          c, len, (const E*)q, ldq, n_head, n, scale, weights ? stats : nullptr, (E*)out, ldo);
+      dst.stats = weights ? stats : nullptr;
+      dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
+      if (rows <= 16)
+        kv4_attend_kernel<HD, E, true><<<dim3((unsigned)(c.nkv * nch)), 256, attend_lds<HD, E, true>(), s>>>(
+            c, len, (const E*)q, ldq, n_head, n, scale, csz, nch, dst, (E*)out, ldo);
+      else
+        kv4_attend_kernel<HD, E, false><<<dim3((unsigned)((rows + 63) / 64 * c.nkv * nch)), 256, attend_lds<HD, E, false>(), s>>>(
+            c, len, (const E*)q, ldq, n_head, n, scale, csz, nch, dst, (E*)out, ldo);
       DZ_HIP_CHECK(hipGetLastError());
+      if (nch > 1) {
+        kv4_merge_kernel<HD, E><<<dim3((unsigned)n, (unsigned)n_head), 4 * HD, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
+        DZ_HIP_CHECK(hipGetLastError());
+      }
       if (weights) {
-        kv4_weights_simple_kernel<HD, E><<<dim3((unsigned)((len + 255) / 256), (unsigned)c.nkv), 256, 0, s>>>(
-            c, len, (const E*)q, ldq, n_head, n, scale, stats, weights, ldw);
+        const int64_t tiles = ((int64_t)len + 15) / 16 * c.nkv;
+        auto run = [&](auto P) {
+          constexpr int PT = decltype(P)::value;
+          kv4_weights_kernel<HD, E, PT><<<dim3((unsigned)((len + 64 * PT - 1) / (64 * PT)), (unsigned)c.nkv), 256, 0, s>>>(
+              c, len, (const E*)q, ldq, n_head, n, scale, stats, weights, ldw);
+        };
+        if (tiles >= 16 * 256) run(std::integral_constant<int, 4>{});
+        else if (tiles >= 8 * 256) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, 1>{});
         DZ_HIP_CHECK(hipGetLastError());
       }
       return DZ_OK;
@@ -374,7 +876,8 @@ int dz_kv4_create(int kv_heads, int head_dim, int capacity, dz_kv4** out) {
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return set_error(DZ_ERR_UNSUPPORTED, "4-bit cache: head_dim %d (64, 128 or 256)", head_dim);
   if (capacity < 1 || capacity > (1 << 30)) return set_error(DZ_ERR_TENSOR, "4-bit cache: capacity %d", capacity);
-  if (int rc = ensure_device()) return rc;
+  int rc = ensure_device();
+  if (rc || (rc = prepare_kv4_kernels())) return rc;
   dz_kv4* c = new (std::nothrow) dz_kv4();
   if (!c) return set_error(DZ_ERR_MODEL, "out of memory");
   const int cap = (capacity + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
@@ -442,7 +945,7 @@ int dz_kv4_read_dev(const dz_kv4* c, int start, int n, float* k, float* v, void*
 }
 
 size_t dz_kv4_attend_work_bytes(const dz_kv4* c, int n_head, int n) {
-  return !c || n_head < 1 || n < 1 ? 0 : kv4_attend_work(c->v.hd, n_head, n);
+  return !c || n_head < 1 || n < 1 || n_head % c->v.nkv ? 0 : kv4_attend_work(c->v, n_head, n);
 }
 
 int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
