@@ -9,17 +9,17 @@
 
 namespace dz {
 
-constexpr int kLogprobTop = 64;     // most alternatives
-constexpr int kLpThreads = 256;
-constexpr int kLpVals = 16;         // logits of a thread and step
-constexpr int kLpStep = kLpThreads * kLpVals;
-constexpr int kLpMaxSplits = 64;    // parts of a row
-constexpr int kLpCand = kLogprobTop * kLpVals + 2 * kLogprobTop;  // candidates in LDS (see logprobs_kernel)
+constexpr int kLogprobTop = 64;   // most alternatives: a wave's lanes
+constexpr int kLpVals = 16;       // logits of a lane and step
+constexpr int kLpStep = 64 * kLpVals;
+constexpr int kLpMaxParts = 256;  // parts of a row: the join's threads
+constexpr int kLpKeep = 2 * kLogprobTop + 16;       // a longer list is cut to the best
+constexpr int kLpCand = kLpKeep + kLpStep;          // ... which one step can outgrow by this much
 
 // A logit and its id as one word whose unsigned order is "larger value first, then lower id", NaN below -inf.
 __device__ __forceinline__ uint64_t logit_key(float v, int i) {
-  const uint64_t id = (unsigned)~(unsigned)i;
-  return v != v ? id : (cand_key(v, i) & 0xFFFFFFFF00000000ull) | id;
+  const unsigned u = __float_as_uint(v + 0.f), o = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+  return (uint64_t)(v != v ? 0u : o) << 32 | (unsigned)~(unsigned)i;
 }
 
 // Σ e^(x-m) (z) and Σ e^(x-m) (x-m) (a) over some logits whose largest is m.
@@ -39,85 +39,71 @@ __device__ __forceinline__ LogitSums join(const LogitSums& x, const LogitSums& y
   return LogitSums{M, p.z + q.z, p.a + q.a};
 }
 
-// N consecutive elements from an address of the element's own alignment.
-template <class E, int N>
-__device__ __forceinline__ void load_elems(const E* p, float (&x)[N]) {
+// 16 bytes from an address of the element's own alignment, and the values that they are.
+template <class E>
+__device__ __forceinline__ u32x4 load16(const E* p) {
   struct __attribute__((packed, aligned(sizeof(E)))) Raw {
-    E e[N];
+    u32x4 w;
   };
-  const Raw r = *reinterpret_cast<const Raw*>(p);
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = to_f32(r.e[i]);
+  return reinterpret_cast<const Raw*>(p)->w;
 }
+template <class E, int R>
+__device__ __forceinline__ void values_of(u32x4 w, float* x) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if constexpr (R == 4) x[i] = __uint_as_float(w[i]);
+    else x[i] = to_f32(__builtin_bit_cast(E, (uint16_t)(w[i / 2] >> (16 * (i & 1)))));
+  }
+}
+
+// Wave-wide (one wave a workgroup, so LDS needs no barrier but the compiler's).
+__device__ __forceinline__ void lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // The `top` largest of the cnt (>= top) distinct keys in c, in order, to c[0 .. top): every key counts the larger ones.
-// The workgroup's threads call it together; cnt <= kLpCand.
-__device__ __forceinline__ void prune(uint64_t* c, int cnt, int top, int tid) {
-  constexpr int N = (kLpCand + kLpThreads - 1) / kLpThreads;
-  uint64_t mine[N];
-  int rank[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int i = tid + k * kLpThreads;
-    rank[k] = kLpCand;
-    if (i < cnt) {
-      mine[k] = c[i];
-      int r = 0;
-      for (int j = 0; j < cnt; ++j) r += c[j] > mine[k] ? 1 : 0;
-      rank[k] = r;
-    }
+__device__ __forceinline__ void prune(uint64_t* c, int cnt, int top, int lane) {
+  // in rounds of 64: a key's rank is known before any is moved, so the best of all go to a second place first
+  uint64_t best = 0;  // lane r: the key of rank r
+  __shared__ uint64_t out[kLogprobTop];
+  for (int i0 = 0; i0 < cnt; i0 += 64) {
+    const uint64_t mine = i0 + lane < cnt ? c[i0 + lane] : 0;
+    int r = mine ? 0 : kLogprobTop;
+    for (int j = 0; j < cnt; ++j) r += c[j] > mine ? 1 : 0;
+    if (r < top) out[r] = mine;
   }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (rank[k] < top) c[rank[k]] = mine[k];
-  __syncthreads();
+  lds_fence();
+  if (lane < top) best = out[lane];
+  if (lane < top) c[lane] = best;
+  lds_fence();
 }
 
-// One part of a row: its sums and its `top` best keys.  A pass over the logits, 4096 a step: each thread keeps its own
-// running maximum and sums; keys above the part's top-th best so far go to a list in LDS.  A step in which more than 64
-// threads have such a key (the first one; rows that keep rising) first raises the bound to the top-th largest of the threads'
-// own best keys of the step: only threads whose best is above it can then add any, so that a step adds at most
-// 64 x 16 keys to the 64 that a pruned list holds.
-// Grid (parts, n), 256 threads.  part -> sums[row][part], keys[row][part][top].
+// One part of a row by one wave: its sums and its `top` best keys in order.  A pass over the logits, 1024 a step, the next
+// step's on their way: each lane keeps its own running maximum and sums.  Keys above the part's top-th best so far
+// (`bound`) go to a list in LDS; a lane looks at its keys only where the largest of its logits reaches the bound's value.
+// Where more than 32 lanes do (the first step; rows that keep rising) the bound first rises to the top-th largest of the
+// lanes' own best keys: only lanes whose best is above it can then add any.
+// Bound by the loads at many rows: 16 exponentials and about 120 other instructions a lane and step of 4 KB of f32.
+// Grid (parts, n), 64 threads.
 template <class E, bool TOP>
-__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const E* __restrict__ x, int64_t ld, int vocab, int per, int top,
-                                                              LogitSums* __restrict__ sums, uint64_t* __restrict__ keys) {
-  __shared__ uint64_t cand[TOP ? kLpCand : 1], best[TOP ? kLpThreads : 1];
-  __shared__ int s_cnt, s_n;
-  __shared__ uint64_t s_bound;
-  __shared__ LogitSums red[kLpThreads / 64];
-  const int tid = threadIdx.x, part = blockIdx.x, parts = gridDim.x;
+__global__ __launch_bounds__(64) void logprobs_kernel(const E* __restrict__ x, int64_t ld, int vocab, int per, int top,
+                                                      LogitSums* __restrict__ sums, uint64_t* __restrict__ keys) {
+  constexpr int R = 16 / sizeof(E);  // a lane's logits: runs of 16 bytes, the wave's runs one after another
+  __shared__ uint64_t cand[TOP ? kLpCand : 1];
+  const int lane = threadIdx.x, part = blockIdx.x, parts = gridDim.x;
   const size_t row = blockIdx.y;
   x += row * (size_t)ld;
   const int beg = part * per, end = min(vocab, beg + per);
   LogitSums s{-INFINITY, 0.f, 0.f};
   uint64_t bound = 0;  // keys up to this one are not among the part's best
-  if (TOP && tid == 0) s_cnt = 0;
-  float v[kLpVals];
-  auto load = [&](int c0) {
-    // a thread's logits: runs of 16 bytes, the workgroup's runs one after another
-    constexpr int R = 16 / sizeof(E);
-#pragma unroll
-    for (int k = 0; k < kLpVals / R; ++k) {
-      const int c = c0 + (k * kLpThreads + tid) * R;
-      float r[R];
-      if (c + R <= end) {
-        load_elems(x + c, r);
-      } else {
-#pragma unroll
-        for (int i = 0; i < R; ++i) r[i] = c + i < end ? to_f32(x[c + i]) : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i) v[k * R + i] = r[i];
-    }
+  float floor = 0.f;   // only larger logits have keys above it, where it is that of a number
+  bool any = true;     // it is none: every key is looked at
+  int cnt = 0;
+  auto raise = [&](uint64_t key) {
+    bound = key;
+    floor = cand_of(key).v;
+    any = key <= (uint64_t)0x00800000u << 32;  // NaN, nothing, or -inf
   };
-  auto index = [&](int c0, int i) {
-    constexpr int R = 16 / sizeof(E);
-    return c0 + ((i / R) * kLpThreads + tid) * R + i % R;
-  };
-  for (int c0 = beg; c0 < end; c0 += kLpStep) {
-    load(c0);
+  // the logits of the step at c0
+  auto step = [&](int c0, const float (&v)[kLpVals]) {
     float vm = v[0];
 #pragma unroll
     for (int i = 1; i < kLpVals; ++i) vm = fmaxf(vm, v[i]);
@@ -135,123 +121,179 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(const E* __restric
     s.z += z;
     s.a += a;
     if constexpr (TOP) {
-      uint64_t top_key = 0;
+      const unsigned long long over = __ballot(any || vm > floor);
+      if (over) {
+        auto key_at = [&](int i) {
+          const int c = c0 + ((i / R) * 64 + lane) * R + i % R;
+          return c < end ? logit_key(v[i], c) : (uint64_t)0;
+        };
+        if (__popcll(over) > 32) {
+          uint64_t best = 0;
 #pragma unroll
-      for (int i = 0; i < kLpVals; ++i) {
-        const int c = index(c0, i);
-        const uint64_t k = c < end ? logit_key(v[i], c) : 0;
-        top_key = k > top_key ? k : top_key;
-      }
-      if (tid == 0) s_n = 0;
-      __syncthreads();  // also: the list is whole
-      const unsigned long long over = __ballot(top_key > bound);
-      if ((tid & 63) == 0 && over) atomicAdd(&s_n, __popcll(over));
-      __syncthreads();
-      const int n = s_n;
-      if (n == 0) continue;
-      if (n > kLogprobTop) {
-        best[tid] = top_key;
-        if (tid == 0) s_bound = bound;
-        __syncthreads();
-        int r = 0;
-        for (int j = 0; j < kLpThreads; ++j) r += best[j] > top_key ? 1 : 0;
-        // threads without a logit share the key 0: no rank is top - 1 then, and the bound stays
-        if (r == top - 1 && top_key > bound) s_bound = top_key - 1;
-        __syncthreads();
-        bound = s_bound;
-      }
+          for (int i = 0; i < kLpVals; ++i) {
+            const uint64_t k = key_at(i);
+            best = k > best ? k : best;
+          }
+          cand[cnt + lane] = best;  // behind the list
+          lds_fence();
+          int r = best > bound ? 0 : 64;
+#pragma unroll 8
+          for (int j = 0; j < 64; ++j) r += cand[cnt + j] > best ? 1 : 0;
+          lds_fence();
+          const unsigned long long at = __ballot(r == top - 1);  // none where fewer lanes than top are above the bound
+          if (at) {
+            const int l = __builtin_ctzll(at);
+            const uint64_t k = ((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(best >> 32), l) << 32) |
+                               (unsigned)__builtin_amdgcn_readlane((int)(unsigned)best, l);
+            raise(k - 1);
+            // an equal logit of a lower id in this step is above the bound: the next number down (below 0, past -0)
+            floor = floor == 0.f ? -__uint_as_float(1u) : cand_of(bound - ((uint64_t)1 << 32)).v;
+          }
+        }
 #pragma unroll
-      for (int i = 0; i < kLpVals; ++i) {
-        const int c = index(c0, i);
-        const uint64_t k = c < end ? logit_key(v[i], c) : 0;
-        if (k > bound) cand[atomicAdd(&s_cnt, 1)] = k;
-      }
-      __syncthreads();
-      const int cnt = s_cnt;
-      if (cnt >= top) {
-        prune(cand, cnt, top, tid);
-        bound = cand[top - 1];
-        if (tid == 0) s_cnt = top;
+        for (int i = 0; i < kLpVals; ++i) {
+          if (!__ballot(any || v[i] > floor)) continue;
+          const uint64_t k = key_at(i);
+          const unsigned long long in = __ballot(k > bound);
+          if (k > bound) cand[cnt + __popcll(in & ((1ull << lane) - 1))] = k;
+          cnt += __popcll(in);
+        }
+        lds_fence();
+        if (cnt > kLpKeep || (any && cnt >= top)) {
+          prune(cand, cnt, top, lane);
+          cnt = top;
+          raise(cand[top - 1]);
+        } else if (!any) {
+          floor = cand_of(bound).v;  // later ids do not win ties
+        }
       }
     }
+  };
+  // whole steps, whose loads need no bounds and are requested a step ahead; then what is left
+  const int whole = beg + (end - beg) / kLpStep * kLpStep;
+  if (beg < whole) {
+    const E* p = x + lane * R;
+    u32x4 next[kLpVals / R];
+#pragma unroll
+    for (int k = 0; k < kLpVals / R; ++k) next[k] = load16(p + beg + k * 64 * R);
+    for (int c0 = beg; c0 < whole; c0 += kLpStep) {
+      float v[kLpVals];
+#pragma unroll
+      for (int k = 0; k < kLpVals / R; ++k) values_of<E, R>(next[k], v + k * R);
+      const int cn = min(c0 + kLpStep, whole - kLpStep);
+#pragma unroll
+      for (int k = 0; k < kLpVals / R; ++k) next[k] = load16(p + cn + k * 64 * R);
+      step(c0, v);
+    }
   }
-  // the threads' sums, lanes and then waves in a fixed order
+  if (whole < end) {
+    float v[kLpVals];
+#pragma unroll
+    for (int i = 0; i < kLpVals; ++i) {
+      const int c = whole + ((i / R) * 64 + lane) * R + i % R;
+      const float u = to_f32(x[min(c, end - 1)]);
+      v[i] = c < end ? u : -INFINITY;
+    }
+    step(whole, v);
+  }
+  // the lanes' sums in a fixed order
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const LogitSums y{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.a, o)};
     s = join(s, y);
   }
-  if ((tid & 63) == 0) red[tid >> 6] = s;
-  __syncthreads();
-  if (tid == 0) {
-    s = join(join(red[0], red[1]), join(red[2], red[3]));
-    sums[row * parts + part] = s;
-  }
+  if (lane == 0) sums[row * parts + part] = s;
   if constexpr (TOP) {
-    const int cnt = s_cnt;
-    if (tid < top) keys[(row * parts + part) * top + tid] = tid < cnt ? cand[tid] : 0;  // a part of fewer logits than top: unordered
+    // a part of fewer logits than top keeps what it has, in order, and zeros
+    for (int i = cnt + lane; i < top; i += 64) cand[i] = 0;
+    lds_fence();
+    prune(cand, max(cnt, top), top, lane);
+    if (lane < top) keys[(row * parts + part) * top + lane] = lane < cnt ? cand[lane] : 0;
   }
 }
 
-// The parts of a row as its results.  Grid (n), 256 threads.
+// The parts of a row as its results.  Of the parts' lists, each in order, only those whose first key is among the `top`
+// largest first keys can hold one of the row's best, and only keys not below the last of those: they are gathered
+// in LDS (at most top x top of them, a few more than top as a rule) and ranked by counting the larger ones.
+// Grid (n), 256 threads, thread p for part p.
 template <class E>
-__global__ __launch_bounds__(kLpThreads) void logprobs_join_kernel(const E* __restrict__ x, int64_t ld, int vocab, int parts, int top,
-                                                                   const LogitSums* __restrict__ sums,
-                                                                   const uint64_t* __restrict__ keys,
-                                                                   const int32_t* __restrict__ tokens, float* __restrict__ logp,
-                                                                   float* __restrict__ entropy, int32_t* __restrict__ top_ids,
-                                                                   float* __restrict__ top_logp) {
-  __shared__ uint64_t cand[kLpCand];
-  __shared__ LogitSums sh;
-  const int tid = threadIdx.x;
+__global__ __launch_bounds__(256) void logprobs_join_kernel(const E* __restrict__ x, int64_t ld, int vocab, int parts, int top,
+                                                            const LogitSums* __restrict__ sums, const uint64_t* __restrict__ keys,
+                                                            const int32_t* __restrict__ tokens, float* __restrict__ logp,
+                                                            float* __restrict__ entropy, int32_t* __restrict__ top_ids,
+                                                            float* __restrict__ top_logp) {
+  __shared__ uint64_t cand[kLogprobTop * kLogprobTop], first[256], out[kLogprobTop];
+  __shared__ LogitSums red[4];
+  __shared__ uint64_t s_bound;
+  __shared__ int s_cnt;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const size_t row = blockIdx.x;
   x += row * (size_t)ld;
-  if (tid < 64) {
-    LogitSums s{-INFINITY, 0.f, 0.f};
-    if (tid < parts) s = sums[row * parts + tid];
+  if (tid < top) out[tid] = 0;
+  const bool has = tid < parts;
+  const int t = logp ? tokens[row] : -1;
+  LogitSums s{-INFINITY, 0.f, 0.f};
+  if (has) s = sums[row * parts + tid];
+  const uint64_t* list = keys + (row * (size_t)parts + (has ? tid : 0)) * top;
+  constexpr int N = 4;  // of its list, requested with the sums
+  uint64_t k[N];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const LogitSums y{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.a, o)};
-      s = join(s, y);
-    }
-    if (tid == 0) sh = s;
+  for (int i = 0; i < N; ++i) k[i] = has && i < top ? list[min(i, top - 1)] : 0;
+  const float xt = t >= 0 && t < vocab ? to_f32(x[t]) : __builtin_nanf("");
+  if (tid == 0) {
+    s_cnt = 0;
+    s_bound = 1;  // fewer parts than top: every key
   }
-  // the parts' best keys, as many parts at a time as the list holds beside those kept so far
-  int cnt = 0;
-  if (top) {
-    const uint64_t* kr = keys + row * (size_t)parts * top;
-    const int total = parts * top;
-    for (int at = 0; at < total;) {
-      const int take = min(total - at, kLpCand - cnt);
-      for (int i = tid; i < take; i += kLpThreads) cand[cnt + i] = kr[at + i];
-      at += take;
-      cnt += take;
-      __syncthreads();
-      prune(cand, cnt, top, tid);
-      cnt = top;
-    }
+  first[tid] = k[0];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const LogitSums y{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.a, o)};
+    s = join(s, y);
+  }
+  if (lane == 0) red[w] = s;
+  __syncthreads();
+  if (parts >= top && top && 64 * w < parts) {
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < parts; ++j) r += first[j] > k[0] ? 1 : 0;
+    if (k[0] && r == top - 1) s_bound = k[0];
   }
   __syncthreads();
-  const LogitSums s = sh;
+  const uint64_t bound = s_bound;
+  for (int i = 0; i < top; ++i) {
+    const uint64_t key = i == 0 ? k[0] : i == 1 ? k[1] : i == 2 ? k[2] : i == 3 ? k[3] : has ? list[i] : 0;
+    const bool in = key >= bound;
+    if (!__ballot(in)) break;
+    if (in) cand[atomicAdd(&s_cnt, 1)] = key;
+  }
+  __syncthreads();
+  const int cnt = s_cnt;
+  for (int i = tid; i < cnt; i += 256) {
+    const uint64_t mine = cand[i];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < cnt; ++j) r += cand[j] > mine ? 1 : 0;
+    if (r < top) out[r] = mine;
+  }
+  __syncthreads();
+  s = join(join(red[0], red[1]), join(red[2], red[3]));
   const float lz = s.m == -INFINITY ? __builtin_nanf("") : logf(s.z);
   if (tid == 0) {
-    if (logp) {
-      const int t = tokens[row];
-      logp[row] = t < 0 || t >= vocab ? __builtin_nanf("") : (to_f32(x[t]) - s.m) - lz;
-    }
+    if (logp) logp[row] = (xt - s.m) - lz;
     if (entropy) entropy[row] = lz - s.a / s.z;
   }
   if (tid < top) {
-    const int id = (int)~(unsigned)cand[tid];
+    const uint64_t key = out[tid];
+    const int id = (int)min(~(unsigned)key, (unsigned)(vocab - 1));
     top_ids[row * top + tid] = id;
     if (top_logp) top_logp[row * top + tid] = (to_f32(x[id]) - s.m) - lz;
   }
 }
 
-// Parts of a row: whole steps, as many workgroups as fill the device a few times over.
+// Parts of a row: whole steps, enough waves to fill the device.
 static int logprob_parts(int n, int64_t vocab, int* per) {
   const int64_t steps = (vocab + kLpStep - 1) / kLpStep;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({steps, kLpMaxSplits, 2048 / n}));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({steps, kLpMaxParts, 4096 / n}));
   const int64_t p = (steps + want - 1) / want;
   *per = (int)(p * kLpStep);
   return (int)((steps + p - 1) / p);
@@ -276,12 +318,11 @@ int logprobs(const void* logits, int64_t ld, int type, int n, int vocab, const i
     for (int r0 = 0; r0 < n; r0 += 65535) {
       const dim3 g((unsigned)parts, (unsigned)std::min(65535, n - r0));
       const size_t at = (size_t)r0 * parts;
-      if (top) logprobs_kernel<E, true><<<g, kLpThreads, 0, s>>>(x + (size_t)r0 * ld, ld, vocab, per, top, sums + at, keys + at * top);
-      else logprobs_kernel<E, false><<<g, kLpThreads, 0, s>>>(x + (size_t)r0 * ld, ld, vocab, per, top, sums + at, keys);
+      if (top) logprobs_kernel<E, true><<<g, 64, 0, s>>>(x + (size_t)r0 * ld, ld, vocab, per, top, sums + at, keys + at * top);
+      else logprobs_kernel<E, false><<<g, 64, 0, s>>>(x + (size_t)r0 * ld, ld, vocab, per, top, sums + at, keys);
       DZ_HIP_CHECK(hipGetLastError());
     }
-    logprobs_join_kernel<E><<<(unsigned)n, kLpThreads, 0, s>>>(x, ld, vocab, parts, top, sums, keys, tokens, logp, entropy, top_ids,
-                                                                top_logp);
+    logprobs_join_kernel<E><<<(unsigned)n, 256, 0, s>>>(x, ld, vocab, parts, top, sums, keys, tokens, logp, entropy, top_ids, top_logp);
     DZ_HIP_CHECK(hipGetLastError());
     return DZ_OK;
   });
