@@ -9,12 +9,14 @@
 
 namespace dz {
 
-constexpr int kLogprobTop = 64;   // most alternatives: a wave's lanes
-constexpr int kLpVals = 16;       // logits of a lane and step
+constexpr int kLogprobTop = 64;  // most alternatives
+constexpr int kLpVals = 16;      // logits of a lane and step
 constexpr int kLpStep = 64 * kLpVals;
-constexpr int kLpMaxParts = 256;  // parts of a row: the join's threads
-constexpr int kLpKeep = 2 * kLogprobTop + 16;       // a longer list is cut to the best
-constexpr int kLpCand = kLpKeep + kLpStep;          // ... which one step can outgrow by this much
+constexpr int kLpGroups = 4;     // groups of a step: the 16 lanes of a DPP row
+constexpr int kLpMaxParts = 256; // parts of a row
+constexpr int kLpCand = kLogprobTop * kLpVals + 2 * kLogprobTop;  // candidates in LDS (see logprobs_join_kernel)
+constexpr int kLpJoin = 512;     // threads of the join
+constexpr int kLpListed = 1024;  // groups looked through at a time
 
 // A logit and its id as one word whose unsigned order is "larger value first, then lower id", NaN below -inf.
 __device__ __forceinline__ uint64_t logit_key(float v, int i) {
@@ -56,54 +58,45 @@ __device__ __forceinline__ void values_of(u32x4 w, float* x) {
   }
 }
 
-// Wave-wide (one wave a workgroup, so LDS needs no barrier but the compiler's).
-__device__ __forceinline__ void lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
-
-// The `top` largest of the cnt (>= top) distinct keys in c, in order, to c[0 .. top): every key counts the larger ones.
-__device__ __forceinline__ void prune(uint64_t* c, int cnt, int top, int lane) {
-  // in rounds of 64: a key's rank is known before any is moved, so the best of all go to a second place first
-  uint64_t best = 0;  // lane r: the key of rank r
-  __shared__ uint64_t out[kLogprobTop];
-  for (int i0 = 0; i0 < cnt; i0 += 64) {
-    const uint64_t mine = i0 + lane < cnt ? c[i0 + lane] : 0;
-    int r = mine ? 0 : kLogprobTop;
-    for (int j = 0; j < cnt; ++j) r += c[j] > mine ? 1 : 0;
-    if (r < top) out[r] = mine;
+// Logits 16 lanes of a step hold: a lane's are runs of 16 bytes, the wave's runs one after another.
+template <class E>
+__device__ __forceinline__ int logit_at(int step, int lane, int i) {
+  constexpr int R = 16 / sizeof(E);
+  return step * kLpStep + ((i / R) * 64 + lane) * R + i % R;
+}
+// ... of a step that ends behind the row: -inf there.
+template <class E>
+__device__ __forceinline__ void load_ragged(const E* __restrict__ x, int step, int lane, int vocab, float (&v)[kLpVals]) {
+#pragma unroll
+  for (int i = 0; i < kLpVals; ++i) {
+    const int c = logit_at<E>(step, lane, i);
+    const float u = to_f32(x[min(c, vocab - 1)]);
+    v[i] = c < vocab ? u : -INFINITY;
   }
-  lds_fence();
-  if (lane < top) best = out[lane];
-  if (lane < top) c[lane] = best;
-  lds_fence();
 }
 
-// One part of a row by one wave: its sums and its `top` best keys in order.  A pass over the logits, 1024 a step, the next
-// step's on their way: each lane keeps its own running maximum and sums.  Keys above the part's top-th best so far
-// (`bound`) go to a list in LDS; a lane looks at its keys only where the largest of its logits reaches the bound's value.
-// Where more than 32 lanes do (the first step; rows that keep rising) the bound first rises to the top-th largest of the
-// lanes' own best keys: only lanes whose best is above it can then add any.
-// Bound by the loads at many rows: 16 exponentials and about 120 other instructions a lane and step of 4 KB of f32.
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false)));
+}
+
+// One part of a row by one wave: its sums, and the largest logit of every group of 256 (for the alternatives; gmax null:
+// none wanted).  A pass over the logits, 1024 a step, the next step's on their way; each lane keeps its own running maximum
+// and sums.  Bound by the loads: 1024 rows of 248320 bf16 logits at the rate of a copy (5.2 TB/s).  Keys and ids take no part
+// here: a list of best keys kept during the pass cost 40% of it at 20 alternatives.
 // Grid (parts, n), 64 threads.
-template <class E, bool TOP>
-__global__ __launch_bounds__(64) void logprobs_kernel(const E* __restrict__ x, int64_t ld, int vocab, int per, int top,
-                                                      LogitSums* __restrict__ sums, uint64_t* __restrict__ keys) {
-  constexpr int R = 16 / sizeof(E);  // a lane's logits: runs of 16 bytes, the wave's runs one after another
-  __shared__ uint64_t cand[TOP ? kLpCand : 1];
+template <class E>
+__global__ __launch_bounds__(64) void logprobs_kernel(const E* __restrict__ x, int64_t ld, int vocab, int per,
+                                                      LogitSums* __restrict__ sums, float* __restrict__ gmax) {
+  constexpr int R = 16 / sizeof(E);
   const int lane = threadIdx.x, part = blockIdx.x, parts = gridDim.x;
   const size_t row = blockIdx.y;
+  const int steps = (vocab + kLpStep - 1) / kLpStep;
   x += row * (size_t)ld;
-  const int beg = part * per, end = min(vocab, beg + per);
+  if (gmax) gmax += row * (size_t)steps * kLpGroups + (lane >> 4);
+  const int beg = part * per, end = min(steps, beg + per);
   LogitSums s{-INFINITY, 0.f, 0.f};
-  uint64_t bound = 0;  // keys up to this one are not among the part's best
-  float floor = 0.f;   // only larger logits have keys above it, where it is that of a number
-  bool any = true;     // it is none: every key is looked at
-  int cnt = 0;
-  auto raise = [&](uint64_t key) {
-    bound = key;
-    floor = cand_of(key).v;
-    any = key <= (uint64_t)0x00800000u << 32;  // NaN, nothing, or -inf
-  };
-  // the logits of the step at c0
-  auto step = [&](int c0, const float (&v)[kLpVals]) {
+  auto take = [&](int step, const float (&v)[kLpVals]) {
     float vm = v[0];
 #pragma unroll
     for (int i = 1; i < kLpVals; ++i) vm = fmaxf(vm, v[i]);
@@ -120,81 +113,36 @@ __global__ __launch_bounds__(64) void logprobs_kernel(const E* __restrict__ x, i
     }
     s.z += z;
     s.a += a;
-    if constexpr (TOP) {
-      const unsigned long long over = __ballot(any || vm > floor);
-      if (over) {
-        auto key_at = [&](int i) {
-          const int c = c0 + ((i / R) * 64 + lane) * R + i % R;
-          return c < end ? logit_key(v[i], c) : (uint64_t)0;
-        };
-        if (__popcll(over) > 32) {
-          uint64_t best = 0;
-#pragma unroll
-          for (int i = 0; i < kLpVals; ++i) {
-            const uint64_t k = key_at(i);
-            best = k > best ? k : best;
-          }
-          cand[cnt + lane] = best;  // behind the list
-          lds_fence();
-          int r = best > bound ? 0 : 64;
-#pragma unroll 8
-          for (int j = 0; j < 64; ++j) r += cand[cnt + j] > best ? 1 : 0;
-          lds_fence();
-          const unsigned long long at = __ballot(r == top - 1);  // none where fewer lanes than top are above the bound
-          if (at) {
-            const int l = __builtin_ctzll(at);
-            const uint64_t k = ((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(best >> 32), l) << 32) |
-                               (unsigned)__builtin_amdgcn_readlane((int)(unsigned)best, l);
-            raise(k - 1);
-            // an equal logit of a lower id in this step is above the bound: the next number down (below 0, past -0)
-            floor = floor == 0.f ? -__uint_as_float(1u) : cand_of(bound - ((uint64_t)1 << 32)).v;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kLpVals; ++i) {
-          if (!__ballot(any || v[i] > floor)) continue;
-          const uint64_t k = key_at(i);
-          const unsigned long long in = __ballot(k > bound);
-          if (k > bound) cand[cnt + __popcll(in & ((1ull << lane) - 1))] = k;
-          cnt += __popcll(in);
-        }
-        lds_fence();
-        if (cnt > kLpKeep || (any && cnt >= top)) {
-          prune(cand, cnt, top, lane);
-          cnt = top;
-          raise(cand[top - 1]);
-        } else if (!any) {
-          floor = cand_of(bound).v;  // later ids do not win ties
-        }
-      }
+    if (gmax) {
+      float g = vm;
+      g = dpp_max<0xB1>(g);
+      g = dpp_max<0x4E>(g);
+      g = dpp_max<0x141>(g);
+      g = dpp_max<0x140>(g);
+      if ((lane & 15) == 0) gmax[step * kLpGroups] = g;
     }
   };
   // whole steps, whose loads need no bounds and are requested a step ahead; then what is left
-  const int whole = beg + (end - beg) / kLpStep * kLpStep;
+  const int whole = min(end, vocab / kLpStep);
   if (beg < whole) {
     const E* p = x + lane * R;
     u32x4 next[kLpVals / R];
 #pragma unroll
-    for (int k = 0; k < kLpVals / R; ++k) next[k] = load16(p + beg + k * 64 * R);
-    for (int c0 = beg; c0 < whole; c0 += kLpStep) {
+    for (int k = 0; k < kLpVals / R; ++k) next[k] = load16(p + (size_t)beg * kLpStep + k * 64 * R);
+    for (int c = beg; c < whole; ++c) {
       float v[kLpVals];
 #pragma unroll
       for (int k = 0; k < kLpVals / R; ++k) values_of<E, R>(next[k], v + k * R);
-      const int cn = min(c0 + kLpStep, whole - kLpStep);
+      const int cn = min(c + 1, whole - 1);
 #pragma unroll
-      for (int k = 0; k < kLpVals / R; ++k) next[k] = load16(p + cn + k * 64 * R);
-      step(c0, v);
+      for (int k = 0; k < kLpVals / R; ++k) next[k] = load16(p + (size_t)cn * kLpStep + k * 64 * R);
+      take(c, v);
     }
   }
   if (whole < end) {
     float v[kLpVals];
-#pragma unroll
-    for (int i = 0; i < kLpVals; ++i) {
-      const int c = whole + ((i / R) * 64 + lane) * R + i % R;
-      const float u = to_f32(x[min(c, end - 1)]);
-      v[i] = c < end ? u : -INFINITY;
-    }
-    step(whole, v);
+    load_ragged(x, whole, lane, vocab, v);
+    take(whole, v);
   }
   // the lanes' sums in a fixed order
 #pragma unroll
@@ -203,77 +151,81 @@ __global__ __launch_bounds__(64) void logprobs_kernel(const E* __restrict__ x, i
     s = join(s, y);
   }
   if (lane == 0) sums[row * parts + part] = s;
-  if constexpr (TOP) {
-    // a part of fewer logits than top keeps what it has, in order, and zeros
-    for (int i = cnt + lane; i < top; i += 64) cand[i] = 0;
-    lds_fence();
-    prune(cand, max(cnt, top), top, lane);
-    if (lane < top) keys[(row * parts + part) * top + lane] = lane < cnt ? cand[lane] : 0;
-  }
 }
 
-// The parts of a row as its results.  Of the parts' lists, each in order, only those whose first key is among the `top`
-// largest first keys can hold one of the row's best, and only keys not below the last of those: they are gathered
-// in LDS (at most top x top of them, a few more than top as a rule) and ranked by counting the larger ones.
-// Grid (n), 256 threads, thread p for part p.
+// The `top` largest of the cnt distinct keys in c, in order, to c[0 .. min(top, cnt)): every key counts the larger ones.
+__device__ __forceinline__ void prune(uint64_t* c, int cnt, int top, int tid) {
+  constexpr int N = (kLpCand + kLpJoin - 1) / kLpJoin;
+  uint64_t mine[N];
+  int rank[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = tid + kLpJoin * k;
+    rank[k] = kLpCand;
+    if (i < cnt) {
+      mine[k] = c[i];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < cnt; ++j) r += c[j] > mine[k] ? 1 : 0;
+      rank[k] = r;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (rank[k] < top) c[rank[k]] = mine[k];
+  __syncthreads();
+}
+
+// A row's results.  Alternatives: the groups' maxima are dealt to 256 threads, and the top-th largest of what each thread holds
+// is a value that at least `top` logits reach, so that only groups that reach it (a few more than top of them) hold any
+// of the best; those are read again, 32 at a time, and their keys not below it gathered in LDS and ranked by counting the
+// larger ones.  Where more keys come than the list holds (rows full of ties), the bound first rises to the top-th
+// largest of the threads' own best keys of the batch: at most top threads, of 16 logits each, then have any above it.
+// Grid (n), 512 threads, thread p for part p.
 template <class E>
-__global__ __launch_bounds__(256) void logprobs_join_kernel(const E* __restrict__ x, int64_t ld, int vocab, int parts, int top,
-                                                            const LogitSums* __restrict__ sums, const uint64_t* __restrict__ keys,
-                                                            const int32_t* __restrict__ tokens, float* __restrict__ logp,
-                                                            float* __restrict__ entropy, int32_t* __restrict__ top_ids,
-                                                            float* __restrict__ top_logp) {
-  __shared__ uint64_t cand[kLogprobTop * kLogprobTop], first[256], out[kLogprobTop];
-  __shared__ LogitSums red[4];
+__global__ __launch_bounds__(kLpJoin) void logprobs_join_kernel(const E* __restrict__ x, int64_t ld, int vocab, int parts, int top,
+                                                                const LogitSums* __restrict__ sums,
+                                                                const float* __restrict__ gmax, const int32_t* __restrict__ tokens,
+                                                                float* __restrict__ logp, float* __restrict__ entropy,
+                                                                int32_t* __restrict__ top_ids, float* __restrict__ top_logp) {
+  constexpr int R = 16 / sizeof(E), kHeld = 4;
+  __shared__ uint64_t cand[kLpCand], best[kLpJoin];
+  __shared__ __align__(16) unsigned order[256];
+  __shared__ int group[kLpListed];
+  __shared__ LogitSums red[kLpMaxParts / 64];
   __shared__ uint64_t s_bound;
-  __shared__ int s_cnt;
+  __shared__ unsigned s_least;
+  __shared__ int s_cnt, s_n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const size_t row = blockIdx.x;
   x += row * (size_t)ld;
-  if (tid < top) out[tid] = 0;
-  const bool has = tid < parts;
   const int t = logp ? tokens[row] : -1;
   LogitSums s{-INFINITY, 0.f, 0.f};
-  if (has) s = sums[row * parts + tid];
-  const uint64_t* list = keys + (row * (size_t)parts + (has ? tid : 0)) * top;
-  constexpr int N = 4;  // of its list, requested with the sums
-  uint64_t k[N];
+  if (tid < parts) s = sums[row * parts + tid];
+  const int groups = (vocab + kLpStep - 1) / kLpStep * kLpGroups;
+  gmax += row * (size_t)groups;
+  float held[kHeld], gm = -INFINITY;  // the groups tid + 256 i of the first 1024, and the largest of all of the thread's
+  if (top && tid < 256) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) k[i] = has && i < top ? list[min(i, top - 1)] : 0;
+    for (int i = 0; i < kHeld; ++i) held[i] = gmax[min(tid + 256 * i, groups - 1)];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) gm = tid + 256 * i < groups ? fmaxf(gm, held[i]) : gm;
+    for (int g = tid + 256 * kHeld; g < groups; g += 256) gm = fmaxf(gm, gmax[g]);
+    order[tid] = (unsigned)(cand_key(gm, 0) >> 32);
+  }
   const float xt = t >= 0 && t < vocab ? to_f32(x[t]) : __builtin_nanf("");
   if (tid == 0) {
-    s_cnt = 0;
-    s_bound = 1;  // fewer parts than top: every key
+    s_cnt = s_n = 0;
+    s_least = ~0u;
   }
-  first[tid] = k[0];
+  if (w < kLpMaxParts / 64) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const LogitSums y{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.a, o)};
-    s = join(s, y);
-  }
-  if (lane == 0) red[w] = s;
-  __syncthreads();
-  if (parts >= top && top && 64 * w < parts) {
-    int r = 0;
-#pragma unroll 8
-    for (int j = 0; j < parts; ++j) r += first[j] > k[0] ? 1 : 0;
-    if (k[0] && r == top - 1) s_bound = k[0];
-  }
-  __syncthreads();
-  const uint64_t bound = s_bound;
-  for (int i = 0; i < top; ++i) {
-    const uint64_t key = i == 0 ? k[0] : i == 1 ? k[1] : i == 2 ? k[2] : i == 3 ? k[3] : has ? list[i] : 0;
-    const bool in = key >= bound;
-    if (!__ballot(in)) break;
-    if (in) cand[atomicAdd(&s_cnt, 1)] = key;
-  }
-  __syncthreads();
-  const int cnt = s_cnt;
-  for (int i = tid; i < cnt; i += 256) {
-    const uint64_t mine = cand[i];
-    int r = 0;
-#pragma unroll 8
-    for (int j = 0; j < cnt; ++j) r += cand[j] > mine ? 1 : 0;
-    if (r < top) out[r] = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const LogitSums y{__shfl_xor(s.m, o), __shfl_xor(s.z, o), __shfl_xor(s.a, o)};
+      s = join(s, y);
+    }
+    if (lane == 0) red[w] = s;
   }
   __syncthreads();
   s = join(join(red[0], red[1]), join(red[2], red[3]));
@@ -282,47 +234,133 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(const E* __restrict_
     if (logp) logp[row] = (xt - s.m) - lz;
     if (entropy) entropy[row] = lz - s.a / s.z;
   }
+  if (top == 0) return;
+  // the smallest of the values with fewer than top larger ones is the top-th largest
+  const int holders = min(groups, 256);
+  if (tid < holders) {
+    const unsigned mine = order[tid];
+    int r = 0;
+    for (int j = 0; j + 4 <= holders; j += 4) {  // groups come in fours
+      const u32x4 o = *reinterpret_cast<const u32x4*>(order + j);
+      r += (o[0] > mine) + (o[1] > mine) + (o[2] > mine) + (o[3] > mine);
+    }
+    if (r < top) atomicMin(&s_least, mine);
+  }
+  __syncthreads();
+  // every key where fewer than top groups hold a logit above -inf
+  const bool any = holders < top || s_least < 0x00800000u;
+  const float least = any ? -INFINITY : cand_of((uint64_t)s_least << 32).v;
+  uint64_t bound = 0;
+  int cnt = 0;
+  for (int g0 = 0; g0 < groups; g0 += kLpListed) {
+    if (g0) {
+      __syncthreads();
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+    }
+    if (tid < 256) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int g = g0 + tid + 256 * i;
+        const float m = g0 == 0 ? held[i] : gmax[min(g, groups - 1)];
+        if (g < groups && (any || m >= least)) group[atomicAdd(&s_n, 1)] = g;
+      }
+    }
+    __syncthreads();
+    const int listed = s_n;
+    for (int b = 0; b < listed; b += kLpJoin / 16) {
+      const int at = b + (tid >> 4), g = group[min(at, listed - 1)], step = g / kLpGroups, ln = (g % kLpGroups) * 16 + (tid & 15);
+      float v[kLpVals];
+      if ((step + 1) * kLpStep <= vocab) {
+#pragma unroll
+        for (int k = 0; k < kLpVals / R; ++k) values_of<E, R>(load16(x + logit_at<E>(step, ln, k * R)), v + k * R);
+      } else {
+        load_ragged(x, step, ln, vocab, v);
+      }
+      uint64_t key[kLpVals], top_key = 0;
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < kLpVals; ++i) {
+        const int c = logit_at<E>(step, ln, i);
+        key[i] = at < listed && c < vocab && (any || v[i] >= least) ? logit_key(v[i], c) : 0;
+        if (key[i] <= bound) key[i] = 0;
+        mine += key[i] ? 1 : 0;
+        top_key = key[i] > top_key ? key[i] : top_key;
+      }
+      __syncthreads();  // s_n has been read
+      if (tid == 0) {
+        s_n = 0;
+        s_bound = bound;
+      }
+      best[tid] = top_key;
+      __syncthreads();
+      if (mine) atomicAdd(&s_n, mine);
+      __syncthreads();
+      const int all = s_n;
+      if (all == 0) continue;
+      if (cnt + all > kLpCand) {
+        int r = 0;
+#pragma unroll 8
+        for (int j = 0; j < kLpJoin; ++j) r += best[j] > top_key ? 1 : 0;
+        if (top_key && r == top - 1) s_bound = top_key - 1;
+        __syncthreads();
+        bound = s_bound;
+      }
+#pragma unroll
+      for (int i = 0; i < kLpVals; ++i)
+        if (key[i] > bound) cand[atomicAdd(&s_cnt, 1)] = key[i];
+      __syncthreads();
+      cnt = s_cnt;
+      if (cnt > 2 * kLogprobTop) {
+        prune(cand, cnt, top, tid);
+        cnt = top;
+        bound = cand[top - 1];
+        if (tid == 0) s_cnt = top;
+      }
+    }
+  }
+  __syncthreads();
+  prune(cand, cnt, top, tid);
   if (tid < top) {
-    const uint64_t key = out[tid];
-    const int id = (int)min(~(unsigned)key, (unsigned)(vocab - 1));
-    top_ids[row * top + tid] = id;
-    if (top_logp) top_logp[row * top + tid] = (to_f32(x[id]) - s.m) - lz;
+    const SpecCand c = cand_of(cand[tid]);
+    top_ids[row * top + tid] = c.i;
+    if (top_logp) top_logp[row * top + tid] = (c.v - s.m) - lz;
   }
 }
 
-// Parts of a row: whole steps, enough waves to fill the device.
+// Parts of a row, `per` steps each: enough waves to fill the device.
 static int logprob_parts(int n, int64_t vocab, int* per) {
   const int64_t steps = (vocab + kLpStep - 1) / kLpStep;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({steps, kLpMaxParts, 4096 / n}));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({steps, kLpMaxParts, 8192 / n}));
   const int64_t p = (steps + want - 1) / want;
-  *per = (int)(p * kLpStep);
+  *per = (int)p;
   return (int)((steps + p - 1) / p);
 }
 
 size_t logprobs_work(int n, int64_t vocab, int top) {
   int per;
   const size_t parts = (size_t)n * logprob_parts(n, vocab, &per);
-  return parts * ((size_t)top * sizeof(uint64_t)) + parts * sizeof(LogitSums) + 16;
+  const size_t groups = top ? (size_t)n * ((vocab + kLpStep - 1) / kLpStep) * kLpGroups : 0;
+  return groups * sizeof(float) + parts * sizeof(LogitSums) + 16;
 }
 
 int logprobs(const void* logits, int64_t ld, int type, int n, int vocab, const int32_t* tokens, int top, float* logp, float* entropy,
              int32_t* top_ids, float* top_logp, void* work, hipStream_t s) {
   int per;
   const int parts = logprob_parts(n, vocab, &per);
-  uint64_t* keys = static_cast<uint64_t*>(work);
-  LogitSums* sums = reinterpret_cast<LogitSums*>(keys + (size_t)n * parts * top);
+  const size_t groups = (size_t)((vocab + kLpStep - 1) / kLpStep) * kLpGroups;
+  LogitSums* sums = static_cast<LogitSums*>(work);
+  float* gmax = reinterpret_cast<float*>(sums + (size_t)n * parts);
   return with_type(type, [&](auto* e) -> int {
     using E = std::remove_pointer_t<decltype(e)>;
     const E* x = static_cast<const E*>(logits);
     // rows beyond the grid's second dimension go in further launches
     for (int r0 = 0; r0 < n; r0 += 65535) {
-      const dim3 g((unsigned)parts, (unsigned)std::min(65535, n - r0));
-      const size_t at = (size_t)r0 * parts;
-      if (top) logprobs_kernel<E, true><<<g, 64, 0, s>>>(x + (size_t)r0 * ld, ld, vocab, per, top, sums + at, keys + at * top);
-      else logprobs_kernel<E, false><<<g, 64, 0, s>>>(x + (size_t)r0 * ld, ld, vocab, per, top, sums + at, keys);
+      logprobs_kernel<E><<<dim3((unsigned)parts, (unsigned)std::min(65535, n - r0)), 64, 0, s>>>(
+          x + (size_t)r0 * ld, ld, vocab, per, sums + (size_t)r0 * parts, top ? gmax + r0 * groups : nullptr);
       DZ_HIP_CHECK(hipGetLastError());
     }
-    logprobs_join_kernel<E><<<(unsigned)n, 256, 0, s>>>(x, ld, vocab, parts, top, sums, keys, tokens, logp, entropy, top_ids, top_logp);
+    logprobs_join_kernel<E><<<(unsigned)n, kLpJoin, 0, s>>>(x, ld, vocab, parts, top, sums, gmax, tokens, logp, entropy, top_ids, top_logp);
     DZ_HIP_CHECK(hipGetLastError());
     return DZ_OK;
   });
