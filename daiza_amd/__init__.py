@@ -617,39 +617,69 @@ class Context:
         return lib().dz_ctx_stream(self._h)
 
 
-# ---------------------------------------------------------------- device arrays
+# ---------------------------------------------------------------- device arrays (torch tensors)
 
-_TYPES = {"torch.float32": GGUF_F32, "torch.float16": GGUF_F16, "torch.bfloat16": GGUF_BF16}
+_torch = None  # imported by the first call on device arrays
+_TYPES = {}    # {torch dtype: DZ_F32, DZ_F16, DZ_BF16}
+_F32 = {}
+_I32 = {}
 
 
-def _rows(t, what, shape, types=("torch.float32",)):
-    """(pointer, elements from row to row) of a device tensor of this shape (None: any size) with its rows contiguous."""
-    if str(t.dtype) not in types:
+def _use_torch():
+    global _torch
+    import torch
+    _TYPES.update({torch.float32: GGUF_F32, torch.float16: GGUF_F16, torch.bfloat16: GGUF_BF16})
+    _F32[torch.float32] = GGUF_F32
+    _I32[torch.int32] = 0
+    _torch = torch
+
+
+def _rows(t, what, shape, types, whole=False):
+    """(pointer, elements from row to row, type code) of a device tensor of this shape (None: any size) whose rows are contiguous,
+    or that is contiguous as a whole."""
+    code, dims = types.get(t.dtype), t.shape
+    if code is None:
         raise DaizaError(DZ_ERR_UNSUPPORTED, "%s of %s" % (what, t.dtype))
-    if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
-        raise DaizaError(DZ_ERR_TENSOR, "%s of shape %s, expected %s" % (what, tuple(t.shape), tuple("n" if s is None else s for s in shape)))
-    inner = 1
-    for d, st in zip(t.shape[:0:-1], t.stride()[:0:-1]):
-        if d > 1 and st != inner:
-            raise DaizaError(DZ_ERR_TENSOR, "%s: a row is not contiguous" % what)
-        inner *= d
+    if len(dims) != len(shape):
+        raise DaizaError(DZ_ERR_TENSOR, "%s of %d dimensions, expected %d" % (what, len(dims), len(shape)))
+    for want, d in zip(shape, dims):
+        if want is not None and want != d:
+            raise DaizaError(DZ_ERR_TENSOR, "%s of shape %s, expected %s" % (what, tuple(dims), tuple(shape)))
     if not t.is_cuda:
         raise DaizaError(DZ_ERR_TENSOR, "%s is not on a device" % what)
-    return t.data_ptr(), max(t.stride(0), inner) if t.shape[0] < 2 else t.stride(0)
+    if t.is_contiguous():
+        row = 1
+        for d in dims[1:]:
+            row *= d
+        return t.data_ptr(), row, code
+    stride, row = t.stride(), 1
+    for d, st in zip(dims[:0:-1], stride[:0:-1]):
+        if d > 1 and st != row:
+            whole = True
+            break
+        row *= d
+    if whole:
+        raise DaizaError(DZ_ERR_TENSOR, "%s is not contiguous%s" % (what, "" if len(dims) == 1 else " in its rows"))
+    return t.data_ptr(), stride[0], code
 
 
-def _stream_of(t, stream):
-    """The HIP stream (an int) of a call: the one given, or torch's current one."""
-    import torch
-    return torch.cuda.current_stream(t.device).cuda_stream if stream is None else int(getattr(stream, "cuda_stream", stream))
+def _call_stream(t, stream):
+    """The HIP stream (an int) of a call on t's device: the one given (an int or a torch stream), or torch's current one."""
+    if stream is None:
+        return _current_stream(t)
+    return int(getattr(stream, "cuda_stream", stream))
+
+
+def _current_stream(t):
+    raw = getattr(_torch._C, "_cuda_getCurrentRawStream", None)  # the same as below without a stream object
+    return raw(t.get_device()) if raw else _torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _work(t, n_bytes, stream):
     """Device memory for one call, from torch's allocator: it goes back when the call has run on its stream."""
-    import torch
-    w = torch.empty(max(16, n_bytes), dtype=torch.uint8, device=t.device)
-    if stream != torch.cuda.current_stream(t.device).cuda_stream:
-        w.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
+    w = _torch.empty(max(16, n_bytes), dtype=_torch.uint8, device=t.device)
+    if stream != _current_stream(t):
+        w.record_stream(_torch.cuda.ExternalStream(stream, device=t.device))
     return w
 
 
@@ -662,6 +692,9 @@ class Kv4Cache:
 
     def __init__(self, kv_heads, head_dim, capacity):
         self.kv_heads, self.head_dim, self.capacity = int(kv_heads), int(head_dim), int(capacity)
+        self._h = None
+        if _torch is None:
+            _use_torch()
         h = _vp()
         _check(lib().dz_kv4_create(self.kv_heads, self.head_dim, self.capacity, ctypes.byref(h)))
         self._h = h
@@ -686,68 +719,69 @@ class Kv4Cache:
 
     def append_dev(self, k, v, stream=None):
         """Writes rows k, v [n][kv_heads][head_dim] (float32, float16 or bfloat16) behind the rows held."""
-        shape = (None, self.kv_heads, self.head_dim)
-        kp, ldk = _rows(k, "k", shape, _TYPES)
-        vp, ldv = _rows(v, "v", (k.shape[0],) + shape[1:], (str(k.dtype),))
-        _check(lib().dz_kv4_append_dev(self._h, kp, ldk, vp, ldv, _TYPES[str(k.dtype)], k.shape[0], _stream_of(k, stream)))
+        n = k.shape[0]
+        kp, ldk, ty = _rows(k, "k", (n, self.kv_heads, self.head_dim), _TYPES)
+        vp, ldv, tv = _rows(v, "v", (n, self.kv_heads, self.head_dim), _TYPES)
+        if ty != tv:
+            raise DaizaError(DZ_ERR_TENSOR, "k of %s, v of %s" % (k.dtype, v.dtype))
+        _check(lib().dz_kv4_append_dev(self._h, kp, ldk, vp, ldv, ty, n, _call_stream(k, stream)))
 
     def read_dev(self, start, k=None, v=None, stream=None):
         """The float32 values of rows start .. into k and v [kv_heads][n][head_dim] (contiguous; either may be None)."""
         t = k if k is not None else v
         if t is None:
             return
-        for x, what in ((k, "k"), (v, "v")):
-            if x is not None:
-                _rows(x, what, (self.kv_heads, t.shape[1], self.head_dim))
-                if not x.is_contiguous():
-                    raise DaizaError(DZ_ERR_TENSOR, "%s is not contiguous" % what)
-        _check(lib().dz_kv4_read_dev(self._h, int(start), t.shape[1], None if k is None else k.data_ptr(),
-                                     None if v is None else v.data_ptr(), _stream_of(t, stream)))
+        shape = (self.kv_heads, t.shape[1], self.head_dim)
+        kp = None if k is None else _rows(k, "k", shape, _F32, True)[0]
+        vp = None if v is None else _rows(v, "v", shape, _F32, True)[0]
+        _check(lib().dz_kv4_read_dev(self._h, int(start), shape[1], kp, vp, _call_stream(t, stream)))
 
     def attend_dev(self, q, out, scale=None, weights=None, stream=None):
         """Causal attention of the newest rows' queries q [n][heads][head_dim] into out (the same shape and type); scale is
         1/sqrt(head_dim) if None.  weights (float32 [kv_heads][>= rows held]) grow by the attention that each row received."""
-        qp, ldq = _rows(q, "q", (None, None, self.head_dim), _TYPES)
-        op, ldo = _rows(out, "out", q.shape, (str(q.dtype),))
-        wp, ldw = (None, 0) if weights is None else _rows(weights, "weights", (self.kv_heads, None))
-        if weights is not None and weights.shape[1] < len(self):
-            raise DaizaError(DZ_ERR_TENSOR, "weights of %d rows, %d held" % (weights.shape[1], len(self)))
-        s = _stream_of(q, stream)
-        w = _work(q, lib().dz_kv4_attend_work_bytes(self._h, q.shape[1], q.shape[0]), s)
-        _check(lib().dz_kv4_attend_dev(self._h, qp, ldq, _TYPES[str(q.dtype)], q.shape[1], q.shape[0],
-                                       self.head_dim ** -0.5 if scale is None else float(scale), wp, ldw, op, ldo, w.data_ptr(), s))
+        qp, ldq, ty = _rows(q, "q", (None, None, self.head_dim), _TYPES)
+        n, heads, _ = q.shape
+        op, ldo, to = _rows(out, "out", (n, heads, self.head_dim), _TYPES)
+        if ty != to:
+            raise DaizaError(DZ_ERR_TENSOR, "q of %s, out of %s" % (q.dtype, out.dtype))
+        wp, ldw = None, 0
+        if weights is not None:
+            wp, ldw, _ = _rows(weights, "weights", (self.kv_heads, None), _F32)
+            if weights.shape[1] < len(self):
+                raise DaizaError(DZ_ERR_TENSOR, "weights of %d rows, %d held" % (weights.shape[1], len(self)))
+        s, L = _call_stream(q, stream), lib()
+        w = _work(q, L.dz_kv4_attend_work_bytes(self._h, heads, n), s)
+        _check(L.dz_kv4_attend_dev(self._h, qp, ldq, ty, heads, n, self.head_dim ** -0.5 if scale is None else float(scale), wp, ldw,
+                                   op, ldo, w.data_ptr(), s))
 
     def evict_dev(self, dst, keep, recent, weights, dst_weights, kept, stream=None):
         """Copies the newest `recent` rows and the keep - recent others of the largest weights to dst, in order; kept (int32
         [kv_heads][m], m = min(keep, rows held)) receives their indices, dst_weights [kv_heads][>= m] (or None) their weights."""
         m = min(int(keep), len(self))
-        wp, ldw = _rows(weights, "weights", (self.kv_heads, None))
-        dp, ldd = (None, 0) if dst_weights is None else _rows(dst_weights, "dst_weights", (self.kv_heads, None))
+        wp, ldw, _ = _rows(weights, "weights", (self.kv_heads, None), _F32)
+        dp, ldd = None, 0
+        if dst_weights is not None:
+            dp, ldd, _ = _rows(dst_weights, "dst_weights", (self.kv_heads, None), _F32)
         if weights.shape[1] < len(self) or (dst_weights is not None and dst_weights.shape[1] < m):
             raise DaizaError(DZ_ERR_TENSOR, "evict: fewer weights than rows")
-        kp, ldk = _rows(kept, "kept", (self.kv_heads, m), ("torch.int32",))
-        if not kept.is_contiguous():
-            raise DaizaError(DZ_ERR_TENSOR, "kept is not contiguous")
-        _check(lib().dz_kv4_evict_dev(self._h, wp, ldw, int(keep), int(recent), dst._h, dp, ldd, kp, _stream_of(weights, stream)))
+        kp = _rows(kept, "kept", (self.kv_heads, max(0, m)), _I32, True)[0]
+        _check(lib().dz_kv4_evict_dev(self._h, wp, ldw, int(keep), int(recent), dst._h, dp, ldd, kp, _call_stream(weights, stream)))
 
 
 def logprobs_dev(logits, tokens=None, logp=None, entropy=None, top_ids=None, top_logp=None, stream=None):
     """Of rows of logits [n][vocab] (a torch tensor on the device, float32, float16 or bfloat16, any stride between rows): the
     log probabilities logp [n] of tokens [n] (int32), the entropies [n] in nats, and the ids (int32) and log probabilities
     of the top_ids.shape[1] best tokens, larger first, the lower id first among equal ones.  Every output may be None."""
-    lp, ld = _rows(logits, "logits", (None, None), _TYPES)
+    if _torch is None:
+        _use_torch()
+    lp, ld, ty = _rows(logits, "logits", (None, None), _TYPES)
     n, vocab = logits.shape
     top = 0 if top_ids is None else top_ids.shape[1]
-    ptr = {}
-    for what, t, shape, ty in (("tokens", tokens, (n,), "torch.int32"), ("logp", logp, (n,), "torch.float32"),
-                               ("entropy", entropy, (n,), "torch.float32"), ("top_ids", top_ids, (n, top), "torch.int32"),
-                               ("top_logp", top_logp, (n, top), "torch.float32")):
-        if t is not None:
-            _rows(t, what, shape, (ty,))
-            if not t.is_contiguous():
-                raise DaizaError(DZ_ERR_TENSOR, "%s is not contiguous" % what)
-        ptr[what] = None if t is None else t.data_ptr()
-    s = _stream_of(logits, stream)
-    w = _work(logits, lib().dz_logprobs_work_bytes(n, vocab, top), s)
-    _check(lib().dz_logprobs_dev(lp, ld, _TYPES[str(logits.dtype)], n, vocab, ptr["tokens"], top, ptr["logp"], ptr["entropy"],
-                                 ptr["top_ids"], ptr["top_logp"], w.data_ptr(), s))
+    tp = None if tokens is None else _rows(tokens, "tokens", (n,), _I32, True)[0]
+    gp = None if logp is None else _rows(logp, "logp", (n,), _F32, True)[0]
+    ep = None if entropy is None else _rows(entropy, "entropy", (n,), _F32, True)[0]
+    ip = None if top_ids is None else _rows(top_ids, "top_ids", (n, top), _I32, True)[0]
+    tl = None if top_logp is None else _rows(top_logp, "top_logp", (n, top), _F32, True)[0]
+    s, L = _call_stream(logits, stream), lib()
+    w = _work(logits, L.dz_logprobs_work_bytes(n, vocab, top), s)
+    _check(L.dz_logprobs_dev(lp, ld, ty, n, vocab, tp, top, gp, ep, ip, tl, w.data_ptr(), s))

@@ -30,44 +30,54 @@ static int with_head_dim(int hd, F&& f) {
 
 // ---------------------------------------------------------------- rows in and out
 
-// One row of one head of keys (z = 0) or values (z = 1) per workgroup, a thread per dim: a block's 32 threads find its
-// largest value, the codes meet in LDS and leave in the layout's words.  Grid (n, nkv, 2), HD threads.
-template <int HD, class E>
-__global__ __launch_bounds__(HD) void kv4_append_kernel(Kv4View c, int row0, const E* __restrict__ k, int64_t ldk,
-                                                        const E* __restrict__ v, int64_t ldv) {
-  constexpr int T = HD / 32;
-  __shared__ uint8_t code[HD];
-  const int d = threadIdx.x, g = blockIdx.y;
-  const int64_t r = (int64_t)row0 + blockIdx.x;
-  const bool values = blockIdx.z != 0;
-  const float x = to_f32((values ? v + (size_t)blockIdx.x * ldv : k + (size_t)blockIdx.x * ldk)[(size_t)g * HD + d]);
-  unsigned big = __float_as_uint(x) & 0x7FFFFFFFu;  // as whole numbers: a NaN is larger than every number
+// Four consecutive elements from an address of the element's own alignment.
+template <class E>
+__device__ __forceinline__ void load4(const E* p, float (&x)[4]) {
+  struct __attribute__((packed, aligned(sizeof(E)))) Raw {
+    E e[4];
+  };
+  const Raw r = *reinterpret_cast<const Raw*>(p);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, o));
+  for (int i = 0; i < 4; ++i) x[i] = to_f32(r.e[i]);
+}
+
+constexpr int kKv4RowThreads = 256;
+template <int HD>
+constexpr int kv4_wg_rows() { return kKv4RowThreads / (HD / 4); }
+
+// Rows of keys (z = 0) or values (z = 1) of a head into the cache, a thread per four dims: the eight threads of a block
+// find its largest value; a thread's four codes are half a word of keys, or a byte of values for each of two lanes.
+// Grid (ceil(n / kv4_wg_rows), nkv, 2), 256 threads.
+template <int HD, class E>
+__global__ __launch_bounds__(kKv4RowThreads) void kv4_append_kernel(Kv4View c, int row0, int n, const E* __restrict__ k, int64_t ldk,
+                                                                    const E* __restrict__ v, int64_t ldv) {
+  constexpr int T = HD / 32, D4 = HD / 4;
+  const int a = (int)threadIdx.x % D4, g = blockIdx.y, b = a / 8;
+  const int64_t i = (int64_t)blockIdx.x * kv4_wg_rows<HD>() + threadIdx.x / D4, r = row0 + i;
+  if (i >= n) return;  // all lanes of a block at once
+  const bool values = blockIdx.z != 0;
+  float x[4];
+  load4((values ? v + (size_t)i * ldv : k + (size_t)i * ldk) + (size_t)g * HD + 4 * a, x);
+  unsigned big = 0;  // as whole numbers: a NaN is larger than every number
+#pragma unroll
+  for (int j = 0; j < 4; ++j) big = max(big, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, o));
   const int sb = kv4_scale_byte(__uint_as_float(big));
-  code[d] = (uint8_t)kv4_code(x, sb);
-  if ((d & 31) == 0) {
-    (values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + d / 32] = (uint8_t)sb;
+  unsigned code = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) code |= kv4_code(x[j], sb) << (4 * j);
+  if (a % 8 == 0) {
+    (values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + b] = (uint8_t)sb;
     if (sb == 255) c.bad[(size_t)g * (c.cap / kKv4Tile) + r / kKv4Tile] = 1;
   }
-  __syncthreads();
   if (!values) {
-    if (d < HD / 8) {
-      const int lk = d / T, b = d % T;
-      unsigned w = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w |= (unsigned)code[32 * b + 8 * lk + i] << (4 * i);
-      *reinterpret_cast<unsigned*>(c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 4 * d) = w;
-    }
-  } else if (d < 16) {
-    uint8_t* p = c.vc + g * c.code_head() + kv4_value_offset<HD>(r, d);
-    unsigned short* w = reinterpret_cast<unsigned short*>(p);
-#pragma unroll
-    for (int t = 0; t < T; t += 2) {
-      const unsigned a = code[32 * t + 2 * d] | (unsigned)code[32 * t + 2 * d + 1] << 4;
-      const unsigned b = code[32 * t + 32 + 2 * d] | (unsigned)code[32 * t + 33 + 2 * d] << 4;
-      w[t / 2] = (unsigned short)(a | b << 8);
-    }
+    uint8_t* p = c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 4 * (((a % 8) / 2) * T + b) + 2 * (a & 1);
+    *reinterpret_cast<unsigned short*>(p) = (unsigned short)code;
+  } else {
+    uint8_t* p = c.vc + g * c.code_head() + kv4_value_offset<HD>(r, 2 * (a % 8)) + b;
+    p[0] = (uint8_t)code;
+    p[16] = (uint8_t)(code >> 8);
   }
 }
 
@@ -77,30 +87,42 @@ __device__ __forceinline__ float kv4_grid(unsigned code) {
   return code & 8u ? -a : a;
 }
 
-// The values of rows start + blockIdx.x, f32 [kv head][n][HD].  Grid (n, nkv, 2), HD threads.
+// The values of rows start .. start + n, f32 [kv head][n][HD], a thread per four dims.
+// Grid (ceil(n / kv4_wg_rows), nkv, 2), 256 threads.
 template <int HD>
-__global__ __launch_bounds__(HD) void kv4_read_kernel(Kv4View c, int start, int n, float* __restrict__ k, float* __restrict__ v) {
-  constexpr int T = HD / 32;
-  const int d = threadIdx.x, g = blockIdx.y, t = d / 32, in = d % 32;
-  const int64_t r = (int64_t)start + blockIdx.x;
+__global__ __launch_bounds__(kKv4RowThreads) void kv4_read_kernel(Kv4View c, int start, int n, float* __restrict__ k,
+                                                                  float* __restrict__ v) {
+  constexpr int T = HD / 32, D4 = HD / 4;
+  const int a = (int)threadIdx.x % D4, g = blockIdx.y, b = a / 8;
+  const int64_t i = (int64_t)blockIdx.x * kv4_wg_rows<HD>() + threadIdx.x / D4, r = start + i;
   const bool values = blockIdx.z != 0;
   float* out = values ? v : k;
-  if (!out) return;
-  const size_t ch = g * c.code_head();
-  unsigned byte;
-  if (values) byte = c.vc[ch + kv4_value_offset<HD>(r, in / 2) + t];
-  else byte = c.kc[ch + (size_t)r * (HD / 2) + 4 * ((in / 8) * T + t) + (in % 8) / 2];
-  const unsigned code = (byte >> (4 * (d & 1))) & 15u;
-  const unsigned sb = (values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + t];
-  out[((size_t)g * n + blockIdx.x) * HD + d] = kv4_grid(code) * kv4_scale(sb);
+  if (!out || i >= n) return;
+  unsigned code;
+  if (values) {
+    const uint8_t* p = c.vc + g * c.code_head() + kv4_value_offset<HD>(r, 2 * (a % 8)) + b;
+    code = p[0] | (unsigned)p[16] << 8;
+  } else {
+    code = *reinterpret_cast<const unsigned short*>(c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 4 * (((a % 8) / 2) * T + b) +
+                                                    2 * (a & 1));
+  }
+  const float s = kv4_scale((values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + b]);
+  struct __attribute__((packed, aligned(4))) Four {
+    float x[4];
+  };
+  Four y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y.x[j] = kv4_grid((code >> (4 * j)) & 15u) * s;
+  *reinterpret_cast<Four*>(out + ((size_t)g * n + i) * HD + 4 * a) = y;
 }
 
 int kv4_append(const Kv4View& c, int row0, const void* k, int64_t ldk, const void* v, int64_t ldv, int type, int n, hipStream_t s) {
   return with_head_dim(c.hd, [&](auto D) {
-    constexpr int HD = decltype(D)::value;
+    constexpr int HD = decltype(D)::value, W = kv4_wg_rows<HD>();
     return with_type(type, [&](auto* e) -> int {
       using E = std::remove_pointer_t<decltype(e)>;
-      kv4_append_kernel<HD, E><<<dim3((unsigned)n, (unsigned)c.nkv, 2), HD, 0, s>>>(c, row0, (const E*)k, ldk, (const E*)v, ldv);
+      kv4_append_kernel<HD, E><<<dim3((unsigned)((n + W - 1) / W), (unsigned)c.nkv, 2), kKv4RowThreads, 0, s>>>(
+          c, row0, n, (const E*)k, ldk, (const E*)v, ldv);
       DZ_HIP_CHECK(hipGetLastError());
       return DZ_OK;
     });
@@ -109,8 +131,8 @@ int kv4_append(const Kv4View& c, int row0, const void* k, int64_t ldk, const voi
 
 int kv4_read(const Kv4View& c, int start, int n, float* k, float* v, hipStream_t s) {
   return with_head_dim(c.hd, [&](auto D) -> int {
-    constexpr int HD = decltype(D)::value;
-    kv4_read_kernel<HD><<<dim3((unsigned)n, (unsigned)c.nkv, 2), HD, 0, s>>>(c, start, n, k, v);
+    constexpr int HD = decltype(D)::value, W = kv4_wg_rows<HD>();
+    kv4_read_kernel<HD><<<dim3((unsigned)((n + W - 1) / W), (unsigned)c.nkv, 2), kKv4RowThreads, 0, s>>>(c, start, n, k, v);
     DZ_HIP_CHECK(hipGetLastError());
     return DZ_OK;
   });
@@ -737,48 +759,103 @@ __device__ __forceinline__ unsigned weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+constexpr int kKv4Held = 32;  // keys a thread of the selection holds
+
 // kept[g] of head g: the `take` rows of [0, old) with the largest keys (the lower row first among equal ones), then the rows
-// [old, old + recent), in ascending order.  The key of the take-th largest is found byte by byte from the top
-// (a histogram of the keys that share the bytes found so far); then every wave counts and writes its span in order.
-// Grid (nkv), 1024 threads.
+// [old, old + recent), in ascending order.  Each wave has a span of the rows; the key of the take-th largest is
+// found 11, 11 and 10 bits at a time from the top, by a histogram of the keys that share the bits found so far; then every
+// wave counts and writes its span in order.  HELD: the keys stay in registers (old <= 32768), else they are read anew.
+// Bound by latency: one workgroup a head.  Grid (nkv), 1024 threads.
+template <bool HELD>
 __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restrict__ w, int64_t ldw, int old, int take, int recent,
                                                           int32_t* __restrict__ kept) {
-  __shared__ unsigned hist[256], wsum[16][2], s_prefix, s_left;
+  __shared__ unsigned hist[2048], wsum[16][2], wtot[16], s_prefix, s_left;
   const unsigned tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
   const int g = blockIdx.x, m = take + recent;
   w += (size_t)g * ldw;
   kept += (size_t)g * m;
   for (int i = (int)tid; i < recent; i += 1024) kept[take + i] = old + i;
   if (take == 0) return;
-  unsigned prefix = 0, left = (unsigned)take;  // the key's bytes so far; how many rows come from the keys that share them
-  for (int sh = 24; sh >= 0; sh -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = (int)tid; i < old; i += 1024) {
-      const unsigned k = weight_key(w[i]);
-      if (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(k >> sh) & 255u], 1u);
+  const int span = (old + 1023) / 1024 * 64, b0 = (int)wv * span, b1 = min(old, b0 + span);
+  unsigned held[HELD ? kKv4Held : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kKv4Held; ++j) {
+      const int r = b0 + 64 * j + (int)lane;
+      held[j] = r < b1 ? __float_as_uint(w[r]) : 0u;
     }
+#pragma unroll
+    for (int j = 0; j < kKv4Held; ++j) held[j] = weight_key(__uint_as_float(held[j]));
+  }
+  // f(row, key, whether there is one) for the wave's rows, 64 at a time, in order
+  auto rows = [&](auto&& f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < kKv4Held; ++j) {
+        if (b0 + 64 * j >= b1) break;
+        const int r = b0 + 64 * j + (int)lane;
+        f(r, held[j], r < b1);
+      }
+    } else {
+      for (int i = b0; i < b1; i += 256) {
+        unsigned k[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = weight_key(w[min(i + 64 * j + (int)lane, b1 - 1)]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = i + 64 * j + (int)lane;
+          f(r, k[j], r < b1);
+        }
+      }
+    }
+  };
+  unsigned prefix = 0, left = (unsigned)take;  // the key's bits so far; how many rows come from the keys that share them
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, up = pass == 0 ? 32 : pass == 1 ? 21 : 10;
+    hist[tid] = hist[1024 + tid] = 0;
     __syncthreads();
-    if (tid == 0) {
-      unsigned b = 255, seen = 0;
-      while (seen + hist[b] < left) seen += hist[b--];
-      s_prefix = prefix | b << sh;
-      s_left = left - seen;
+    rows([&](int, unsigned k, bool has) {
+      const bool in = has && (pass == 0 || (k >> (up & 31)) == (prefix >> (up & 31)));
+      const unsigned long long any = __ballot(in);
+      if (!any) return;
+      const unsigned bin = (k >> sh) & (pass == 2 ? 1023u : 2047u);
+      // a wave of equal keys (rows never attended to) counts once
+      const unsigned first = (unsigned)__builtin_amdgcn_readlane((int)bin, __builtin_ctzll(any));
+      if (__ballot(in && bin == first) == any) {
+        if (lane == 0) atomicAdd(&hist[first], (unsigned)__popcll(any));
+      } else if (in) {
+        atomicAdd(&hist[bin], 1u);
+      }
+    });
+    __syncthreads();
+    // how many keys lie in the bins above a thread's two, from the top
+    const unsigned hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid], own = hi + lo;
+    unsigned up_to = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned v = (unsigned)__shfl_up((int)up_to, o);
+      if ((int)lane >= o) up_to += v;
+    }
+    if (lane == 63) wtot[wv] = up_to;
+    __syncthreads();
+    unsigned above = up_to - own;
+    for (unsigned i = 0; i < wv; ++i) above += wtot[i];
+    if (above < left && above + own >= left) {
+      const bool h = above + hi >= left;
+      s_prefix = prefix | (h ? 2047u - 2 * tid : 2046u - 2 * tid) << sh;
+      s_left = left - above - (h ? 0u : hi);
     }
     __syncthreads();
     prefix = s_prefix;
     left = s_left;
-    __syncthreads();
   }
   // rows above the key, and the first `left` rows at it
-  const int span = (old + 1023) / 1024 * 64, b0 = (int)wv * span, b1 = min(old, b0 + span);
   unsigned above = 0, at = 0;
-  for (int i = b0; i < b1; i += 64) {
-    const int r = i + (int)lane;
-    const unsigned k = r < b1 ? weight_key(w[r]) : 0u;
-    above += (unsigned)__popcll(__ballot(r < b1 && k > prefix));
-    at += (unsigned)__popcll(__ballot(r < b1 && k == prefix));
-  }
+  rows([&](int, unsigned k, bool has) {
+    above += (unsigned)__popcll(__ballot(has && k > prefix));
+    at += (unsigned)__popcll(__ballot(has && k == prefix));
+  });
   if (lane == 0) {
     wsum[wv][0] = above;
     wsum[wv][1] = at;
@@ -789,43 +866,60 @@ __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restric
     above += wsum[i][0];
     at += wsum[i][1];
   }
-  for (int i = b0; i < b1; i += 64) {
-    const int r = i + (int)lane;
-    const unsigned k = r < b1 ? weight_key(w[r]) : 0u;
-    const unsigned long long ba = __ballot(r < b1 && k > prefix), bt = __ballot(r < b1 && k == prefix);
+  rows([&](int r, unsigned k, bool has) {
+    const unsigned long long ba = __ballot(has && k > prefix), bt = __ballot(has && k == prefix);
     const unsigned long long below = (1ull << lane) - 1;
     const unsigned ra = above + (unsigned)__popcll(ba & below), rt = at + (unsigned)__popcll(bt & below);
-    if (r < b1 && (k > prefix || (k == prefix && rt < left))) kept[ra + min(rt, left)] = r;
+    if (has && (k > prefix || (k == prefix && rt < left))) kept[ra + min(rt, left)] = r;
     above += (unsigned)__popcll(ba);
     at += (unsigned)__popcll(bt);
-  }
+  });
 }
 
-// Row kept[g][i] of c -> row i of dst, with its weight.  Grid (ceil(m / 4), nkv), 256 threads, a wave per row.
+// Rows kept[g] of c -> the rows of dst, with their weights: a tile of 32 rows of dst per workgroup, its loads all under way
+// at once.  Grid (ceil(m / 32), nkv), 256 threads.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_gather_kernel(Kv4View c, Kv4View dst, const int32_t* __restrict__ kept, int m,
                                                          const float* __restrict__ w, int64_t ldw, float* __restrict__ dw,
                                                          int64_t ld_dw) {
-  constexpr int T = HD / 32;
-  const int g = blockIdx.y, i = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (i >= m) return;
-  const int64_t r = kept[(size_t)g * m + i];
+  constexpr int T = HD / 32, KU = HD / 32, NK = 32 * KU / 256 > 0 ? 32 * KU / 256 : 1;  // KU: 16-byte units of a row's keys
   typedef uint8_t bytes __attribute__((ext_vector_type(T)));
-  if (lane < HD / 8)
-    reinterpret_cast<unsigned*>(dst.kc + g * dst.code_head() + (size_t)i * (HD / 2))[lane] =
-        reinterpret_cast<const unsigned*>(c.kc + g * c.code_head() + (size_t)r * (HD / 2))[lane];
-  else if (lane < HD / 8 + 16) {
-    const int ln = lane - HD / 8;
-    *reinterpret_cast<bytes*>(dst.vc + g * dst.code_head() + kv4_value_offset<HD>(i, ln)) =
-        *reinterpret_cast<const bytes*>(c.vc + g * c.code_head() + kv4_value_offset<HD>(r, ln));
-  } else if (lane == 48)
-    *reinterpret_cast<bytes*>(dst.ks + g * dst.scale_head() + (size_t)i * T) =
-        *reinterpret_cast<const bytes*>(c.ks + g * c.scale_head() + (size_t)r * T);
-  else if (lane == 49)
-    *reinterpret_cast<bytes*>(dst.vs + g * dst.scale_head() + (size_t)i * T) =
-        *reinterpret_cast<const bytes*>(c.vs + g * c.scale_head() + (size_t)r * T);
-  else if (lane == 50 && dw)
-    dw[(size_t)g * ld_dw + i] = w[(size_t)g * ldw + r];
+  __shared__ int src[32];
+  const int g = blockIdx.y, i0 = (int)blockIdx.x * 32, tid = threadIdx.x, nr = min(32, m - i0);
+  if (tid < 32) src[tid] = kept[(size_t)g * m + min(i0 + tid, m - 1)];
+  __syncthreads();
+  const uint8_t *kc = c.kc + g * c.code_head(), *vc = c.vc + g * c.code_head();
+  uint8_t *dkc = dst.kc + g * dst.code_head(), *dvc = dst.vc + g * dst.code_head();
+  u32x4 kk[NK];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) {
+    const int u = tid + 256 * j, q = min(u / KU, nr - 1);
+    kk[j] = *reinterpret_cast<const u32x4*>(kc + (size_t)src[q] * (HD / 2) + 16 * (u % KU));
+  }
+  bytes vv[2];  // of row (tid + 256 j) / 16, lane tid % 16
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    vv[j] = *reinterpret_cast<const bytes*>(vc + kv4_value_offset<HD>(src[min((tid + 256 * j) / 16, nr - 1)], tid % 16));
+  const int q = tid & 31, what = tid >> 5;  // 0: the keys' scales, 1: the values', 2: the weight
+  if (q < nr && what < 2) {
+    const bytes e = *reinterpret_cast<const bytes*>((what ? c.vs : c.ks) + g * c.scale_head() + (size_t)src[q] * T);
+    *reinterpret_cast<bytes*>((what ? dst.vs : dst.ks) + g * dst.scale_head() + (size_t)(i0 + q) * T) = e;
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < T; ++t) bad |= e[t] == 255;
+    if (bad) dst.bad[(size_t)g * (dst.cap / kKv4Tile) + (i0 + q) / kKv4Tile] = 1;
+  }
+  if (q < nr && what == 2 && dw) dw[(size_t)g * ld_dw + i0 + q] = w[(size_t)g * ldw + src[q]];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) {
+    const int u = tid + 256 * j;
+    if (u / KU < nr) *reinterpret_cast<u32x4*>(dkc + (size_t)(i0 + u / KU) * (HD / 2) + 16 * (u % KU)) = kk[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = (tid + 256 * j) / 16;
+    if (r < nr) *reinterpret_cast<bytes*>(dvc + kv4_value_offset<HD>(i0 + r, tid % 16)) = vv[j];
+  }
 }
 
 int kv4_evict(const Kv4View& c, int len, const float* weights, int64_t ldw, int keep, int recent, const Kv4View& dst,
@@ -833,12 +927,16 @@ int kv4_evict(const Kv4View& c, int len, const float* weights, int64_t ldw, int 
   const int m = std::min(keep, len);
   if (m == 0) return DZ_OK;
   recent = std::min(recent, len);
-  kv4_select_kernel<<<dim3((unsigned)c.nkv), 1024, 0, s>>>(weights, ldw, len - recent, m - recent, recent, kept);
+  const int old = len - recent;
+  if (old <= 1024 * kKv4Held)
+    kv4_select_kernel<true><<<dim3((unsigned)c.nkv), 1024, 0, s>>>(weights, ldw, old, m - recent, recent, kept);
+  else
+    kv4_select_kernel<false><<<dim3((unsigned)c.nkv), 1024, 0, s>>>(weights, ldw, old, m - recent, recent, kept);
   DZ_HIP_CHECK(hipGetLastError());
   return with_head_dim(c.hd, [&](auto D) -> int {
     constexpr int HD = decltype(D)::value;
-    kv4_gather_kernel<HD><<<dim3((unsigned)((m + 3) / 4), (unsigned)c.nkv), 256, 0, s>>>(c, dst, kept, m, weights, ldw,
-                                                                                          dst_weights, ld_dst);
+    kv4_gather_kernel<HD><<<dim3((unsigned)((m + 31) / 32), (unsigned)c.nkv), 256, 0, s>>>(c, dst, kept, m, weights, ldw,
+                                                                                            dst_weights, ld_dst);
     DZ_HIP_CHECK(hipGetLastError());
     return DZ_OK;
   });
