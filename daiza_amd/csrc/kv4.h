@@ -21,7 +21,7 @@
 namespace dz {
 
 constexpr int kKv4Tile = 32;  // rows of a tile
-constexpr int kKv4MaxChunks = 512;
+constexpr int kKv4MaxChunks = 256;  // a thread of the merge each
 constexpr int kKv4MinExp = -120, kKv4MaxExp = 125;  // 6 · 2^125 is the largest f32 of the format
 
 struct Kv4View {

@@ -209,7 +209,10 @@ struct KeyWords {
   static constexpr int T = HD / 32;
   unsigned code[2][T];           // rows 16h + ln: dims 32b + 8lk .. +7
   unsigned scale[2][(T + 3) / 4];
-  __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ks, int64_t row, int ln, int lk) {
+  unsigned odd;  // the tile may hold blocks that are not numbers
+  // The flag comes with the tile: loads return in order, so one issued at its use would wait for the tiles requested since.
+  __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ks, const uint8_t* bad, int64_t row, int ln, int lk) {
+    odd = bad[row >> 5];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t r = row + 16 * h + ln;
@@ -275,44 +278,63 @@ struct ValueWords {
   }
   // Blocks that are not numbers count as zeros from here on (their codes are zeros); first[t] becomes the first row of
   // the tile, at `row`, with such a block t, if that is earlier.
-  __device__ __forceinline__ void take_bad(int64_t row, int lk, int (&first)[T]) {
+  __device__ __forceinline__ void take_bad(int row, int lk, int (&first)[T]) {
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+    for (int t = 0; t < T; ++t) {
+      int at = 0x7FFFFFFF;
 #pragma unroll
       for (int j = 7; j >= 0; --j) {
         const int s = (j & 3) * T + t;
-        unsigned& w = scale[j >> 2][s / 4];
-        const bool bad = ((w >> (8 * (s % 4))) & 255u) == 255u;
-        const unsigned long long m = __ballot(bad);
-        if (bad) w ^= 0x80u << (8 * (s % 4));  // 127
-        if (m) first[t] = min(first[t], (int)row + 16 * (j >> 2) + 4 * (__builtin_ctzll(m) >> 4) + (j & 3));
+        if (((scale[j >> 2][s / 4] >> (8 * (s % 4))) & 255u) == 255u) at = row + 16 * (j >> 2) + 4 * lk + (j & 3);
       }
+      at = min(at, __shfl_xor(at, 16));
+      at = min(at, __shfl_xor(at, 32));
+      first[t] = min(first[t], at);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < T; ++i)  // bytes of 255 become 127
+        scale[h][i] ^= ((scale[h][i] & 0x7F7F7F7Fu) + 0x01010101u) & scale[h][i] & 0x80808080u;
   }
 };
 
 // The query rows of a workgroup, row ρ = token · grp + head of the group, as operands in LDS: [row tile][block][part]
-// [lane][16 B], lane 16·lk + ln holding dims 32b + 8lk .. +7 of the tile's row ln.
-template <int HD, class E>
-__device__ __forceinline__ void stage_queries(u32x4* lds, int tiles, const E* __restrict__ q, int64_t ldq, int head0, int grp,
-                                              int row0, int rows, unsigned tid, unsigned nt) {
-  constexpr int T = HD / 32, QP = Parts<E>::q;
-  for (unsigned u = tid; u < (unsigned)(tiles * T * 64); u += nt) {
-    const int lane = (int)(u & 63u), b = (int)((u >> 6) % T), tile = (int)((u >> 6) / T);
-    const int rho = row0 + 16 * tile + (lane & 15);
-    float x[8];
+// [lane][16 B], lane 16·lk + ln holding dims 32b + 8lk .. +7 of the tile's row ln.  Requested and stored apart, for
+// other loads to be on their way in between.
+template <int HD, class E, int TILES, int NT>
+struct QueryStage {
+  static constexpr int T = HD / 32, QP = Parts<E>::q, N = (TILES * T * 64 + NT - 1) / NT;
+  E x[N][8];
+  __device__ __forceinline__ void load(const E* __restrict__ q, int64_t ldq, int head0, int grp, int row0, int rows, int tid) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (rho < rows) {
-      const E* p = q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD + 32 * b + 8 * (lane >> 4);
+    for (int i = 0; i < N; ++i) {
+      const int u = tid + i * NT, lane = u & 63, b = (u >> 6) % T, tile = (u >> 6) / T;
+      const int rho = min(row0 + 16 * tile + (lane & 15), rows - 1);  // a row past the last is the last one again: not used
+      struct __attribute__((packed, aligned(sizeof(E)))) Raw {
+        E e[8];
+      };
+      const Raw r = *reinterpret_cast<const Raw*>(q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD + 32 * b +
+                                                  8 * (lane >> 4));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+      for (int j = 0; j < 8; ++j) x[i][j] = r.e[j];
     }
-    u32x4 part[QP];
-    split8<QP>(x, part);
-#pragma unroll
-    for (int k = 0; k < QP; ++k) lds[((tile * T + b) * QP + k) * 64 + lane] = part[k];
   }
-}
+  __device__ __forceinline__ void store(u32x4* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int u = tid + i * NT, lane = u & 63, b = (u >> 6) % T, tile = (u >> 6) / T;
+      if (N * NT != TILES * T * 64 && u >= TILES * T * 64) break;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_f32(x[i][j]);
+      u32x4 part[QP];
+      split8<QP>(v, part);
+#pragma unroll
+      for (int k = 0; k < QP; ++k) lds[((tile * T + b) * QP + k) * 64 + lane] = part[k];
+    }
+  }
+};
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -322,39 +344,67 @@ struct AttendOut {
   float2* stats;  // [n][nq] (m, l), or null
 };
 
+// The largest (sum) of x over the four lanes ln, ln + 16, ln + 32, ln + 48.
+__device__ __forceinline__ float max_over_lk(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_over_lk(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 // Causal attention of the n·grp query rows of a key/value head on the matrix cores.  Scores as S^T = K · Q^T: the operand
 // of the keys is the dequantised block itself (a block of 32 dims is one 16x16x32 instruction), that of the queries comes from LDS;
 // lane (ln, lk) gets the scores of row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that order, its
 // part of the operand P of O += P · V.  Dequantising is exact, queries and probabilities are sums of bf16 operands
 // (Parts), so products are those of f32 values and the sums f32.
 //
-// ROWS16: up to 16 rows; the workgroup's four waves take the chunk's tiles of 32 positions in turn and their results meet in
-// LDS.  Otherwise a workgroup has 64 rows, 16 a wave, and every wave all of the chunk's tiles.
-// Grid: (row tiles x key/value heads x chunks), 256 threads.
-template <int HD, class E, bool ROWS16>
-__global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq, int n,
-                                                            float scale, int csz, int nch, AttendOut dst, E* __restrict__ out,
-                                                            int64_t ldo) {
-  constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p;
+// A workgroup has RT tiles of 16 rows and PS waves for each, which take the chunk's tiles of 32 positions in turn, each a
+// tile ahead with its loads; their results meet in LDS at the end.  Two waves a SIMD, so that one's dequantising (about 400
+// vector instructions a tile) runs beside the other's matrix instructions (96 of 16 cycles with f32 queries).
+// Grid: row tiles x key/value heads x chunks; 64 RT PS threads.
+template <int HD, class E, int RT, int PS>
+__global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq,
+                                                                     int n, float scale, int csz, int nch, AttendOut dst,
+                                                                     E* __restrict__ out, int64_t ldo) {
+  constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p, NT = 64 * RT * PS;
   extern __shared__ __align__(16) uint8_t smem[];
   u32x4* qs = reinterpret_cast<u32x4*>(smem);
-  const int grp = nq / c.nkv, rows = n * grp, ntile = ROWS16 ? 1 : (rows + 63) / 64;
+  const int grp = nq / c.nkv, rows = n * grp, ntile = (rows + 16 * RT - 1) / (16 * RT);
   const int pairs = c.nkv * nch, pair = (int)blockIdx.x % pairs;
   const int tile = ntile - 1 - (int)blockIdx.x / pairs, g = pair % c.nkv, z = pair / c.nkv;
-  const unsigned tid = threadIdx.x, lane = tid & 63u, w = tid >> 6;
+  const unsigned tid = threadIdx.x, lane = tid & 63u;
+  const int w = __builtin_amdgcn_readfirstlane((int)(tid >> 6)), rt = w % RT, turn = w / RT;
   const int ln = (int)(lane & 15u), lk = (int)(lane >> 4);
-  const int row0 = ROWS16 ? 0 : 64 * tile, wrow = ROWS16 ? 0 : row0 + 16 * (int)w;
+  const int row0 = 16 * RT * tile, wrow = row0 + 16 * rt;
   const int before = len - n;
   // the positions that any row of the workgroup (of the wave) sees in the chunk
-  const int last_row = min(ROWS16 ? rows : row0 + 64, rows) - 1, wlast = min(wrow + 16, rows) - 1;
+  const int last_row = min(row0 + 16 * RT, rows) - 1, wlast = min(wrow + 16, rows) - 1;
   const int pbeg = z * csz, pend = min(min((z + 1) * csz, len), before + last_row / grp + 1);
   const int wend = wrow < rows ? min(pend, before + wlast / grp + 1) : pbeg;
   const int wmin = wrow < rows ? before + wrow / grp + 1 : 0;  // what the wave's first row sees
   const int rho = wrow + ln;
   const int ctx = rho < rows ? before + rho / grp + 1 : 0;
-  if (pbeg < pend) stage_queries<HD, E>(qs, ROWS16 ? 1 : 4, q, ldq, g * grp, grp, row0, rows, tid, 256);
+  const uint8_t *kc = c.kc + g * c.code_head(), *vc = c.vc + g * c.code_head();
+  const uint8_t *ks = c.ks + g * c.scale_head(), *vs = c.vs + g * c.scale_head();
+  const uint8_t* bad = c.bad + (size_t)g * (c.cap / kKv4Tile);
+  constexpr int step = 32 * PS;
+  const int p_first = pbeg + 32 * turn;
+  KeyWords<HD> kw;
+  ValueWords<HD> vw;
+  QueryStage<HD, E, RT, NT> queries;
+  queries.load(q, ldq, g * grp, grp, row0, rows, (int)tid);
+  if (p_first < wend) {
+    kw.load(kc, ks, bad, p_first, ln, lk);
+    vw.load(vc, vs, p_first, (int)lane);
+  }
+  queries.store(qs, (int)tid);
   __syncthreads();
-  const u32x4* qw = qs + (ROWS16 ? 0 : (int)w * T * QP * 64) + lane;
   f32x4 o[2 * T];
 #pragma unroll
   for (int t = 0; t < 2 * T; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -362,26 +412,19 @@ __global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, 
   int first[T];  // first position seen whose value block t is not a number
 #pragma unroll
   for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
-  const uint8_t *kc = c.kc + g * c.code_head(), *vc = c.vc + g * c.code_head();
-  const uint8_t *ks = c.ks + g * c.scale_head(), *vs = c.vs + g * c.scale_head();
-  const uint8_t* bad = c.bad + (size_t)g * (c.cap / kKv4Tile);
-  const int step = ROWS16 ? 128 : 32;
-  int p0 = pbeg + (ROWS16 ? 32 * (int)w : 0);
-  KeyWords<HD> kw;
-  ValueWords<HD> vw;
-  if (p0 < wend) {
-    kw.load(kc, ks, p0, ln, lk);
-    vw.load(vc, vs, p0, (int)lane);
-  }
-  for (; p0 < wend; p0 += step) {
-    const bool odd = bad[p0 >> 5] != 0;
+  unsigned qoff = (unsigned)(rt * T * QP * 64) + lane;
+  for (int p0 = p_first; p0 < wend; p0 += step) {
+    const int pn = p0 + step < wend ? p0 + step : p0;  // past the last tile: not used
+    const bool odd = __builtin_amdgcn_readfirstlane((int)kw.odd) != 0;
+    // the queries are read from LDS anew for every tile: in registers they would cost the second wave its place
+    asm volatile("" : "+v"(qoff));
     f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int b = 0; b < T; ++b) {
       const u32x4 k0 = kw.operand(0, b), k1 = kw.operand(1, b);
 #pragma unroll
       for (int k = 0; k < QP; ++k) {
-        const u32x4 qq = qw[(b * QP + k) * 64];
+        const u32x4 qq = qs[qoff + (b * QP + k) * 64];
         s[0] = mfma(k0, qq, s[0]);
         s[1] = mfma(k1, qq, s[1]);
       }
@@ -395,16 +438,13 @@ __global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, 
       for (int j = 0; j < 8; ++j)
         if (((j < 4 ? b0 : b1) >> (4 * lk + (j & 3))) & 1u) x[j] = __builtin_nanf("");
     }
-    const int pn = p0 + step < wend ? p0 + step : p0;
-    kw.load(kc, ks, pn, ln, lk);
+    kw.load(kc, ks, bad, pn, ln, lk);
     if (p0 + 32 > wmin) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
     }
-    float bm = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    bm = fmaxf(bm, __shfl_xor(bm, 16));
-    bm = fmaxf(bm, __shfl_xor(bm, 32));
+    const float bm = max_over_lk(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
     const float mn = fmaxf(m, bm);
     // a row that has seen nothing keeps m = -inf: its factor is 1 by definition, and its probabilities 0
     const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
@@ -415,9 +455,7 @@ __global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, 
       p[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
       ps += p[j];
     }
-    ps += __shfl_xor(ps, 16);
-    ps += __shfl_xor(ps, 32);
-    l = l * al + ps;
+    l = l * al + sum_over_lk(ps);
     m = mn;
     // the O rows of this lane are 4lk + i: their factors live in lanes 4lk + i
     if (__ballot(al != 1.f)) {
@@ -451,53 +489,42 @@ __global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, 
     for (int t = 0; t < T; ++t)
       if (first[t] < ci) o[2 * t][i] = o[2 * t + 1][i] = __builtin_nanf("");
   }
-  if constexpr (ROWS16) {
-    // the four waves' results: each row's largest maximum, then the sums at it
-    float* ms = reinterpret_cast<float*>(smem);  // [wave][16], over the queries, which every wave has read
-    float* os = ms + 128;                        // [wave][row][HD]
+  // the waves of a row tile: the later half's results go to the earlier half's, until one has all
+  f32x4* os = reinterpret_cast<f32x4*>(smem);  // [slot][2T][lane], over the queries, which every wave has read
+  float2* mls = reinterpret_cast<float2*>(smem + (size_t)(RT * PS / 2) * 2 * T * 1024);  // [slot][lane]
+#pragma unroll
+  for (int half = PS / 2; half > 0; half /= 2) {
     __syncthreads();
-    if (lk == 0) {
-      ms[16 * w + ln] = m;
-      ms[64 + 16 * w + ln] = l;
+    const int slot = (turn - half) * RT + rt;
+    if (turn >= half && turn < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < 2 * T; ++t) os[(slot * 2 * T + t) * 64 + lane] = o[t];
+      mls[slot * 64 + lane] = make_float2(m, l);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-        *reinterpret_cast<float2*>(os + ((size_t)w * 16 + 4 * lk + i) * HD + 32 * t + 2 * ln) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
     __syncthreads();
-    for (unsigned u = tid; u < (unsigned)(rows * (HD / 4)); u += 256) {
-      const int r = (int)(u / (HD / 4)), d = 4 * (int)(u % (HD / 4));
-      const float M = fmaxf(fmaxf(ms[r], ms[16 + r]), fmaxf(ms[32 + r], ms[48 + r]));
-      float L = 0.f;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (turn < half) {
+      const int from = turn * RT + rt;
+      const float2 ml = mls[from * 64 + lane];
+      const float M = fmaxf(m, ml.x);
+      const float ea = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - M) * kLog2e);
+      const float eb = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ml.x - M) * kLog2e);
+      l = l * ea + ml.y * eb;
+      m = M;
+      float fa[4], fb[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float mk = ms[16 * k + r], e = mk == -INFINITY && M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * kLog2e);
-        const float4 v = *reinterpret_cast<const float4*>(os + ((size_t)k * 16 + r) * HD + d);
-        L = __builtin_fmaf(ms[64 + 16 * k + r], e, L);
-        O.x = __builtin_fmaf(v.x, e, O.x);
-        O.y = __builtin_fmaf(v.y, e, O.y);
-        O.z = __builtin_fmaf(v.z, e, O.z);
-        O.w = __builtin_fmaf(v.w, e, O.w);
+      for (int i = 0; i < 4; ++i) {
+        fa[i] = __shfl(ea, 4 * lk + i);
+        fb[i] = __shfl(eb, 4 * lk + i);
       }
-      const size_t row = (size_t)(r / grp) * nq + g * grp + r % grp;
-      if (nch == 1) {
-        E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + d;
-        y[0] = from_f32<E>(O.x / L);
-        y[1] = from_f32<E>(O.y / L);
-        y[2] = from_f32<E>(O.z / L);
-        y[3] = from_f32<E>(O.w / L);
-        if (dst.stats && d == 0) dst.stats[row] = make_float2(M, L);
-      } else {
-        float* rr = dst.rec + (row * nch + z) * (2 + HD);
-        if (d == 0) *reinterpret_cast<float2*>(rr) = make_float2(M, L);
-        *reinterpret_cast<float2*>(rr + 2 + d) = make_float2(O.x, O.y);
-        *reinterpret_cast<float2*>(rr + 4 + d) = make_float2(O.z, O.w);
+#pragma unroll
+      for (int t = 0; t < 2 * T; ++t) {
+        const f32x4 v = os[(from * 2 * T + t) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][i] = o[t][i] * fa[i] + v[i] * fb[i];
       }
     }
-    return;
   }
+  if (turn) return;
   if (lk == 0 && rho < rows) {
     const size_t row = (size_t)(rho / grp) * nq + g * grp + rho % grp;
     if (nch > 1) *reinterpret_cast<float2*>(dst.rec + (row * nch + z) * (2 + HD)) = make_float2(m, l);
@@ -523,53 +550,52 @@ __global__ __launch_bounds__(256, 1) void kv4_attend_kernel(Kv4View c, int len, 
   }
 }
 
-// The chunks' records of a row (query blockIdx.x, head blockIdx.y) as its output and statistics: 4 HD threads, the
-// chunks in four quarters.  A chunk whose positions the row does not see has l = 0, m = -inf and zeros.
+// The chunks' records of a row (query blockIdx.x, head blockIdx.y) as 64 dims (blockIdx.z) of its output, and its
+// statistics: 256 threads, wave w for the w-th quarter of the chunks, 16 of its records requested at a time.  A chunk whose
+// positions the row does not see has l = 0, m = -inf and zeros.
 template <int HD, class E>
-__global__ __launch_bounds__(4 * HD) void kv4_merge_kernel(AttendOut src, int nch, int nq, E* __restrict__ out, int64_t ldo) {
-  __shared__ float fac[kKv4MaxChunks], red[4][HD + 1], mx[4 * HD / 64];
-  const unsigned tid = threadIdx.x, d = tid % HD, part = tid / HD;
+__global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, int nq, E* __restrict__ out, int64_t ldo) {
+  __shared__ float fac[kKv4MaxChunks], red[4][65], mx[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, d = (int)blockIdx.z * 64 + lane;
   const size_t row = (size_t)blockIdx.x * nq + blockIdx.y;
   const float* rec = src.rec + row * nch * (2 + HD);
-  float m = -INFINITY;
-  for (int z = (int)tid; z < nch; z += 4 * HD) m = fmaxf(m, rec[(size_t)z * (2 + HD)]);
+  const int q4 = (nch + 3) / 4, z0 = w * q4, z1 = min(nch, z0 + q4);
+  constexpr int N = 16;
+  float v[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = rec[(size_t)min(z0 + k, nch - 1) * (2 + HD) + 2 + d];
+  const float2 ml = *reinterpret_cast<const float2*>(rec + (size_t)min(tid, nch - 1) * (2 + HD));
+  float m = ml.x;
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  if ((tid & 63u) == 0) mx[tid >> 6] = m;
+  if (lane == 0) mx[w] = m;
   __syncthreads();
+  m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  const float e = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e);
+  if (tid < nch) fac[tid] = e;
+  float l = tid < nch ? ml.y * e : 0.f;
 #pragma unroll
-  for (int k = 0; k < 4 * HD / 64; ++k) m = fmaxf(m, mx[k]);
-  for (int z = (int)tid; z < nch; z += 4 * HD) {
-    const float mz = rec[(size_t)z * (2 + HD)];
-    fac[z] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mz - m) * kLog2e);
-  }
+  for (int k = 1; k < 64; k <<= 1) l += __shfl_xor(l, k);
+  if (lane == 0) red[w][64] = l;
   __syncthreads();
-  const int q4 = (nch + 3) / 4, z0 = (int)part * q4, z1 = min(nch, z0 + q4);
-  float O = 0.f, L = 0.f;
-  for (int z = z0; z < z1; z += 8) {
-    float v[8], lv[8];
+  float o = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float* rr = rec + (size_t)min(z + k, z1 - 1) * (2 + HD);
-      v[k] = rr[2 + d];
-      lv[k] = rr[1];
-    }
+  for (int k = 0; k < N; ++k)
+    if (z0 + k < z1) o = __builtin_fmaf(v[k], fac[z0 + k], o);
+  for (int z = z0 + N; z < z1; z += N) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (z + k < z1) {
-        O = __builtin_fmaf(v[k], fac[z + k], O);
-        L = __builtin_fmaf(lv[k], fac[z + k], L);
-      }
+    for (int k = 0; k < N; ++k) v[k] = rec[(size_t)min(z + k, nch - 1) * (2 + HD) + 2 + d];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (z + k < z1) o = __builtin_fmaf(v[k], fac[z + k], o);
   }
-  red[part][d] = O;
-  if (d == 0) red[part][HD] = L;
+  red[w][lane] = o;
   __syncthreads();
-  if (part == 0) {
-    O = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
-    L = (red[0][HD] + red[1][HD]) + (red[2][HD] + red[3][HD]);
-    out[(size_t)blockIdx.x * ldo + (size_t)blockIdx.y * HD + d] = from_f32<E>(O / L);
-    if (src.stats && d == 0) src.stats[row] = make_float2(m, L);
-  }
+  if (w) return;
+  l = (red[0][64] + red[1][64]) + (red[2][64] + red[3][64]);
+  o = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+  out[(size_t)blockIdx.x * ldo + (size_t)blockIdx.y * HD + d] = from_f32<E>(o / l);
+  if (src.stats && d == 0) src.stats[row] = make_float2(m, l);
 }
 
 // weights[g][r] += Σ over the group's query rows ρ of exp(s_ρr - m_ρ) / l_ρ: a wave holds the operands of 16·PT rows of keys and
@@ -588,6 +614,7 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
   const int pw = (int)blockIdx.x * 64 * PT + 16 * PT * (int)w;  // the wave's first position
   const int pblk = (int)blockIdx.x * 64 * PT;
   const uint8_t *kc = c.kc + g * c.code_head(), *ks = c.ks + g * c.scale_head();
+  const uint8_t* bad = c.bad + (size_t)g * (c.cap / kKv4Tile);
   u32x4 kop[PT][T];
   unsigned nan[PT];
 #pragma unroll
@@ -595,7 +622,7 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     KeyWords<HD> kw;
     // whole tiles of 32 rows; past the last one (a wave with nothing to do, or half a tile) the first is read instead
     const int r = pw + 16 * u, base = r < len ? r & ~31 : 0;
-    kw.load(kc, ks, base, ln, lk);
+    kw.load(kc, ks, bad, base, ln, lk);
     const int h0 = r < len ? (r >> 4) & 1 : 0;
 #pragma unroll
     for (int b = 0; b < T; ++b) {
@@ -621,8 +648,10 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
   // the first query row that sees the workgroup's first position
   const int r0 = max(0, pblk - before) * grp / 16 * 16;
   for (int row = r0; row < rows; row += 16) {
+    QueryStage<HD, E, 1, 256> queries;
+    queries.load(q, ldq, g * grp, grp, row, rows, (int)tid);
     __syncthreads();
-    stage_queries<HD, E>(qs, 1, q, ldq, g * grp, grp, row, rows, tid, 256);
+    queries.store(qs, (int)tid);
     __syncthreads();
     const int rho = row + ln;
     const bool has = rho < rows;
@@ -665,11 +694,21 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     }
 }
 
-// Chunks of positions that a call's row tiles are spread over, at most: enough workgroups to fill the device.
+// The form of the kernel that a call takes: row tiles of a workgroup, and the waves of a row tile.
+static int attend_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+template <class F>
+static int with_row_tiles(int rt, F&& f) {
+  switch (rt) {
+    case 1: return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+    case 2: return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+    default: return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+  }
+}
+// Chunks of positions that a call's row tiles are spread over, at most: as many workgroups as are resident at once.
 static int attend_max_chunks(int n, int n_head, int nkv) {
-  const int rows = n * (n_head / nkv);
-  const int tiles = (rows <= 16 ? 1 : (rows + 63) / 64) * nkv;
-  return std::max(1, std::min(kKv4MaxChunks, (rows <= 16 ? 512 : 256) / tiles));
+  const int rows = n * (n_head / nkv), rt = attend_row_tiles(rows);
+  const int tiles = (rows + 16 * rt - 1) / (16 * rt) * nkv;
+  return std::max(1, std::min(kKv4MaxChunks, 256 / tiles));
 }
 
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
@@ -677,11 +716,10 @@ size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   return (rows * sizeof(float2) + 15) / 16 * 16 + (nch > 1 ? rows * nch * (size_t)(2 + c.hd) * sizeof(float) : 0);
 }
 
-template <int HD, class E, bool ROWS16>
+template <int HD, class E, int RT, int PS>
 constexpr size_t attend_lds() {
-  constexpr size_t queries = (size_t)(ROWS16 ? 1 : 4) * (HD / 32) * Parts<E>::q * 1024;
-  constexpr size_t merge = ROWS16 ? 512 + 4 * 16 * HD * 4 : 0;
-  return queries > merge ? queries : merge;
+  constexpr size_t queries = (size_t)RT * (HD / 32) * Parts<E>::q * 1024, join = (size_t)(RT * PS / 2) * (HD / 32 * 2 * 1024 + 512);
+  return queries > join ? queries : join;
 }
 
 // Dynamic-LDS limits, set once before any launch or capture.
@@ -691,27 +729,28 @@ int prepare_kv4_kernels() {
   std::lock_guard<std::mutex> lock(mu);
   if (done) return DZ_OK;
   for (int hd : {64, 128, 256})
-    for (int type : {DZ_F32, DZ_F16, DZ_BF16}) {
-      const int rc = with_head_dim(hd, [&](auto D) {
-        constexpr int HD = decltype(D)::value;
-        return with_type(type, [&](auto* e) -> int {
-          using E = std::remove_pointer_t<decltype(e)>;
-          DZ_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kv4_attend_kernel<HD, E, true>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, true>()));
-          DZ_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kv4_attend_kernel<HD, E, false>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, false>()));
-          return DZ_OK;
+    for (int type : {DZ_F32, DZ_F16, DZ_BF16})
+      for (int rt : {1, 2, 4}) {
+        const int rc = with_head_dim(hd, [&](auto D) {
+          return with_type(type, [&](auto* e) {
+            return with_row_tiles(rt, [&](auto R, auto P) -> int {
+              using E = std::remove_pointer_t<decltype(e)>;
+              constexpr int HD = decltype(D)::value, RT = decltype(R)::value, PS = decltype(P)::value;
+              DZ_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kv4_attend_kernel<HD, E, RT, PS>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, RT, PS>()));
+              return DZ_OK;
+            });
+          });
         });
-      });
-      if (rc) return rc;
-    }
+        if (rc) return rc;
+      }
   done = true;
   return DZ_OK;
 }
 
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s) {
-  const int rows = n * (n_head / c.nkv), unit = rows <= 16 ? 128 : 32;
+  const int rows = n * (n_head / c.nkv), rt = attend_row_tiles(rows), unit = 256 / rt;  // a tile for every wave
   const int most = attend_max_chunks(n, n_head, c.nkv);
   const int csz = ((len + most - 1) / most + unit - 1) / unit * unit, nch = (len + csz - 1) / csz;
   return with_head_dim(c.hd, [&](auto D) {
@@ -722,15 +761,17 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       float2* stats = static_cast<float2*>(work);
       dst.stats = weights ? stats : nullptr;
       dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
-      if (rows <= 16)
-        kv4_attend_kernel<HD, E, true><<<dim3((unsigned)(c.nkv * nch)), 256, attend_lds<HD, E, true>(), s>>>(
+      const int rc = with_row_tiles(rt, [&](auto R, auto P) -> int {
+        constexpr int RT = decltype(R)::value, PS = decltype(P)::value;
+        const unsigned wgs = (unsigned)((rows + 16 * RT - 1) / (16 * RT) * c.nkv * nch);
+        kv4_attend_kernel<HD, E, RT, PS><<<dim3(wgs), 64 * RT * PS, attend_lds<HD, E, RT, PS>(), s>>>(
             c, len, (const E*)q, ldq, n_head, n, scale, csz, nch, dst, (E*)out, ldo);
-      else
-        kv4_attend_kernel<HD, E, false><<<dim3((unsigned)((rows + 63) / 64 * c.nkv * nch)), 256, attend_lds<HD, E, false>(), s>>>(
-            c, len, (const E*)q, ldq, n_head, n, scale, csz, nch, dst, (E*)out, ldo);
-      DZ_HIP_CHECK(hipGetLastError());
+        DZ_HIP_CHECK(hipGetLastError());
+        return DZ_OK;
+      });
+      if (rc) return rc;
       if (nch > 1) {
-        kv4_merge_kernel<HD, E><<<dim3((unsigned)n, (unsigned)n_head), 4 * HD, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
+        kv4_merge_kernel<HD, E><<<dim3((unsigned)n, (unsigned)n_head, HD / 64), 256, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
         DZ_HIP_CHECK(hipGetLastError());
       }
       if (weights) {
