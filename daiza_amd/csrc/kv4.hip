@@ -209,10 +209,7 @@ struct KeyWords {
   static constexpr int T = HD / 32;
   unsigned code[2][T];           // rows 16h + ln: dims 32b + 8lk .. +7
   unsigned scale[2][(T + 3) / 4];
-  unsigned odd;  // the tile may hold blocks that are not numbers
-  // The flag comes with the tile: loads return in order, so one issued at its use would wait for the tiles requested since.
-  __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ks, const uint8_t* bad, int64_t row, int ln, int lk) {
-    odd = bad[row >> 5];
+  __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ks, int64_t row, int ln, int lk) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int64_t r = row + 16 * h + ln;
@@ -344,6 +341,16 @@ struct AttendOut {
   float2* stats;  // [n][nq] (m, l), or null
 };
 
+// M matrix instructions with V vector instructions spread among them.
+template <int M, int V>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, (V + M - 1) / M, 0);
+  }
+}
+
 // The largest (sum) of x over the four lanes ln, ln + 16, ln + 32, ln + 48.
 __device__ __forceinline__ float max_over_lk(float x) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -399,8 +406,11 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
   ValueWords<HD> vw;
   QueryStage<HD, E, RT, NT> queries;
   queries.load(q, ldq, g * grp, grp, row0, rows, (int)tid);
+  // whether a tile of the chunk may hold blocks that are not numbers: such chunks take a loop of their own
+  unsigned flag = 0;
+  for (int p = pbeg + 32 * (int)lane; p < pend; p += 32 * 64) flag |= bad[p >> 5];
   if (p_first < wend) {
-    kw.load(kc, ks, bad, p_first, ln, lk);
+    kw.load(kc, ks, p_first, ln, lk);
     vw.load(vc, vs, p_first, (int)lane);
   }
   queries.store(qs, (int)tid);
@@ -413,81 +423,154 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
 #pragma unroll
   for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
   unsigned qoff = (unsigned)(rt * T * QP * 64) + lane;
-  for (int p0 = p_first; p0 < wend; p0 += step) {
-    const int pn = p0 + step < wend ? p0 + step : p0;  // past the last tile: not used
-    const bool odd = __builtin_amdgcn_readfirstlane((int)kw.odd) != 0;
-    // the queries are read from LDS anew for every tile: in registers they would cost the second wave its place
-    asm volatile("" : "+v"(qoff));
-    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  auto tiles = [&](auto Odd) {
+    for (int p0 = p_first; p0 < wend; p0 += step) {
+      constexpr bool odd = decltype(Odd)::value;
+      const int pn = p0 + step < wend ? p0 + step : p0;  // past the last tile: not used
+      // the queries are read from LDS anew for every tile: in registers they would cost the second wave its place
+      asm volatile("" : "+v"(qoff));
+      // matrix instructions of block b among the next block's dequantising
+      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QP];
 #pragma unroll
-    for (int b = 0; b < T; ++b) {
-      const u32x4 k0 = kw.operand(0, b), k1 = kw.operand(1, b);
+      for (int k = 0; k < QP; ++k) qq[k] = qs[qoff + k * 64];
 #pragma unroll
-      for (int k = 0; k < QP; ++k) {
-        const u32x4 qq = qs[qoff + (b * QP + k) * 64];
-        s[0] = mfma(k0, qq, s[0]);
-        s[1] = mfma(k1, qq, s[1]);
+      for (int b = 0; b < T; ++b) {
+        u32x4 n0 = k0, n1 = k1, qn[QP];
+        if (b + 1 < T) {
+#pragma unroll
+          for (int k = 0; k < QP; ++k) qn[k] = qs[qoff + ((b + 1) * QP + k) * 64];
+          n0 = kw.operand(0, b + 1);
+          n1 = kw.operand(1, b + 1);
+        }
+#pragma unroll
+        for (int k = 0; k < QP; ++k) {
+          s[0] = mfma(k0, qq[k], s[0]);
+          s[1] = mfma(k1, qq[k], s[1]);
+        }
+        interleave<2 * QP, 10>();
+        __builtin_amdgcn_sched_barrier(0);
+        k0 = n0;
+        k1 = n1;
+#pragma unroll
+        for (int k = 0; k < QP; ++k) qq[k] = qn[k];
       }
-    }
-    float x[8];
+      float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * scale;
-    if (odd) {
-      const unsigned b0 = kw.bad_rows(0), b1 = kw.bad_rows(1);
+      for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * scale;
+      if constexpr (odd) {
+        const unsigned b0 = kw.bad_rows(0), b1 = kw.bad_rows(1);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (((j < 4 ? b0 : b1) >> (4 * lk + (j & 3))) & 1u) x[j] = __builtin_nanf("");
-    }
-    kw.load(kc, ks, bad, pn, ln, lk);
-    if (p0 + 32 > wmin) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
-    }
-    const float bm = max_over_lk(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
-    const float mn = fmaxf(m, bm);
-    // a row that has seen nothing keeps m = -inf: its factor is 1 by definition, and its probabilities 0
-    const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    float p[8], ps = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
-      ps += p[j];
-    }
-    l = l * al + sum_over_lk(ps);
-    m = mn;
-    // the O rows of this lane are 4lk + i: their factors live in lanes 4lk + i
-    if (__ballot(al != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = __shfl(al, 4 * lk + i);
-#pragma unroll
-        for (int t = 0; t < 2 * T; ++t) o[t][i] *= a;
+        for (int j = 0; j < 8; ++j)
+          if (((j < 4 ? b0 : b1) >> (4 * lk + (j & 3))) & 1u) x[j] = __builtin_nanf("");
       }
-    }
-    u32x4 pp[PP];
-    split8<PP>(p, pp);
-    if (odd) vw.take_bad(p0, lk, first);
+      kw.load(kc, ks, pn, ln, lk);
+      if (p0 + 32 > wmin) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
+        for (int j = 0; j < 8; ++j)
+          if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
+      }
+      const float bm = max_over_lk(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+      const float mn = fmaxf(m, bm);
+      // a row that has seen nothing keeps m = -inf: its factor is 1 by definition, and its probabilities 0
+      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      float p[8], ps = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
+        ps += p[j];
+      }
+      l = l * al + sum_over_lk(ps);
+      m = mn;
+      // the O rows of this lane are 4lk + i: their factors live in lanes 4lk + i
+      if (__ballot(al != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = __shfl(al, 4 * lk + i);
+#pragma unroll
+          for (int t = 0; t < 2 * T; ++t) o[t][i] *= a;
+        }
+      }
+      u32x4 pp[PP];
+      split8<PP>(p, pp);
+      if constexpr (odd) vw.take_bad(p0, lk, first);
       u32x4 lo, hi;
-      vw.operands(t, lo, hi);
+      vw.operands(0, lo, hi);
 #pragma unroll
-      for (int k = 0; k < PP; ++k) {
-        o[2 * t] = mfma(pp[k], lo, o[2 * t]);
-        o[2 * t + 1] = mfma(pp[k], hi, o[2 * t + 1]);
+      for (int t = 0; t < T; ++t) {
+        u32x4 nlo = lo, nhi = hi;
+        if (t + 1 < T) vw.operands(t + 1, nlo, nhi);
+#pragma unroll
+        for (int k = 0; k < PP; ++k) {
+          o[2 * t] = mfma(pp[k], lo, o[2 * t]);
+          o[2 * t + 1] = mfma(pp[k], hi, o[2 * t + 1]);
+        }
+        interleave<2 * PP, 24>();
+        __builtin_amdgcn_sched_barrier(0);
+        lo = nlo;
+        hi = nhi;
+      }
+      vw.load(vc, vs, pn, (int)lane);
+    }
+  };
+  if (__ballot(flag != 0)) {
+    tiles(std::true_type{});
+    // rows that see a value which is not a number
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ci = __shfl(ctx, 4 * lk + i);
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        if (first[t] < ci) o[2 * t][i] = o[2 * t + 1][i] = __builtin_nanf("");
+    }
+  } else {
+    tiles(std::false_type{});
+  }
+  if constexpr (RT == 1) {
+    // the waves' results of the rows that there are, [wave][row][HD + 8] (the rows of a store in different banks), over
+    // the queries, which every wave has read; then each row's largest maximum and the sums at it, four dims a thread
+    constexpr int LD = HD + 8;
+    float* ms = reinterpret_cast<float*>(smem);  // m [PS][16], l [PS][16]
+    float* os = ms + 32 * PS;
+    __syncthreads();
+    if (lk == 0) {
+      ms[16 * w + ln] = m;
+      ms[16 * PS + 16 * w + ln] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (4 * lk + i < rows)
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+          *reinterpret_cast<float2*>(os + (size_t)(w * rows + 4 * lk + i) * LD + 32 * t + 2 * ln) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
+    __syncthreads();
+    for (int u = (int)tid; u < rows * (HD / 4); u += NT) {
+      const int r = u / (HD / 4), d = 4 * (u % (HD / 4));
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int k = 0; k < PS; ++k) M = fmaxf(M, ms[16 * k + r]);
+      f32x4 O{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < PS; ++k) {
+        const float e = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ms[16 * k + r] - M) * kLog2e);
+        L = __builtin_fmaf(ms[16 * PS + 16 * k + r], e, L);
+        O += *reinterpret_cast<const f32x4*>(os + (size_t)(k * rows + r) * LD + d) * e;
+      }
+      const size_t row = (size_t)(r / grp) * nq + g * grp + r % grp;
+      if (nch == 1) {
+        E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = from_f32<E>(O[j] / L);
+        if (dst.stats && d == 0) dst.stats[row] = make_float2(M, L);
+      } else {
+        float* rr = dst.rec + (row * nch + z) * (2 + HD);
+        if (d == 0) *reinterpret_cast<float2*>(rr) = make_float2(M, L);
+        *reinterpret_cast<float2*>(rr + 2 + d) = make_float2(O[0], O[1]);
+        *reinterpret_cast<float2*>(rr + 4 + d) = make_float2(O[2], O[3]);
       }
     }
-    vw.load(vc, vs, pn, (int)lane);
-  }
-  // rows that see a value which is not a number
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int ci = __shfl(ctx, 4 * lk + i);
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-      if (first[t] < ci) o[2 * t][i] = o[2 * t + 1][i] = __builtin_nanf("");
+    return;
   }
   // the waves of a row tile: the later half's results go to the earlier half's, until one has all
   f32x4* os = reinterpret_cast<f32x4*>(smem);  // [slot][2T][lane], over the queries, which every wave has read
@@ -614,7 +697,6 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
   const int pw = (int)blockIdx.x * 64 * PT + 16 * PT * (int)w;  // the wave's first position
   const int pblk = (int)blockIdx.x * 64 * PT;
   const uint8_t *kc = c.kc + g * c.code_head(), *ks = c.ks + g * c.scale_head();
-  const uint8_t* bad = c.bad + (size_t)g * (c.cap / kKv4Tile);
   u32x4 kop[PT][T];
   unsigned nan[PT];
 #pragma unroll
@@ -622,7 +704,7 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     KeyWords<HD> kw;
     // whole tiles of 32 rows; past the last one (a wave with nothing to do, or half a tile) the first is read instead
     const int r = pw + 16 * u, base = r < len ? r & ~31 : 0;
-    kw.load(kc, ks, bad, base, ln, lk);
+    kw.load(kc, ks, base, ln, lk);
     const int h0 = r < len ? (r >> 4) & 1 : 0;
 #pragma unroll
     for (int b = 0; b < T; ++b) {
@@ -694,19 +776,27 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     }
 }
 
-// The form of the kernel that a call takes: row tiles of a workgroup, and the waves of a row tile.
-static int attend_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// The form of the kernel that a call takes: row tiles of a workgroup (rt), and the waves of a row tile (ps).  One row tile
+// takes eight waves, or four while 256 workgroups of four have no more than a tile each: fewer results to join, 10.4
+// against 12.1 us at 4096 positions of 4 key/value heads, 16.5 against 14.8 at 16384.
+struct AttendForm {
+  int rt, ps;
+};
+static AttendForm attend_form(int rows, int nkv, int len) {
+  if (rows > 32) return AttendForm{4, 2};
+  if (rows > 16) return AttendForm{2, 4};
+  return AttendForm{1, (int64_t)len * nkv <= 256 * 128 ? 4 : 8};
+}
 template <class F>
-static int with_row_tiles(int rt, F&& f) {
-  switch (rt) {
-    case 1: return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
-    case 2: return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
-    default: return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-  }
+static int with_form(AttendForm form, F&& f) {
+  if (form.rt == 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+  if (form.rt == 2) return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+  if (form.ps == 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
 }
 // Chunks of positions that a call's row tiles are spread over, at most: as many workgroups as are resident at once.
 static int attend_max_chunks(int n, int n_head, int nkv) {
-  const int rows = n * (n_head / nkv), rt = attend_row_tiles(rows);
+  const int rows = n * (n_head / nkv), rt = attend_form(rows, nkv, 0).rt;
   const int tiles = (rows + 16 * rt - 1) / (16 * rt) * nkv;
   return std::max(1, std::min(kKv4MaxChunks, 256 / tiles));
 }
@@ -716,9 +806,11 @@ size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   return (rows * sizeof(float2) + 15) / 16 * 16 + (nch > 1 ? rows * nch * (size_t)(2 + c.hd) * sizeof(float) : 0);
 }
 
+// Dynamic LDS of a workgroup for a call of `rows` rows a key/value head.
 template <int HD, class E, int RT, int PS>
-constexpr size_t attend_lds() {
-  constexpr size_t queries = (size_t)RT * (HD / 32) * Parts<E>::q * 1024, join = (size_t)(RT * PS / 2) * (HD / 32 * 2 * 1024 + 512);
+constexpr size_t attend_lds(int rows) {
+  const size_t queries = (size_t)RT * (HD / 32) * Parts<E>::q * 1024;
+  const size_t join = RT == 1 ? (size_t)PS * (128 + (rows < 16 ? rows : 16) * (HD + 8) * 4) : (size_t)(RT * PS / 2) * (HD / 32 * 2 * 1024 + 512);
   return queries > join ? queries : join;
 }
 
@@ -730,14 +822,14 @@ int prepare_kv4_kernels() {
   if (done) return DZ_OK;
   for (int hd : {64, 128, 256})
     for (int type : {DZ_F32, DZ_F16, DZ_BF16})
-      for (int rt : {1, 2, 4}) {
+      for (AttendForm form : {AttendForm{1, 4}, AttendForm{1, 8}, AttendForm{2, 4}, AttendForm{4, 2}}) {
         const int rc = with_head_dim(hd, [&](auto D) {
           return with_type(type, [&](auto* e) {
-            return with_row_tiles(rt, [&](auto R, auto P) -> int {
+            return with_form(form, [&](auto R, auto P) -> int {
               using E = std::remove_pointer_t<decltype(e)>;
               constexpr int HD = decltype(D)::value, RT = decltype(R)::value, PS = decltype(P)::value;
               DZ_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kv4_attend_kernel<HD, E, RT, PS>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, RT, PS>()));
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)attend_lds<HD, E, RT, PS>(16)));
               return DZ_OK;
             });
           });
@@ -750,7 +842,9 @@ int prepare_kv4_kernels() {
 
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s) {
-  const int rows = n * (n_head / c.nkv), rt = attend_row_tiles(rows), unit = 256 / rt;  // a tile for every wave
+  const int rows = n * (n_head / c.nkv);
+  const AttendForm form = attend_form(rows, c.nkv, len);
+  const int unit = 32 * form.ps;  // a tile for every wave
   const int most = attend_max_chunks(n, n_head, c.nkv);
   const int csz = ((len + most - 1) / most + unit - 1) / unit * unit, nch = (len + csz - 1) / csz;
   return with_head_dim(c.hd, [&](auto D) {
@@ -761,10 +855,10 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       float2* stats = static_cast<float2*>(work);
       dst.stats = weights ? stats : nullptr;
       dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
-      const int rc = with_row_tiles(rt, [&](auto R, auto P) -> int {
+      const int rc = with_form(form, [&](auto R, auto P) -> int {
         constexpr int RT = decltype(R)::value, PS = decltype(P)::value;
         const unsigned wgs = (unsigned)((rows + 16 * RT - 1) / (16 * RT) * c.nkv * nch);
-        kv4_attend_kernel<HD, E, RT, PS><<<dim3(wgs), 64 * RT * PS, attend_lds<HD, E, RT, PS>(), s>>>(
+        kv4_attend_kernel<HD, E, RT, PS><<<dim3(wgs), 64 * RT * PS, attend_lds<HD, E, RT, PS>(rows), s>>>(
             c, len, (const E*)q, ldq, n_head, n, scale, csz, nch, dst, (E*)out, ldo);
         DZ_HIP_CHECK(hipGetLastError());
         return DZ_OK;
