@@ -634,16 +634,15 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
 }
 
 // The chunks' records of a row (query blockIdx.x, head blockIdx.y) as 64 dims (blockIdx.z) of its output, and its
-// statistics: 256 threads, wave w for the w-th quarter of the chunks, 16 of its records requested at a time.  A chunk whose
+// statistics: 256 threads, wave w for the w-th quarter of the chunks, N of its records requested at a time.  A chunk whose
 // positions the row does not see has l = 0, m = -inf and zeros.
-template <int HD, class E>
+template <int HD, class E, int N>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, int nq, E* __restrict__ out, int64_t ldo) {
   __shared__ float fac[kKv4MaxChunks], red[4][65], mx[4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, d = (int)blockIdx.z * 64 + lane;
   const size_t row = (size_t)blockIdx.x * nq + blockIdx.y;
   const float* rec = src.rec + row * nch * (2 + HD);
   const int q4 = (nch + 3) / 4, z0 = w * q4, z1 = min(nch, z0 + q4);
-  constexpr int N = 16;
   float v[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = rec[(size_t)min(z0 + k, nch - 1) * (2 + HD) + 2 + d];
@@ -681,21 +680,35 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, 
   if (src.stats && d == 0) src.stats[row] = make_float2(m, l);
 }
 
+// The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile][block][part][lane].
+// Grid (row tiles, nkv), 256 threads.
+template <int HD, class E>
+__global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q, int64_t ldq, int nkv, int nq, int n,
+                                                        u32x4* __restrict__ split) {
+  const int g = blockIdx.y, grp = nq / nkv;
+  QueryStage<HD, E, 1, 256> queries;
+  queries.load(q, ldq, g * grp, grp, 16 * (int)blockIdx.x, n * grp, (int)threadIdx.x);
+  queries.store(split + ((size_t)g * gridDim.x + blockIdx.x) * (HD / 32 * Parts<E>::q * 64), (int)threadIdx.x);
+}
+
 // weights[g][r] += Σ over the group's query rows ρ of exp(s_ρr - m_ρ) / l_ρ: a wave holds the operands of 16·PT rows of keys and
-// walks the query rows 16 at a time (staged for the workgroup's four waves in LDS), a lane adding up its four positions
+// walks the query rows 16 at a time, in LDS for the workgroup's four waves, a lane adding up its four positions
 // of each 16 over the query rows ln, in order; the sixteen lanes of a position are summed at the end.
+// READY: the queries come as operands (kv4_split_kernel), the next tile's requested ahead and LDS in two halves, one
+// barrier a tile; else the workgroup forms them (few rows, where a launch more would cost more).
+// Bound by the matrix instructions (24 PT of 16 cycles with f32 queries) and the LDS reads beside them (24 KB a wave).
 // Grid (ceil(len / 64PT), nkv), 256 threads.
-template <int HD, class E, int PT>
+template <int HD, class E, int PT, bool READY>
 __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq, int n,
-                                                             float scale, const float2* __restrict__ stats,
-                                                             float* __restrict__ weights, int64_t ldw) {
-  constexpr int T = HD / 32, QP = Parts<E>::q;
-  __shared__ u32x4 qs[T * QP * 64];
+                                                             float scale, const u32x4* __restrict__ split,
+                                                             const float2* __restrict__ stats, float* __restrict__ weights,
+                                                             int64_t ldw) {
+  constexpr int T = HD / 32, QP = Parts<E>::q, TILE = T * QP * 64, N = (TILE + 255) / 256;
+  __shared__ u32x4 qs[(READY ? 2 : 1) * TILE];
   const int g = blockIdx.y, grp = nq / c.nkv, rows = n * grp, before = len - n;
-  const unsigned tid = threadIdx.x, lane = tid & 63u, w = tid >> 6;
-  const int ln = (int)(lane & 15u), lk = (int)(lane >> 4);
-  const int pw = (int)blockIdx.x * 64 * PT + 16 * PT * (int)w;  // the wave's first position
-  const int pblk = (int)blockIdx.x * 64 * PT;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int ln = lane & 15, lk = lane >> 4;
+  const int pblk = (int)blockIdx.x * 64 * PT, pw = pblk + 16 * PT * w;  // the workgroup's and the wave's first position
   const uint8_t *kc = c.kc + g * c.code_head(), *ks = c.ks + g * c.scale_head();
   u32x4 kop[PT][T];
   unsigned nan[PT];
@@ -722,25 +735,49 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
       nan[u + 1] = kw.bad_rows(1);
     }
   }
+  unsigned any_nan = 0;
+#pragma unroll
+  for (int u = 0; u < PT; ++u) any_nan |= nan[u];
   float acc[PT][4];
 #pragma unroll
   for (int u = 0; u < PT; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[u][i] = 0.f;
-  // the first query row that sees the workgroup's first position
-  const int r0 = max(0, pblk - before) * grp / 16 * 16;
-  for (int row = r0; row < rows; row += 16) {
-    QueryStage<HD, E, 1, 256> queries;
-    queries.load(q, ldq, g * grp, grp, row, rows, (int)tid);
+  // from the tile of the first query row that sees the workgroup's first position
+  const int t0 = max(0, pblk - before) * grp / 16, tn = (rows + 15) / 16;
+  u32x4 next[READY ? N : 1];
+  float2 st_next = make_float2(0.f, 1.f);
+  const u32x4* tiles = split + (size_t)g * tn * TILE;
+  auto stat = [&](int t) {
+    const int rho = min(16 * t + ln, rows - 1);
+    return stats[(size_t)(rho / grp) * nq + g * grp + rho % grp];
+  };
+  auto request = [&](int t) {
+    if constexpr (READY)
+#pragma unroll
+      for (int i = 0; i < N; ++i) next[i] = tiles[(size_t)t * TILE + (TILE % 256 ? min(tid + 256 * i, TILE - 1) : tid + 256 * i)];
+    st_next = stat(t);
+  };
+  if (t0 < tn) request(t0);
+  for (int t = t0; t < tn; ++t) {
+    const u32x4* qt = qs;
+    if constexpr (READY) {
+      u32x4* to = qs + (t & 1) * TILE;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (TILE % 256 == 0 || tid + 256 * i < TILE) to[tid + 256 * i] = next[i];
+      qt = to;
+    } else {
+      QueryStage<HD, E, 1, 256> queries;
+      queries.load(q, ldq, g * grp, grp, 16 * t, rows, tid);
+      __syncthreads();
+      queries.store(qs, tid);
+    }
+    const float2 st = st_next;
     __syncthreads();
-    queries.store(qs, (int)tid);
-    __syncthreads();
-    const int rho = row + ln;
-    const bool has = rho < rows;
-    const int ctx = has ? before + rho / grp + 1 : 0;
-    float2 st = make_float2(0.f, 1.f);
-    if (has) st = stats[(size_t)(rho / grp) * nq + g * grp + rho % grp];
-    const float inv = 1.f / st.y;
+    request(min(t + 1, tn - 1));
+    const int rho = 16 * t + ln;
+    const int ctx = rho < rows ? before + rho / grp + 1 : 0;
     f32x4 s[PT];
 #pragma unroll
     for (int u = 0; u < PT; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -748,18 +785,26 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     for (int b = 0; b < T; ++b)
 #pragma unroll
       for (int k = 0; k < QP; ++k) {
-        const u32x4 qq = qs[(b * QP + k) * 64 + lane];
+        const u32x4 qq = qt[(b * QP + k) * 64 + lane];
 #pragma unroll
         for (int u = 0; u < PT; ++u) s[u] = mfma(kop[u][b], qq, s[u]);
       }
+    const float inv = 1.f / st.y;
+    if (any_nan) {
+#pragma unroll
+      for (int u = 0; u < PT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((nan[u] >> (4 * lk + i)) & 1u) s[u][i] = __builtin_nanf("");
+    }
+    // the tile's first row sees the fewest positions; a tile past the last row has rows that count for nothing
+    const bool whole = 16 * t + 16 <= rows && before + 16 * t / grp + 1 >= pw + 16 * PT;
 #pragma unroll
     for (int u = 0; u < PT; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float x = s[u][i] * scale;
-        if (nan[u] && ((nan[u] >> (4 * lk + i)) & 1u)) x = __builtin_nanf("");
-        const float p = __builtin_amdgcn_exp2f((x - st.x) * kLog2e) * inv;
-        if (pw + 16 * u + 4 * lk + i < ctx) acc[u][i] += p;
+        const float p = __builtin_amdgcn_exp2f((s[u][i] * scale - st.x) * kLog2e) * inv;
+        acc[u][i] += whole || pw + 16 * u + 4 * lk + i < ctx ? p : 0.f;
       }
   }
 #pragma unroll
@@ -801,9 +846,15 @@ static int attend_max_chunks(int n, int n_head, int nkv) {
   return std::max(1, std::min(kKv4MaxChunks, 256 / tiles));
 }
 
+// From this many tiles of 16 query rows on the weights' pass takes its queries as operands formed once.
+constexpr int kKv4SplitTiles = 4;
+
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   const size_t rows = (size_t)n * n_head, nch = (size_t)attend_max_chunks(n, n_head, c.nkv);
-  return (rows * sizeof(float2) + 15) / 16 * 16 + (nch > 1 ? rows * nch * (size_t)(2 + c.hd) * sizeof(float) : 0);
+  const size_t rec = nch > 1 ? rows * nch * (size_t)(2 + c.hd) * sizeof(float) : 0;
+  const int tiles = (n * (n_head / c.nkv) + 15) / 16;
+  const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * 16 * c.nkv * c.hd * 2 * Parts<float>::q : 0;  // over the records
+  return (rows * sizeof(float2) + 15) / 16 * 16 + std::max(rec, split);
 }
 
 // Dynamic LDS of a workgroup for a call of `rows` rows a key/value head.
@@ -865,19 +916,33 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       });
       if (rc) return rc;
       if (nch > 1) {
-        kv4_merge_kernel<HD, E><<<dim3((unsigned)n, (unsigned)n_head, HD / 64), 256, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
+        const dim3 grid((unsigned)n, (unsigned)n_head, HD / 64);
+        if (nch <= 4) kv4_merge_kernel<HD, E, 1><<<grid, 256, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
+        else if (nch <= 16) kv4_merge_kernel<HD, E, 4><<<grid, 256, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
+        else kv4_merge_kernel<HD, E, 16><<<grid, 256, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
         DZ_HIP_CHECK(hipGetLastError());
       }
       if (weights) {
-        const int64_t tiles = ((int64_t)len + 15) / 16 * c.nkv;
-        auto run = [&](auto P) {
+        // as many rows of keys a wave as leave about a workgroup for each compute unit
+        const int64_t units = ((int64_t)len + 63) / 64 * c.nkv;
+        const int row_tiles = (rows + 15) / 16;
+        u32x4* split = row_tiles >= kKv4SplitTiles ? reinterpret_cast<u32x4*>(dst.rec) : nullptr;
+        if (split) {
+          kv4_split_kernel<HD, E><<<dim3((unsigned)row_tiles, (unsigned)c.nkv), 256, 0, s>>>((const E*)q, ldq, c.nkv, n_head, n, split);
+          DZ_HIP_CHECK(hipGetLastError());
+        }
+        auto run = [&](auto P, auto R) {
           constexpr int PT = decltype(P)::value;
-          kv4_weights_kernel<HD, E, PT><<<dim3((unsigned)((len + 64 * PT - 1) / (64 * PT)), (unsigned)c.nkv), 256, 0, s>>>(
-              c, len, (const E*)q, ldq, n_head, n, scale, stats, weights, ldw);
+          kv4_weights_kernel<HD, E, PT, decltype(R)::value><<<dim3((unsigned)((len + 64 * PT - 1) / (64 * PT)), (unsigned)c.nkv), 256, 0, s>>>(
+              c, len, (const E*)q, ldq, n_head, n, scale, split, stats, weights, ldw);
         };
-        if (tiles >= 16 * 256) run(std::integral_constant<int, 4>{});
-        else if (tiles >= 8 * 256) run(std::integral_constant<int, 2>{});
-        else run(std::integral_constant<int, 1>{});
+        auto with_rows = [&](auto P) {
+          if (split) run(P, std::true_type{});
+          else run(P, std::false_type{});
+        };
+        if (units >= 4 * 200) with_rows(std::integral_constant<int, 4>{});
+        else if (units >= 2 * 200) with_rows(std::integral_constant<int, 2>{});
+        else with_rows(std::integral_constant<int, 1>{});
         DZ_HIP_CHECK(hipGetLastError());
       }
       return DZ_OK;
