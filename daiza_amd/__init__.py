@@ -24,6 +24,7 @@ DZ_ERR_DEVICE = -4
 _f32p = ctypes.POINTER(ctypes.c_float)
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
+_i32p = ctypes.POINTER(ctypes.c_int32)
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 
@@ -168,6 +169,11 @@ _MODEL_PROTOS = {
     "dz_leviathan_check": ([_f32p, _f32p, ctypes.c_int, ctypes.c_uint32, _vp, ctypes.POINTER(ctypes.c_uint64),
                             ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "dz_sample_bonus": ([_f32p, _f32p, ctypes.c_int, _vp, ctypes.POINTER(ctypes.c_uint64), _u32p], ctypes.c_int),
+    "dz_ctx_create_kv4": ([_vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)], ctypes.c_int),
+    "dz_ctx_kv_evict": ([_vp, ctypes.c_int, ctypes.c_int, _i32p], ctypes.c_int),
+    "dz_ctx_kv_weights": ([_vp, ctypes.c_int, _f32p, ctypes.c_int], ctypes.c_int),
+    "dz_forward_logprobs": ([_vp, _u32p, _i32p, ctypes.c_int, ctypes.c_int, ctypes.c_int, _f32p, _f32p, _i32p, _f32p], ctypes.c_int),
+    "dz_ctx_logprobs": ([_vp, ctypes.c_int32, ctypes.c_int, _f32p, _f32p, _i32p, _f32p], ctypes.c_int),
     "dz_kv4_create": ([ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)], ctypes.c_int),
     "dz_kv4_free": ([_vp], ctypes.c_int),
     "dz_kv4_len": ([_vp], ctypes.c_int),
@@ -455,13 +461,21 @@ def session_cfg_hash(cfg, context_length=CONTEXT_LENGTH):
 
 
 class Context:
-    """ModelState + ForwardContext (forward.rs:32-131) on the device."""
+    """ModelState + ForwardContext (forward.rs:32-131) on the device.
 
-    def __init__(self, model):
+    kv4: the key/value cache in 4 bits (dz_ctx_create_kv4), for kv_rows rows (0: max_ctx); track: with the attention weight
+    that each row receives, for kv_evict."""
+
+    def __init__(self, model, kv4=False, kv_rows=0, track=False):
         self.model = model
         self.cfg = model.cfg
         h = _vp()
-        _check(lib().dz_ctx_create(model._h, ctypes.byref(h)))
+        if kv4:
+            _check(lib().dz_ctx_create_kv4(model._h, int(kv_rows), int(bool(track)), ctypes.byref(h)))
+        elif kv_rows or track:
+            raise DaizaError(DZ_ERR_UNSUPPORTED, "kv_rows and track need kv4")
+        else:
+            _check(lib().dz_ctx_create(model._h, ctypes.byref(h)))
         self._h = h
 
     def close(self):
@@ -527,6 +541,28 @@ class Context:
                                       _f(per) if per_pos_logits else None))
         return per if per_pos_logits else last
 
+    def forward_logprobs(self, ids, targets=None, top=0):
+        """forward_batch with log probabilities in place of logits (dz_forward_logprobs): (logp [n] of targets or None, entropy
+        [n], top_ids [n][top], top_logp [n][top]); targets[i] is scored by the logits after ids[i], -1 for none."""
+        ids = np.ascontiguousarray(ids, np.uint32)
+        n = ids.size
+        t = None if targets is None else np.ascontiguousarray(targets, np.int32)
+        if t is not None and t.size != n:
+            raise DaizaError(DZ_ERR_TENSOR, "%d targets for %d tokens" % (t.size, n))
+        logp = None if t is None else np.empty(n, np.float32)
+        ent, tid, tlp = np.empty(n, np.float32), np.empty((n, max(0, top)), np.int32), np.empty((n, max(0, top)), np.float32)
+        _check(lib().dz_forward_logprobs(self._h, ids.ctypes.data_as(_u32p), None if t is None else t.ctypes.data_as(_i32p), n,
+                                         self.pos, int(top), None if t is None else _f(logp), _f(ent), tid.ctypes.data_as(_i32p),
+                                         _f(tlp)))
+        return logp, ent, tid, tlp
+
+    def logprobs(self, token=-1, top=0):
+        """The same of the last logits: (log probability of token, entropy, top_ids [top], top_logp [top])."""
+        logp, ent = np.empty(1, np.float32), np.empty(1, np.float32)
+        tid, tlp = np.empty(max(0, top), np.int32), np.empty(max(0, top), np.float32)
+        _check(lib().dz_ctx_logprobs(self._h, int(token), int(top), _f(logp), _f(ent), tid.ctypes.data_as(_i32p), _f(tlp)))
+        return float(logp[0]), float(ent[0]), tid, tlp
+
     def decode_greedy(self, first_token, n):
         """n greedy forwards on the device; the pick after each (engine.rs:850-871 without the EOS stop)."""
         out = np.empty(n, np.uint32)
@@ -554,6 +590,26 @@ class Context:
     def kv_truncate(self, n):
         """KvCache::truncate (kv_cache.rs:119-130): keeps n cached positions, pos = n; conv rings stay."""
         _check(lib().dz_kv_truncate(self._h, int(n)))
+
+    def kv_len(self, layer):
+        """Rows that an attention layer's cache holds (dz_ctx_kv_len)."""
+        return lib().dz_ctx_kv_len(self._h, int(layer))
+
+    def kv_evict(self, keep, recent):
+        """Keeps each key/value head's newest `recent` rows and the keep - recent of the largest weights (dz_ctx_kv_evict);
+        the rows that stayed, [attention layer][kv head][m]."""
+        c = self.cfg
+        attn = [i for i in range(c.n_layers) if c.is_full_attention(i)]
+        m = max(0, min(int(keep), self.kv_len(attn[0]))) if attn else 0
+        kept = np.empty((len(attn), c.n_head_kv, m), np.int32)
+        _check(lib().dz_ctx_kv_evict(self._h, int(keep), int(recent), kept.ctypes.data_as(_i32p)))
+        return kept
+
+    def kv_weights(self, layer):
+        """The attention weight that each row of a layer's cache has received, [kv head][rows] (dz_ctx_kv_weights)."""
+        w = np.empty((self.cfg.n_head_kv, self.kv_len(layer)), np.float32)
+        _check(lib().dz_ctx_kv_weights(self._h, int(layer), _f(w), w.shape[1]))
+        return w
 
     def copy_state_from(self, src):
         """ModelState::clone onto this context (dz_ctx_copy_state): checkpoint into a spare context,

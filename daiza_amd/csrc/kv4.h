@@ -49,6 +49,17 @@ inline Kv4View kv4_carve(uint8_t* base, int nkv, int hd, int cap) {
   return v;
 }
 
+// One key/value head of a view.
+inline Kv4View kv4_head(Kv4View v, int h) {
+  v.kc += h * v.code_head();
+  v.vc += h * v.code_head();
+  v.ks += h * v.scale_head();
+  v.vs += h * v.scale_head();
+  v.bad += (size_t)h * (v.cap / kKv4Tile);
+  v.nkv = 1;
+  return v;
+}
+
 // Offset of the T bytes of value row r that lane ln (dims 32t + 2ln, +1) holds.
 template <int HD>
 __device__ __forceinline__ size_t kv4_value_offset(int64_t r, int ln) {
@@ -82,8 +93,9 @@ int kv4_append(const Kv4View& c, int row0, const void* k, int64_t ldk, const voi
 int kv4_read(const Kv4View& c, int start, int n, float* k, float* v, hipStream_t s);
 int prepare_kv4_kernels();
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n);
+// gate: see AttendOut (f32 [n][n_head][head_dim]).
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
-               int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s);
+               int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s, const float* gate);
 int kv4_evict(const Kv4View& c, int len, const float* weights, int64_t ldw, int keep, int recent, const Kv4View& dst,
               float* dst_weights, int64_t ld_dst, int32_t* kept, hipStream_t s);
 

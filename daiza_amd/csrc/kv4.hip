@@ -337,8 +337,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Where a call's results go: the output itself (nch = 1) or a record (m, l, o[HD]) per row and chunk of positions.
 struct AttendOut {
-  float* rec;     // [n][nq][nch][2 + HD]
-  float2* stats;  // [n][nq] (m, l), or null
+  float* rec;         // [n][nq][nch][2 + HD]
+  float2* stats;      // [n][nq] (m, l), or null
+  const float* gate;  // [n][nq][HD]: the output times its sigmoid, or null
+  // Element d of row `row` (HD elements each).
+  template <class E, int HD>
+  __device__ __forceinline__ E value(float o, float l, size_t row, int d) const {
+    float y = o / l;
+    if (gate) y *= 1.0f / (1.0f + expf(-gate[row * HD + d]));
+    return from_f32<E>(y);
+  }
 };
 
 // M matrix instructions with V vector instructions spread among them.
@@ -561,7 +569,7 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
       if (nch == 1) {
         E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + d;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = from_f32<E>(O[j] / L);
+        for (int j = 0; j < 4; ++j) y[j] = dst.value<E, HD>(O[j], L, row, d + j);
         if (dst.stats && d == 0) dst.stats[row] = make_float2(M, L);
       } else {
         float* rr = dst.rec + (row * nch + z) * (2 + HD);
@@ -619,11 +627,12 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
     const float li = __shfl(l, 4 * lk + i);
     if (r >= rows) continue;
     if (nch == 1) {
+      const size_t row = (size_t)(r / grp) * nq + g * grp + r % grp;
       E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + 2 * ln;
 #pragma unroll
       for (int t = 0; t < T; ++t) {
-        y[32 * t] = from_f32<E>(o[2 * t][i] / li);
-        y[32 * t + 1] = from_f32<E>(o[2 * t + 1][i] / li);
+        y[32 * t] = dst.value<E, HD>(o[2 * t][i], li, row, 32 * t + 2 * ln);
+        y[32 * t + 1] = dst.value<E, HD>(o[2 * t + 1][i], li, row, 32 * t + 2 * ln + 1);
       }
     } else {
       float* rr = dst.rec + (((size_t)(r / grp) * nq + g * grp + r % grp) * nch + z) * (2 + HD) + 2 + 2 * ln;
@@ -676,7 +685,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, 
   if (w) return;
   l = (red[0][64] + red[1][64]) + (red[2][64] + red[3][64]);
   o = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-  out[(size_t)blockIdx.x * ldo + (size_t)blockIdx.y * HD + d] = from_f32<E>(o / l);
+  out[(size_t)blockIdx.x * ldo + (size_t)blockIdx.y * HD + d] = src.value<E, HD>(o, l, row, d);
   if (src.stats && d == 0) src.stats[row] = make_float2(m, l);
 }
 
@@ -892,7 +901,7 @@ int prepare_kv4_kernels() {
 }
 
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
-               int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s) {
+               int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s, const float* gate) {
   const int rows = n * (n_head / c.nkv);
   const AttendForm form = attend_form(rows, c.nkv, len);
   const int unit = 32 * form.ps;  // a tile for every wave
@@ -905,6 +914,7 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       AttendOut dst;
       float2* stats = static_cast<float2*>(work);
       dst.stats = weights ? stats : nullptr;
+      dst.gate = gate;
       dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
       const int rc = with_form(form, [&](auto R, auto P) -> int {
         constexpr int RT = decltype(R)::value, PS = decltype(P)::value;
@@ -1263,7 +1273,7 @@ int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int
       (rc = check_array(out, type_size(type), c->device, "out")) || (rc = check_array(work, 16, c->device, "work")) ||
       (weights && (rc = check_array(weights, 4, c->device, "weights"))))
     return rc;
-  return kv4_attend(c->v, c->len, q, ldq, type, n_head, n, scale, weights, ldw, out, ldo, work, static_cast<hipStream_t>(stream));
+  return kv4_attend(c->v, c->len, q, ldq, type, n_head, n, scale, weights, ldw, out, ldo, work, static_cast<hipStream_t>(stream), nullptr);
 }
 
 int dz_kv4_evict_dev(const dz_kv4* c, const float* weights, int64_t ldw, int keep, int recent, dz_kv4* dst, float* dst_weights,

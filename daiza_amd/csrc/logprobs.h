@@ -4,6 +4,8 @@
 
 namespace dz {
 
+constexpr int kLogprobTop = 64;  // most alternatives
+
 // Bytes of work memory, and the launches: see dz_logprobs_dev.  The arguments are checked by the caller.
 size_t logprobs_work(int n, int64_t vocab, int top);
 int logprobs(const void* logits, int64_t ld, int type, int n, int vocab, const int32_t* tokens, int top, float* logp, float* entropy,

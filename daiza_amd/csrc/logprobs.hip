@@ -9,7 +9,6 @@
 
 namespace dz {
 
-constexpr int kLogprobTop = 64;  // most alternatives
 constexpr int kLpVals = 16;      // logits of a lane and step
 constexpr int kLpStep = 64 * kLpVals;
 constexpr int kLpGroups = 4;     // groups of a step: the 16 lanes of a DPP row

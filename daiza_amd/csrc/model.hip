@@ -5,6 +5,8 @@
 #include "model_kernels.h"
 #include "ptk_kernel.h"
 #include "batch_kernels.h"
+#include "kv4_ctx.h"
+#include "logprobs.h"
 #include "daiza_synth.h"
 
 #include <cmath>
@@ -101,12 +103,26 @@ struct dz_ctx {
     float *ygu = nullptr, *sw = nullptr, *qb = nullptr, *gate = nullptr;
     float* logits = nullptr;  // [logits_rows][vocab]
     int logits_rows = 0;
-    dz::Scratch pack, split, arec, spec, chunk, dig;
+    dz::Scratch pack, split, arec, spec, chunk, dig, logp;
     // verify records per DeltaNet layer: conv inputs [kv][qkvd] and the scan's rollback record
     int kv_cap = 0;
     dz::DnRecords recs{};
     int pending = 0;          // tokens of the last verify forward (0: none); their ids are in `ids`
   } bt;
+  // key/value cache in 4 bits (dz_ctx_create_kv4), in place of kv: every attention layer holds the rows of
+  // pos_host - evicted positions
+  struct {
+    bool on = false, track = false;
+    int rows = 0;                     // capacity
+    std::vector<dz::Kv4View> layer;   // per attention layer
+    std::vector<float*> w;            // per attention layer: weights [nkv][cap] (track)
+    dz::Kv4View spare;                // where an eviction puts the rows that stay, before it takes the layer's place
+    float* spare_w = nullptr;
+    int32_t* kept = nullptr;          // [nkv][rows]
+    int evicted = 0, floor = 0;       // rows taken out so far; the position of the last eviction
+    float *q = nullptr, *gate = nullptr;  // one token's attention inputs
+    dz::Scratch work;
+  } kv4;
   std::vector<void*> allocs;
 };
 
@@ -491,6 +507,32 @@ static int launch_attention(int grp, dim3 grid, const AttnArgs& a, hipStream_t s
   });
 }
 
+// Attention of n tokens at positions pos .. of a context whose cache is in 4 bits, from their in-projection: its rows into
+// the cache, then the gated outputs -> out[n][n_head · head_dim].
+template <class Src>
+static int kv4_attention(dz_ctx* x, const LayerDev& l, const Src& src, int pos, int n, float* q, float* gate, float* out, bool track,
+                         hipStream_t s) {
+  const dz_config& c = x->m->cfg;
+  const Kv4View& v = x->kv4.layer[(size_t)l.kind_idx];
+  float* w = x->kv4.track ? x->kv4.w[(size_t)l.kind_idx] : nullptr;
+  const int row = pos - x->kv4.evicted;
+  if (int rc = x->kv4.work.reserve(kv4_attend_work(v, (int)c.n_head, n))) return rc;
+  hipLaunchKernelGGL(kv4_prep_kernel<Src>, dim3((unsigned)n, (unsigned)(c.n_head + c.n_head_kv)), dim3(256), 0, s, src, (int)c.n_head,
+                     (int)c.n_head_kv, (const float*)l.q_norm, (const float*)l.k_norm, c.rms_eps, (const float*)x->rope,
+                     (int)c.rope_dim, pos, row, q, gate, v, w, (int64_t)v.cap);
+  DZ_HIP_CHECK(hipGetLastError());
+  const int64_t ld = (int64_t)c.n_head * c.head_dim;
+  return kv4_attend(v, row + n, q, ld, DZ_F32, (int)c.n_head, n, 1.0f, track ? w : nullptr, v.cap, out, ld, x->kv4.work.ptr, s, gate);
+}
+
+// Whether n more positions fit a 4-bit cache (a context with an f32 cache is bounded by max_ctx alone).
+static int kv4_room(const dz_ctx* x, int n) {
+  if (x->kv4.on && x->pos_host - x->kv4.evicted + n > x->kv4.rows)
+    return set_error(DZ_ERR_TENSOR, "4-bit cache full: %d rows + %d > %d (dz_ctx_kv_evict makes room)", x->pos_host - x->kv4.evicted, n,
+                     x->kv4.rows);
+  return DZ_OK;
+}
+
 // The mixer of one layer on the residual held in (h_in + parts): norm + in-proj GEMV, then the
 // DeltaNet or attention kernel, then the out-projection GEMV into p_o.  `h_mid` receives the
 // materialised layer input with its tile sums of squares in `ss_mid`.
@@ -547,6 +589,15 @@ static int enqueue_mixer(dz_ctx* x, int li, const float* h_in, const float* part
     GatedYSrc src{x->y, x->zs, l.ssm_norm, inner, 1e-6f};
     PartialDst dst{x->p_o, ld_h};
     if ((rc = gemv(l.out_proj, 1, src, dst, s))) return rc;
+  } else if (x->kv4.on) {
+    rc = with_np_bucket(nin, [&](auto B) -> int {
+      const ProjPartials<decltype(B)::value> proj{x->p_in, nin, ld_l, ss_mid, th, H, c.rms_eps};
+      return kv4_attention(x, l, proj, pos, 1, x->kv4.q, x->kv4.gate, x->attn_u, x->kv4.track, s);
+    });
+    if (rc) return rc;
+    PlainSrc src{x->attn_u, (int64_t)c.n_head * c.head_dim};
+    PartialDst dst{x->p_o, ld_h};
+    if ((rc = gemv(l.out_proj, 1, src, dst, s))) return rc;
   } else {
     AttnArgs a;
     a.st = x->st;
@@ -588,7 +639,7 @@ static int enqueue_mixer(dz_ctx* x, int li, const float* h_in, const float* part
 }
 
 // One token (forward_single_token): select/embed, all blocks, final norm, lm_head.
-static int enqueue_token(dz_ctx* x, hipStream_t s) {
+static int enqueue_token(dz_ctx* x, hipStream_t s, int pos = -1) {
   dz_model* m = x->m;
   const dz_config& c = m->cfg;
   int64_t ld_in, ld_h, ld_gu;
@@ -615,7 +666,7 @@ static int enqueue_token(dz_ctx* x, hipStream_t s) {
     LayerDev& l = m->L[li];
     const float* h_in = li == 0 ? x->emb_row : x->h[1];
     const int np = li == 0 ? 0 : (int)m->L[li - 1].down.ntiles;
-    if ((rc = enqueue_mixer(x, li, h_in, x->p_down, np, ld_h, x->h[0], x->ss[0], s))) return rc;
+    if ((rc = enqueue_mixer(x, li, h_in, x->p_down, np, ld_h, x->h[0], x->ss[0], s, pos))) return rc;
     // post-attention norm + gate/up (block.rs:101-120, mlp.rs:28-47)
     rc = with_np_bucket((int)l.out_proj.ntiles, [&](auto B) -> int {
       ResidSrc<decltype(B)::value> src{x->h[0], x->p_o, (int)l.out_proj.ntiles, ld_h, l.post_norm, x->h[1], x->ss[1], H};
@@ -723,7 +774,14 @@ static int ctx_zero_state(dz_ctx* x) {
     DZ_HIP_CHECK(hipMemsetAsync(x->conv, 0, (size_t)x->m->n_ssm * 4 * qkvd * 4, x->s));
     DZ_HIP_CHECK(hipMemsetAsync(x->ring_base_dev, 0, (size_t)x->m->n_ssm * 4, x->s));
   }
-  if (x->m->n_attn) DZ_HIP_CHECK(hipMemsetAsync(x->kv, 0, (size_t)x->m->n_attn * 2 * kvsz * 4, x->s));
+  if (x->kv4.on) {
+    for (size_t i = 0; i < x->kv4.layer.size(); ++i) {
+      const Kv4View& v = x->kv4.layer[i];
+      DZ_HIP_CHECK(hipMemsetAsync(v.kc, 0, kv4_bytes(v.nkv, v.hd, v.cap), x->s));
+      if (x->kv4.track) DZ_HIP_CHECK(hipMemsetAsync(x->kv4.w[i], 0, (size_t)v.nkv * v.cap * 4, x->s));
+    }
+    x->kv4.evicted = x->kv4.floor = 0;
+  } else if (x->m->n_attn) DZ_HIP_CHECK(hipMemsetAsync(x->kv, 0, (size_t)x->m->n_attn * 2 * kvsz * 4, x->s));
   std::fill(x->ring_base.begin(), x->ring_base.end(), 0);
   TokState st;
   memset(&st, 0, sizeof st);
@@ -762,7 +820,12 @@ static bool use_graph() {
 static int ctx_run(dz_ctx* x, int n) {
   if (x->pos_host + n > x->m->cfg.max_ctx)
     return set_error(DZ_ERR_TENSOR, "context full: pos %d + %d > max_ctx %d", x->pos_host, n, x->m->cfg.max_ctx);
-  if (use_graph()) {
+  if (int rc = kv4_room(x, n)) return rc;
+  if (x->kv4.on) {
+    // the rows that a token's attention reads size its launches: no graph
+    for (int i = 0; i < n; ++i)
+      if (int rc = enqueue_token(x, x->s, x->pos_host + i)) return rc;
+  } else if (use_graph()) {
     int rc = ctx_build_graph(x);
     if (rc) return rc;
     for (int i = 0; i < n; ++i) DZ_HIP_CHECK(hipGraphLaunch(x->gexec, x->s));
@@ -1259,6 +1322,10 @@ static void bt_release(dz_ctx* x) {
   x->bt.spec = Scratch{};
   x->bt.chunk = Scratch{};
   x->bt.dig = Scratch{};
+  if (x->bt.logp.ptr) (void)hipFree(x->bt.logp.ptr);
+  if (x->kv4.work.ptr) (void)hipFree(x->kv4.work.ptr);
+  x->bt.logp = Scratch{};
+  x->kv4.work = Scratch{};
 }
 
 // Activation buffers for chunks of up to cap tokens.
@@ -1504,6 +1571,11 @@ static int bt_forward(dz_ctx* x, const uint32_t* ids, int n, int out_rows, bool 
                             (int)c.ssm_v_heads, x->bt.gy));
         if ((rc = bt_gemm(x, l.out_proj, x->bt.gy, inner, n, nullptr, x->bt.h, H, 1))) return rc;
       }
+    } else if (x->kv4.on) {
+      // a verify's drafts may be dropped again: only forwards that are kept add to the weights
+      const ProjRows proj{x->bt.yin, ld_in};
+      if ((rc = kv4_attention(x, l, proj, p0, n, x->bt.qb, x->bt.gate, x->bt.gy, x->kv4.track && !verify, s))) return rc;
+      if ((rc = bt_gemm(x, l.out_proj, x->bt.gy, qd, n, nullptr, x->bt.h, H, 1, few ? &gd : nullptr))) return rc;
     } else {
       float* kc = x->kv + (size_t)l.kind_idx * 2 * kvsz;
       float* vc = kc + kvsz;
@@ -1575,6 +1647,7 @@ static int bt_finish(dz_ctx* x, int n, int p0, int last_row) {
 // rollback records kept.  The position does not move until bt_verify_commit.
 static int bt_verify_forward(dz_ctx* x, const uint32_t* draft, int k) {
   if (x->pos_host + k > x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "verify: context full");
+  if (int rc = kv4_room(x, k)) return rc;
   x->bt.pending = 0;
   int rc = bt_forward(x, draft, k, k, true);
   if (rc) return rc;
@@ -1659,18 +1732,48 @@ static int bt_prefill(dz_ctx* x, const uint32_t* ids, int n, float* last_logits,
   return DZ_OK;
 }
 
+// Log probabilities of n rows of logits on the device, targets and results in host arrays (dz_forward_logprobs); enqueued,
+// the caller waits.
+static int ctx_logprobs(dz_ctx* x, const float* logits, int n, const int32_t* targets, int top, float* logp, float* entropy,
+                        int32_t* top_ids, float* top_logp) {
+  const int V = (int)x->m->cfg.vocab;
+  const size_t work = (logprobs_work(n, V, top) + 15) / 16 * 16, nt = (size_t)n * top;
+  if (int rc = x->bt.logp.reserve(work + ((size_t)3 * n + 2 * nt) * 4)) return rc;
+  uint8_t* base = static_cast<uint8_t*>(x->bt.logp.ptr);
+  int32_t* tok = reinterpret_cast<int32_t*>(base + work);
+  float *lp = reinterpret_cast<float*>(tok + n), *en = lp + n, *tl = en + n;
+  int32_t* ids = reinterpret_cast<int32_t*>(tl + nt);
+  if (logp) DZ_HIP_CHECK(hipMemcpyAsync(tok, targets, (size_t)n * 4, hipMemcpyHostToDevice, x->s));
+  if (int rc = logprobs(logits, V, DZ_F32, n, V, tok, top, logp ? lp : nullptr, entropy ? en : nullptr, ids, top_logp ? tl : nullptr,
+                        base, x->s))
+    return rc;
+  if (logp) DZ_HIP_CHECK(hipMemcpyAsync(logp, lp, (size_t)n * 4, hipMemcpyDeviceToHost, x->s));
+  if (entropy) DZ_HIP_CHECK(hipMemcpyAsync(entropy, en, (size_t)n * 4, hipMemcpyDeviceToHost, x->s));
+  if (top) DZ_HIP_CHECK(hipMemcpyAsync(top_ids, ids, nt * 4, hipMemcpyDeviceToHost, x->s));
+  if (top && top_logp) DZ_HIP_CHECK(hipMemcpyAsync(top_logp, tl, nt * 4, hipMemcpyDeviceToHost, x->s));
+  return DZ_OK;
+}
+static int check_logprobs(const dz_ctx* x, int top, const void* targets, const void* logp, const void* top_ids) {
+  const int V = (int)x->m->cfg.vocab;
+  if (top < 0 || top > kLogprobTop || top > V)
+    return set_error(DZ_ERR_UNSUPPORTED, "logprobs: %d alternatives of %d (at most %d)", top, V, kLogprobTop);
+  if ((top && !top_ids) || (logp && !targets)) return set_error(DZ_ERR_MODEL, "null argument");
+  return DZ_OK;
+}
+
 }  // namespace dz
 
-extern "C" {
-
-int dz_ctx_create(dz_model* m, dz_ctx** out) {
-  if (!m || !out) return set_error(DZ_ERR_MODEL, "null argument");
+// A context; kv4_rows > 0: with its key/value cache in 4 bits, for that many rows.
+static int ctx_create(dz_model* m, int kv4_rows, bool track, dz_ctx** out) {
   int rc = ensure_device();
   if (rc) return rc;
-  if ((rc = prepare_gemv_kernels())) return rc;
+  if ((rc = prepare_gemv_kernels()) || (kv4_rows && (rc = prepare_kv4_kernels()))) return rc;
   dz_ctx* x = new dz_ctx();
   x->m = m;
   const dz_config& c = m->cfg;
+  x->kv4.on = kv4_rows > 0;
+  x->kv4.track = kv4_rows > 0 && track;
+  x->kv4.rows = kv4_rows;
   auto fail = [&](int code) { ctx_release(x); return code; };
   hipError_t e = hipStreamCreateWithFlags(&x->s, hipStreamNonBlocking);
   if (e != hipSuccess) return fail(set_error(DZ_ERR_DEVICE, "stream: %s", hipGetErrorString(e)));
@@ -1698,17 +1801,52 @@ int dz_ctx_create(dz_model* m, dz_ctx** out) {
       (rc = alloc_t(A, &x->ssm_state, (size_t)std::max(1, m->n_ssm) * c.ssm_v_heads * hd * hd)) ||
       (rc = alloc_t(A, &x->conv, (size_t)std::max(1, m->n_ssm) * 4 * qkvd)) ||
       (rc = alloc_t(A, &x->ring_base_dev, (size_t)std::max(1, m->n_ssm))) ||
-      (rc = alloc_t(A, &x->kv, (size_t)std::max(1, m->n_attn) * 2 * kvsz)))
+      (rc = alloc_t(A, &x->kv, x->kv4.on ? 1 : (size_t)std::max(1, m->n_attn) * 2 * kvsz)))
     return fail(rc);
+  if (x->kv4.on) {
+    const int nkv = (int)c.n_head_kv, hd4 = (int)c.head_dim, cap = (kv4_rows + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
+    const size_t bytes = kv4_bytes(nkv, hd4, cap);
+    x->kv4.layer.resize((size_t)m->n_attn);
+    x->kv4.w.assign((size_t)m->n_attn, nullptr);
+    for (int i = 0; i <= m->n_attn; ++i) {  // the last is the spare, which an eviction alone needs
+      if (i == m->n_attn && !track) break;
+      uint8_t* base = nullptr;
+      float* w = nullptr;
+      if ((rc = alloc_t(A, &base, bytes)) || (track && (rc = alloc_t(A, &w, (size_t)nkv * cap)))) return fail(rc);
+      (i < m->n_attn ? x->kv4.layer[(size_t)i] : x->kv4.spare) = kv4_carve(base, nkv, hd4, cap);
+      (i < m->n_attn ? x->kv4.w[(size_t)i] : x->kv4.spare_w) = w;
+    }
+    if (track) {
+      // zeros: a tile's rows past the last one are read (and masked), so they must stand for numbers
+      const hipError_t e4 = hipMemsetAsync(x->kv4.spare.kc, 0, bytes, x->s);
+      if (e4 != hipSuccess) return fail(set_error(DZ_ERR_DEVICE, "hipMemsetAsync: %s", hipGetErrorString(e4)));
+      if ((rc = alloc_t(A, &x->kv4.kept, (size_t)nkv * cap))) return fail(rc);
+    }
+    if ((rc = alloc_t(A, &x->kv4.q, (size_t)c.n_head * c.head_dim)) || (rc = alloc_t(A, &x->kv4.gate, (size_t)c.n_head * c.head_dim)))
+      return fail(rc);
+  }
   x->ring_base.assign((size_t)m->n_ssm, 0);
   std::vector<float> rope;
   rope_table(c, rope);
   if ((rc = upload_f32(A, &x->rope, rope.data(), rope.size()))) return fail(rc);
   // argmax partials of "no logits yet": value -inf everywhere, selects token 0 if ever read
   if ((rc = ctx_zero_state(x))) return fail(rc);
-  if (ptk_wanted() && (rc = ptk_prepare(x))) return fail(rc);
+  if (!x->kv4.on && ptk_wanted() && (rc = ptk_prepare(x))) return fail(rc);
   *out = x;
   return DZ_OK;
+}
+
+extern "C" {
+
+int dz_ctx_create(dz_model* m, dz_ctx** out) {
+  if (!m || !out) return set_error(DZ_ERR_MODEL, "null argument");
+  return ctx_create(m, 0, false, out);
+}
+
+int dz_ctx_create_kv4(dz_model* m, int kv_rows, int track, dz_ctx** out) {
+  if (!m || !out) return set_error(DZ_ERR_MODEL, "null argument");
+  if (kv_rows < 0 || kv_rows > m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "4-bit cache of %d rows (max_ctx %d)", kv_rows, m->cfg.max_ctx);
+  return ctx_create(m, kv_rows ? kv_rows : m->cfg.max_ctx, track != 0, out);
 }
 
 int dz_ctx_free(dz_ctx* x) {
@@ -1771,6 +1909,7 @@ int dz_forward_batch(dz_ctx* x, const uint32_t* ids, int n, int start_pos, float
   if (start_pos != x->pos_host)
     return set_error(DZ_ERR_TENSOR, "forward_batch: start_pos %d != context position %d", start_pos, x->pos_host);
   if (x->pos_host + n > x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "forward_batch: context full");
+  if (int rc0 = kv4_room(x, n)) return rc0;
   x->bt.pending = 0;
   const size_t V = (size_t)x->m->cfg.vocab;
   if (batch_wanted()) return bt_prefill(x, ids, n, last_logits, per_pos);
@@ -1926,6 +2065,39 @@ int dz_ctx_get_ssm_state(dz_ctx* x, int layer, float* state, float* conv_hist, i
   return DZ_OK;
 }
 
+// Rows [0, len) of a 4-bit cache from (set) or to host arrays [kv head][len][dim].
+static int kv4_rows_io(dz_ctx* x, int layer, float* k, float* v, int len, bool set) {
+  const Kv4View& c = x->kv4.layer[(size_t)layer];
+  if (len > x->kv4.rows) return set_error(DZ_ERR_TENSOR, "kv len %d of a 4-bit cache for %d rows", len, x->kv4.rows);
+  if (len == 0) return DZ_OK;
+  const size_t per = (size_t)len * c.hd, n = (size_t)c.nkv * per;
+  Scratch tmp;
+  int rc = tmp.reserve(2 * n * sizeof(float));
+  if (rc) return rc;
+  float *dk = static_cast<float*>(tmp.ptr), *dv = dk + n;
+  auto run = [&]() -> int {
+    if (!set) {
+      if (int r = kv4_read(c, 0, len, dk, dv, x->s)) return r;
+      DZ_HIP_CHECK(hipMemcpyAsync(k, dk, n * sizeof(float), hipMemcpyDeviceToHost, x->s));
+      DZ_HIP_CHECK(hipMemcpyAsync(v, dv, n * sizeof(float), hipMemcpyDeviceToHost, x->s));
+      return DZ_OK;
+    }
+    DZ_HIP_CHECK(hipMemcpyAsync(dk, k, n * sizeof(float), hipMemcpyHostToDevice, x->s));
+    DZ_HIP_CHECK(hipMemcpyAsync(dv, v, n * sizeof(float), hipMemcpyHostToDevice, x->s));
+    for (int h = 0; h < c.nkv; ++h)
+      if (int r = kv4_append(kv4_head(c, h), 0, dk + h * per, c.hd, dv + h * per, c.hd, DZ_F32, len, x->s)) return r;
+    if (x->kv4.track)
+      DZ_HIP_CHECK(hipMemset2DAsync(x->kv4.w[(size_t)layer], (size_t)c.cap * 4, 0, (size_t)len * 4, (size_t)c.nkv, x->s));
+    return DZ_OK;
+  };
+  rc = run();
+  const hipError_t e = hipStreamSynchronize(x->s);
+  (void)hipFree(tmp.ptr);
+  if (rc) return rc;
+  DZ_HIP_CHECK(e);
+  return DZ_OK;
+}
+
 int dz_ctx_set_kv(dz_ctx* x, int layer, const float* k, const float* v, int len) {
   LayerDev* l;
   int rc = layer_of(x, layer, true, &l);
@@ -1934,6 +2106,7 @@ int dz_ctx_set_kv(dz_ctx* x, int layer, const float* k, const float* v, int len)
   if (len < 0 || len > c.max_ctx) return set_error(DZ_ERR_TENSOR, "kv len %d", len);
   // the copies below are not ordered with the context's stream: enqueued steps still read and append rows
   DZ_HIP_CHECK(hipStreamSynchronize(x->s));
+  if (x->kv4.on) return kv4_rows_io(x, l->kind_idx, const_cast<float*>(k), const_cast<float*>(v), len, true);
   const size_t kvsz = (size_t)c.n_head_kv * c.max_ctx * c.head_dim, hd = (size_t)c.head_dim;
   float* kb = x->kv + (size_t)l->kind_idx * 2 * kvsz;
   for (int h = 0; h < c.n_head_kv; ++h) {
@@ -1951,6 +2124,7 @@ int dz_ctx_get_kv(dz_ctx* x, int layer, float* k, float* v, int len) {
   const dz_config& c = x->m->cfg;
   if (len < 0 || len > c.max_ctx) return set_error(DZ_ERR_TENSOR, "kv len %d", len);
   DZ_HIP_CHECK(hipStreamSynchronize(x->s));
+  if (x->kv4.on) return kv4_rows_io(x, l->kind_idx, k, v, len, false);
   const size_t kvsz = (size_t)c.n_head_kv * c.max_ctx * c.head_dim, hd = (size_t)c.head_dim;
   const float* kb = x->kv + (size_t)l->kind_idx * 2 * kvsz;
   for (int h = 0; h < c.n_head_kv; ++h) {
@@ -1961,11 +2135,66 @@ int dz_ctx_get_kv(dz_ctx* x, int layer, float* k, float* v, int len) {
   return DZ_OK;
 }
 
-// In this build every attention layer holds exactly `pos` cached positions.
+// Every attention layer holds exactly `pos` cached positions, less those evicted from a 4-bit cache.
 int dz_ctx_kv_len(dz_ctx* x, int layer) {
   LayerDev* l;
   if (layer_of(x, layer, true, &l)) return -1;
-  return x->pos_host;
+  return x->pos_host - x->kv4.evicted;
+}
+
+int dz_ctx_kv_weights(dz_ctx* x, int layer, float* weights, int len) {
+  LayerDev* l;
+  int rc = layer_of(x, layer, true, &l);
+  if (rc) return rc;
+  if (!x->kv4.track) return set_error(DZ_ERR_UNSUPPORTED, "the context keeps no weights (dz_ctx_create_kv4 with track)");
+  if (!weights || len < 0 || len > x->kv4.rows) return set_error(DZ_ERR_TENSOR, "kv weights: len %d", len);
+  const Kv4View& v = x->kv4.layer[(size_t)l->kind_idx];
+  if (len)
+    DZ_HIP_CHECK(hipMemcpy2DAsync(weights, (size_t)len * 4, x->kv4.w[(size_t)l->kind_idx], (size_t)v.cap * 4, (size_t)len * 4,
+                                  (size_t)v.nkv, hipMemcpyDeviceToHost, x->s));
+  DZ_HIP_CHECK(hipStreamSynchronize(x->s));
+  return DZ_OK;
+}
+
+int dz_ctx_kv_evict(dz_ctx* x, int keep, int recent, int32_t* kept) {
+  if (!x) return set_error(DZ_ERR_MODEL, "null context");
+  if (int rc0 = ctx_usable(x)) return rc0;
+  if (!x->kv4.track) return set_error(DZ_ERR_UNSUPPORTED, "the context keeps no weights (dz_ctx_create_kv4 with track)");
+  if (recent < 0 || keep < recent) return set_error(DZ_ERR_TENSOR, "evict: keep %d, of which %d recent", keep, recent);
+  const int rows = x->pos_host - x->kv4.evicted, m = std::min(keep, rows);
+  x->bt.pending = 0;
+  auto run = [&]() -> int {
+    for (size_t i = 0; i < x->kv4.layer.size(); ++i) {
+      Kv4View& v = x->kv4.layer[i];
+      if (int rc = kv4_evict(v, rows, x->kv4.w[i], v.cap, keep, recent, x->kv4.spare, x->kv4.spare_w, v.cap, x->kv4.kept, x->s)) return rc;
+      std::swap(v, x->kv4.spare);
+      std::swap(x->kv4.w[i], x->kv4.spare_w);
+      if (kept && m)
+        DZ_HIP_CHECK(hipMemcpyAsync(kept + i * (size_t)v.nkv * m, x->kv4.kept, (size_t)v.nkv * m * 4, hipMemcpyDeviceToHost, x->s));
+    }
+    return DZ_OK;
+  };
+  const int rc = run();
+  const hipError_t e = hipStreamSynchronize(x->s);
+  if (rc || e != hipSuccess) {
+    x->poisoned = true;  // some layers may hold other rows than the others
+    if (rc) return rc;
+    DZ_HIP_CHECK(e);
+  }
+  if (m < rows) {
+    x->kv4.evicted += rows - m;
+    x->kv4.floor = x->pos_host;
+  }
+  return DZ_OK;
+}
+
+// Positions before an eviction cannot be gone back to, and a 4-bit cache may hold fewer rows than max_ctx.
+static int kv4_back(const dz_ctx* x, int pos) {
+  if (!x->kv4.on) return DZ_OK;
+  if (x->kv4.evicted && pos < x->kv4.floor)
+    return set_error(DZ_ERR_TENSOR, "position %d lies before the eviction at %d", pos, x->kv4.floor);
+  if (pos - x->kv4.evicted > x->kv4.rows) return set_error(DZ_ERR_TENSOR, "position %d: 4-bit cache for %d rows", pos, x->kv4.rows);
+  return DZ_OK;
 }
 
 int dz_kv_truncate(dz_ctx* x, int len) {
@@ -1973,6 +2202,7 @@ int dz_kv_truncate(dz_ctx* x, int len) {
   x->bt.pending = 0;
   if (len >= x->pos_host) return DZ_OK;  // KvCache::truncate keeps longer requests as no-ops
   if (len < 0) return set_error(DZ_ERR_TENSOR, "truncate to %d", len);
+  if (int rc = kv4_back(x, len)) return rc;
   return ctx_move_pos(x, len);
 }
 
@@ -1981,6 +2211,7 @@ int dz_ctx_set_pos(dz_ctx* x, int pos) {
   x->bt.pending = 0;
   // max_ctx itself is a full context: forwards are refused there, but the state is valid
   if (pos < 0 || pos > x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "pos %d out of [0, max_ctx]", pos);
+  if (int rc = kv4_back(x, pos)) return rc;
   return ctx_move_pos(x, pos);
 }
 
@@ -2001,6 +2232,11 @@ int dz_ctx_copy_state(dz_ctx* dst, const dz_ctx* src) {
   if (!same) return set_error(DZ_ERR_MODEL, "copy_state: the contexts' model shapes differ");
   const int pos = src->pos_host;
   if (pos > a.max_ctx) return set_error(DZ_ERR_TENSOR, "copy_state: position %d exceeds max_ctx %d", pos, a.max_ctx);
+  if (dst->kv4.on != src->kv4.on || dst->kv4.track != src->kv4.track)
+    return set_error(DZ_ERR_MODEL, "copy_state: the contexts' key/value caches are of different kinds");
+  const int rows = pos - src->kv4.evicted;
+  if (dst->kv4.on && rows > dst->kv4.rows)
+    return set_error(DZ_ERR_TENSOR, "copy_state: %d rows into a 4-bit cache for %d", rows, dst->kv4.rows);
   DZ_HIP_CHECK(hipStreamSynchronize(src->s));
   DZ_HIP_CHECK(hipStreamSynchronize(dst->s));
   dst->bt.pending = 0;
@@ -2013,7 +2249,27 @@ int dz_ctx_copy_state(dz_ctx* dst, const dz_ctx* src) {
     DZ_HIP_CHECK(hipMemcpyAsync(dst->conv, src->conv, (size_t)n_ssm * 4 * qkvd * 4, hipMemcpyDeviceToDevice, s));
     DZ_HIP_CHECK(hipMemcpyAsync(dst->ring_base_dev, src->ring_base_dev, (size_t)n_ssm * 4, hipMemcpyDeviceToDevice, s));
   }
-  if (n_attn && pos) {
+  if (dst->kv4.on) {
+    // whole tiles of 32 rows
+    const size_t t = (size_t)(rows + kKv4Tile - 1) / kKv4Tile;
+    for (size_t i = 0; i < dst->kv4.layer.size() && t; ++i) {
+      const Kv4View &d = dst->kv4.layer[i], &o = src->kv4.layer[i];
+      auto copy = [&](uint8_t* to, size_t ldd, const uint8_t* from, size_t lds, size_t n) {
+        return hipMemcpy2DAsync(to, ldd, from, lds, n, (size_t)d.nkv, hipMemcpyDeviceToDevice, s);
+      };
+      const size_t nc = t * kKv4Tile * (size_t)(d.hd / 2), ns = t * kKv4Tile * (size_t)(d.hd / 32);
+      DZ_HIP_CHECK(copy(d.kc, d.code_head(), o.kc, o.code_head(), nc));
+      DZ_HIP_CHECK(copy(d.vc, d.code_head(), o.vc, o.code_head(), nc));
+      DZ_HIP_CHECK(copy(d.ks, d.scale_head(), o.ks, o.scale_head(), ns));
+      DZ_HIP_CHECK(copy(d.vs, d.scale_head(), o.vs, o.scale_head(), ns));
+      DZ_HIP_CHECK(copy(d.bad, (size_t)(d.cap / kKv4Tile), o.bad, (size_t)(o.cap / kKv4Tile), t));
+      if (dst->kv4.track)
+        DZ_HIP_CHECK(copy(reinterpret_cast<uint8_t*>(dst->kv4.w[i]), (size_t)d.cap * 4, reinterpret_cast<const uint8_t*>(src->kv4.w[i]),
+                          (size_t)o.cap * 4, t * kKv4Tile * 4));
+    }
+    dst->kv4.evicted = src->kv4.evicted;
+    dst->kv4.floor = src->kv4.floor;
+  } else if (n_attn && pos) {
     // rows [0, pos) of every (layer, K|V, kv head) block; each context strides by its own max_ctx
     const size_t row = (size_t)a.head_dim * 4;
     DZ_HIP_CHECK(hipMemcpy2DAsync(dst->kv, (size_t)a.max_ctx * row, src->kv, (size_t)b.max_ctx * row, (size_t)pos * row,
@@ -2041,6 +2297,7 @@ int dz_ctx_mixer_step_dev(dz_ctx* x, int layer, const float* h_dev, float* h_out
   if (int rc0 = ctx_usable(x)) return rc0;
   if (layer < 0 || layer >= x->m->cfg.n_layers) return set_error(DZ_ERR_TENSOR, "layer %d out of range", layer);
   if (x->pos_host >= x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "context full");
+  if (int rc0 = kv4_room(x, 1)) return rc0;
   const dz_config& c = x->m->cfg;
   int64_t ld_in, ld_h, ld_gu;
   int th, to, tf;
@@ -2068,6 +2325,7 @@ int dz_ctx_mixer_step(dz_ctx* x, int layer, float* h) {
   if (int rc0 = ctx_usable(x)) return rc0;
   if (layer < 0 || layer >= x->m->cfg.n_layers) return set_error(DZ_ERR_TENSOR, "layer %d out of range", layer);
   if (x->pos_host >= x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "context full");
+  if (int rc0 = kv4_room(x, 1)) return rc0;
   const dz_config& c = x->m->cfg;
   int64_t ld_in, ld_h, ld_gu;
   int th, to, tf;
@@ -2089,4 +2347,53 @@ int dz_ctx_mixer_step(dz_ctx* x, int layer, float* h) {
   return ctx_set_pos_dev(x, P + 1);
 }
 
+int dz_forward_logprobs(dz_ctx* x, const uint32_t* ids, const int32_t* targets, int n, int start_pos, int top, float* logp,
+                        float* entropy, int32_t* top_ids, float* top_logp) {
+  if (!x || !ids) return set_error(DZ_ERR_MODEL, "null argument");
+  if (n < 1) return set_error(DZ_ERR_TENSOR, "forward_logprobs: empty batch");
+  if (int rc0 = ctx_usable(x)) return rc0;
+  if (int rc0 = check_logprobs(x, top, targets, logp, top_ids)) return rc0;
+  if (start_pos != x->pos_host)
+    return set_error(DZ_ERR_TENSOR, "forward_logprobs: start_pos %d != context position %d", start_pos, x->pos_host);
+  if (x->pos_host + n > x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "forward_logprobs: context full");
+  if (int rc0 = kv4_room(x, n)) return rc0;
+  for (int i = 0; i < n; ++i)
+    if (ids[i] >= (uint32_t)x->m->cfg.vocab) return set_error(DZ_ERR_TENSOR, "token id %u >= vocab %d", ids[i], x->m->cfg.vocab);
+  x->bt.pending = 0;
+  constexpr int kChunk = 128;  // rows of logits on the device at a time, as the per-position logits of a batch
+  auto run = [&]() -> int {
+    for (int i0 = 0; i0 < n; i0 += kChunk) {
+      const int k = std::min(kChunk, n - i0);
+      int rc = bt_forward(x, ids + i0, k, k, false);
+      if (rc || (rc = bt_finish(x, k, x->pos_host, k - 1))) return rc;
+      const size_t t0 = (size_t)i0 * top;
+      if ((rc = ctx_logprobs(x, x->bt.logits, k, targets ? targets + i0 : nullptr, top, logp ? logp + i0 : nullptr,
+                             entropy ? entropy + i0 : nullptr, top_ids + t0, top_logp ? top_logp + t0 : nullptr)))
+        return rc;
+    }
+    return DZ_OK;
+  };
+  const int rc = run();
+  // also when a later chunk fails: those before it still read ids and write the results
+  const hipError_t e = hipStreamSynchronize(x->s);
+  if (rc) return rc;
+  DZ_HIP_CHECK(e);
+  return DZ_OK;
+}
+
+int dz_ctx_logprobs(dz_ctx* x, int32_t token, int top, float* logp, float* entropy, int32_t* top_ids, float* top_logp) {
+  if (!x) return set_error(DZ_ERR_MODEL, "null context");
+  if (int rc0 = check_logprobs(x, top, &token, logp, top_ids)) return rc0;
+  const int rc = ctx_logprobs(x, x->logits, 1, &token, top, logp, entropy, top_ids, top_logp);
+  const hipError_t e = hipStreamSynchronize(x->s);
+  if (rc) return rc;
+  DZ_HIP_CHECK(e);
+  return DZ_OK;
+}
+
 }  // extern "C"
+
+namespace dz {
+int ctx_kv_capacity(const dz_ctx* x) { return x->kv4.on ? x->kv4.rows : x->m->cfg.max_ctx; }
+int ctx_kv_evicted(const dz_ctx* x) { return x->kv4.evicted; }
+}  // namespace dz

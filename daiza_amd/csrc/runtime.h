@@ -55,6 +55,10 @@ const dz_config* ctx_config(const dz_ctx* x);
 // save is refused until a reset or a restore), else DZ_OK.
 int ctx_usable(const dz_ctx* x);
 
+// Rows that a context's key/value cache holds at most, and rows evicted from it.
+int ctx_kv_capacity(const dz_ctx* x);
+int ctx_kv_evicted(const dz_ctx* x);
+
 // Sum of the tile-group partials into each segment's output: y = [y +] sum_tg part[tg][row].
 hipError_t launch_partial_reduce(const float* part, int64_t ld, int n_tg, const ReduceSeg* segs, int nseg,
                                  int accumulate, hipStream_t s);

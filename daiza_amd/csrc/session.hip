@@ -102,6 +102,7 @@ static int ctx_save(dz_ctx* x, const char* path, uint64_t context_length, const 
   if (int rc0 = ctx_usable(x)) return rc0;
   const dz_config* c = ctx_config(x);
   const int pos = dz_ctx_pos(x);
+  if (ctx_kv_evicted(x)) return set_error(DZ_ERR_UNSUPPORTED, "a session file holds every position's row; %d were evicted", ctx_kv_evicted(x));
   File fh;
   fh.f = fopen(path, "wb");
   if (!fh.f) return set_error(DZ_ERR_MODEL, "create %s", path);
@@ -187,6 +188,8 @@ static int ctx_load(dz_ctx* x, const char* path, uint64_t context_length, uint32
   if (nb != (uint32_t)c->n_layers) return set_error(DZ_ERR_MODEL, "block_count mismatch: file=%u expected=%d", nb, c->n_layers);
   if (pos > (uint64_t)c->max_ctx) return set_error(DZ_ERR_TENSOR, "session position %llu exceeds max_ctx %d",
                                                    (unsigned long long)pos, c->max_ctx);
+  if (pos > (uint64_t)ctx_kv_capacity(x))
+    return set_error(DZ_ERR_TENSOR, "session position %llu exceeds the cache's %d rows", (unsigned long long)pos, ctx_kv_capacity(x));
   // the history is bounded before anything is allocated for it: at most 2^32 tokens, and no more
   // than the bytes left after the header
   struct stat sb;

@@ -262,6 +262,25 @@ int dz_model_create_synth(const dz_config* cfg, uint64_t seed, dz_model** out);
 int dz_model_free(dz_model* m);
 int dz_model_weight_bytes(const dz_model* m, uint64_t* q1_bytes);
 
+/*
+ * A context whose attention layers hold their keys and values in 4 bits (dz_kv4 above, 1088 instead of 8192 bytes a position
+ * and layer at the 27B shape), for kv_rows rows (0: max_ctx; fewer than max_ctx with eviction).  Every call on
+ * contexts works on it, by the per-kernel path (dz_ctx_token_kernel is 0); results differ from an f32 context's by what
+ * 4 bits lose.  dz_ctx_get_kv reads what the rows stand for, dz_ctx_set_kv rounds to it; dz_ctx_copy_state
+ * needs contexts of one kind.  The reference has no such cache.
+ * track != 0: the context also sums the attention weight that each cached row receives (over the heads of a key/value
+ * head's group) in every forward that is kept, starting from 0 when the row is written; a verify adds none.
+ */
+int dz_ctx_create_kv4(dz_model* m, int kv_rows, int track, dz_ctx** out);
+/* Eviction by accumulated attention weight on a context that tracks it: every attention layer keeps, per key/value head,
+ * its newest `recent` rows and the keep - recent others of the largest weights (dz_kv4_evict_dev), their weights with
+ * them.  The position stays where it is and later tokens' positions follow it; dz_ctx_kv_len tells the rows held.
+ * kept (host, may be NULL) receives [attention layer][kv head][min(keep, rows held)] indices of the rows that stayed.
+ * A position before the last eviction cannot be gone back to (dz_kv_truncate, dz_ctx_set_pos), nor saved (dz_ctx_save). */
+int dz_ctx_kv_evict(dz_ctx* c, int keep, int recent, int32_t* kept);
+/* The weights of an attention layer's first len rows, weights[kv_heads][len] on the host. */
+int dz_ctx_kv_weights(dz_ctx* c, int layer, float* weights, int len);
+
 /* Context = ModelState + ForwardContext (forward.rs:32-131): KV caches, SSM states, position.
  * If a forward fails with DZ_ERR_DEVICE because a device-side wait gave up, the launch may have
  * updated part of the state; the context then refuses every forward with DZ_ERR_DEVICE until
@@ -286,6 +305,17 @@ int dz_forward_token(dz_ctx* c, uint32_t token, float* logits_or_null, uint32_t*
  */
 int dz_forward_batch(dz_ctx* c, const uint32_t* ids, int n, int start_pos,
                      float* last_logits_or_null, float* per_pos_logits_or_null);
+
+/*
+ * dz_forward_batch with log probabilities in place of logits, formed on the device (dz_logprobs_dev; 1 MB of logits a position
+ * stay there): logp[i] of targets[i] under the logits after ids[i] (targets[i] outside the vocabulary, -1 for one:
+ * NaN), entropy[i], and the `top` best alternatives top_ids[i][top], top_logp[i][top].  Host arrays; logp (with
+ * targets), entropy and top_logp may be NULL, top may be 0.  A prompt's score is targets[i] = ids[i + 1].
+ */
+int dz_forward_logprobs(dz_ctx* c, const uint32_t* ids, const int32_t* targets, int n, int start_pos, int top, float* logp,
+                        float* entropy, int32_t* top_ids, float* top_logp);
+/* The same of the context's last logits (which predict the next token). */
+int dz_ctx_logprobs(dz_ctx* c, int32_t token, int top, float* logp, float* entropy, int32_t* top_ids, float* top_logp);
 
 /*
  * Greedy decode of n tokens entirely on the device: the first forward consumes `first_token`,
