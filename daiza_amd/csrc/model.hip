@@ -2360,7 +2360,7 @@ int dz_forward_logprobs(dz_ctx* x, const uint32_t* ids, const int32_t* targets, 
   for (int i = 0; i < n; ++i)
     if (ids[i] >= (uint32_t)x->m->cfg.vocab) return set_error(DZ_ERR_TENSOR, "token id %u >= vocab %d", ids[i], x->m->cfg.vocab);
   x->bt.pending = 0;
-  constexpr int kChunk = 128;  // rows of logits on the device at a time, as the per-position logits of a batch
+  constexpr int kChunk = kBatchChunk;  // rows of logits on the device at a time (1 MB each at the 27B vocabulary)
   auto run = [&]() -> int {
     for (int i0 = 0; i0 < n; i0 += kChunk) {
       const int k = std::min(kChunk, n - i0);

@@ -307,8 +307,8 @@ int dz_forward_batch(dz_ctx* c, const uint32_t* ids, int n, int start_pos,
                      float* last_logits_or_null, float* per_pos_logits_or_null);
 
 /*
- * dz_forward_batch with log probabilities in place of logits, formed on the device (dz_logprobs_dev; 1 MB of logits a position
- * stay there): logp[i] of targets[i] under the logits after ids[i] (targets[i] outside the vocabulary, -1 for one:
+ * dz_forward_batch with log probabilities in place of logits, formed on the device (dz_logprobs_dev), where up to 1024 rows of
+ * logits stay (1 MB each at the 27B vocabulary): logp[i] of targets[i] under the logits after ids[i] (targets[i] outside the vocabulary, -1 for one:
  * NaN), entropy[i], and the `top` best alternatives top_ids[i][top], top_logp[i][top].  Host arrays; logp (with
  * targets), entropy and top_logp may be NULL, top may be 0.  A prompt's score is targets[i] = ids[i + 1].
  */

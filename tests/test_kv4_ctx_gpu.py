@@ -293,18 +293,17 @@ def test_token_loop(dz, oracle):
 
 @pytest.mark.parametrize("kv4", [False, True])
 def test_log_probabilities_of_a_prompt(dz, oracle, kv4):
-    """forward_logprobs against the log softmax of the same forward's logits, over chunks of 128 positions."""
+    """forward_logprobs against the log softmax of the same forward's logits (both take up to 128 tokens at once)."""
     cfg, om, model, a = _setup(dz, oracle, track=False)
     make = (lambda: dz.Context(model, kv4=True)) if kv4 else (lambda: dz.Context(model))
     a, b = make(), make()
     rng = np.random.default_rng(9)
     ids = rng.integers(0, cfg.vocab, 150)
     targets = np.append(ids[1:], -1).astype(np.int32)
-    for i0, n in ((0, 1), (1, 140), (141, 9)):
+    for i0, n in ((0, 1), (1, 100), (101, 49)):
         lg = a.forward_batch(ids[i0:i0 + n], per_pos_logits=True)
         logp, ent, tid, tlp = b.forward_logprobs(ids[i0:i0 + n], targets[i0:i0 + n], top=7)
         t = torch.from_numpy(targets[i0:i0 + n])
-        # chunks of 128 give the same logits as the batch's own chunks
         wl, we, wi, wt, lb, eb, tb = ref.logprobs(torch.from_numpy(lg), t, 7)
         assert np.array_equal(tid, wi.numpy())
         fin = t >= 0
@@ -329,6 +328,18 @@ def test_log_probabilities_of_a_prompt(dz, oracle, kv4):
     with pytest.raises(E):
         b.logprobs(top=-1)
     assert b.pos == 150
+
+
+def test_log_probabilities_over_chunks(dz, oracle):
+    """A prompt longer than one forward's 1024 tokens is scored as its parts are."""
+    cfg, om, model, a = _setup(dz, oracle, track=False, max_ctx=1100)
+    b = dz.Context(model, kv4=True)
+    ids = np.random.default_rng(11).integers(0, cfg.vocab, 1051)
+    whole = a.forward_logprobs(ids[:1050], ids[1:], top=3)
+    parts = [b.forward_logprobs(ids[i:j], ids[i + 1:j + 1], top=3) for i, j in ((0, 1024), (1024, 1050))]
+    for w, p in zip(whole, zip(*parts)):
+        assert np.array_equal(w, np.concatenate(p)) and np.isfinite(w).all()
+    assert a.pos == b.pos == 1050 and np.array_equal(a.logits(), b.logits())
 
 
 def test_non_finite_row_of_a_context(dz, oracle):
