@@ -337,9 +337,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Where a call's results go: the output itself (nch = 1) or a record (m, l, o[HD]) per row and chunk of positions.
 struct AttendOut {
-  float* rec;         // [n][nq][nch][2 + HD]
-  float2* stats;      // [n][nq] (m, l), or null
-  const float* gate;  // [n][nq][HD]: the output times its sigmoid, or null
+  float* rec = nullptr;         // [n][nq][nch][2 + HD]
+  float2* stats = nullptr;      // [n][nq] (m, l), or null
+  const float* gate = nullptr;  // [n][nq][HD]: the output times its sigmoid, or null
+  float* scores = nullptr;      // [n][nq][cap]: the scores (few rows, for the weights), or null
   // Element d of row `row` (HD elements each).
   template <class E, int HD>
   __device__ __forceinline__ E value(float o, float l, size_t row, int d) const {
@@ -477,6 +478,14 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
+      }
+      if constexpr (RT == 1) {
+        // every position up to the last row's is in some wave's tile, so that the rows are written whole
+        if (dst.scores && rho < rows) {
+          float* y = dst.scores + ((size_t)(rho / grp) * nq + g * grp + rho % grp) * c.cap + p0 + 4 * lk;
+          *reinterpret_cast<f32x4*>(y) = f32x4{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<f32x4*>(y + 16) = f32x4{x[4], x[5], x[6], x[7]};
+        }
       }
       const float bm = max_over_lk(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
       const float mn = fmaxf(m, bm);
@@ -689,6 +698,39 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, 
   if (src.stats && d == 0) src.stats[row] = make_float2(m, l);
 }
 
+// weights[g][r] += Σ exp(s_ρr - m_ρ) / l_ρ over the group's query rows ρ in order, from the scores that the attention left
+// (few rows): four positions a thread.  Grid (ceil(len / 1024), nkv), 256 threads.
+__global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __restrict__ scores, int cap, int len, int nq, int grp,
+                                                              int rows, const float2* __restrict__ stats,
+                                                              float* __restrict__ weights, int64_t ldw) {
+  const int g = blockIdx.y, r = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+  if (r >= len) return;
+  f32x4 s[16];
+  float2 st[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int rho = min(k, rows - 1);
+    const size_t row = (size_t)(rho / grp) * nq + g * grp + rho % grp;
+    s[k] = *reinterpret_cast<const f32x4*>(scores + row * cap + r);  // cap is a multiple of 32
+    st[k] = stats[row];
+  }
+  f32x4 a{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (k < rows) {
+      const float inv = 1.f / st[k].y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // what a row does not see has the score -inf; it adds nothing though the row's sum be a NaN
+        const float p = __builtin_amdgcn_exp2f((s[k][i] - st[k].x) * kLog2e) * inv;
+        a[i] += s[k][i] == -INFINITY ? 0.f : p;
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (r + i < len) weights[(size_t)g * ldw + r + i] += a[i];
+}
+
 // The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile][block][part][lane].
 // Grid (row tiles, nkv), 256 threads.
 template <int HD, class E>
@@ -860,8 +902,9 @@ constexpr int kKv4SplitTiles = 4;
 
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   const size_t rows = (size_t)n * n_head, nch = (size_t)attend_max_chunks(n, n_head, c.nkv);
-  const size_t rec = nch > 1 ? rows * nch * (size_t)(2 + c.hd) * sizeof(float) : 0;
+  const size_t rec = nch > 1 ? (rows * nch * (size_t)(2 + c.hd) * sizeof(float) + 15) / 16 * 16 : 0;
   const int tiles = (n * (n_head / c.nkv) + 15) / 16;
+  if (tiles == 1) return (rows * sizeof(float2) + 15) / 16 * 16 + rec + rows * (size_t)c.cap * sizeof(float);
   const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * 16 * c.nkv * c.hd * 2 * Parts<float>::q : 0;  // over the records
   return (rows * sizeof(float2) + 15) / 16 * 16 + std::max(rec, split);
 }
@@ -874,12 +917,14 @@ constexpr size_t attend_lds(int rows) {
   return queries > join ? queries : join;
 }
 
-// Dynamic-LDS limits, set once before any launch or capture.
+// Dynamic-LDS limits, set once for each device before any launch or capture.
 int prepare_kv4_kernels() {
   static std::mutex mu;
-  static bool done = false;
+  static bool done[64];
   std::lock_guard<std::mutex> lock(mu);
-  if (done) return DZ_OK;
+  int dev = 0;
+  DZ_HIP_CHECK(hipGetDevice(&dev));
+  if (dev < 64 && done[dev]) return DZ_OK;
   for (int hd : {64, 128, 256})
     for (int type : {DZ_F32, DZ_F16, DZ_BF16})
       for (AttendForm form : {AttendForm{1, 4}, AttendForm{1, 8}, AttendForm{2, 4}, AttendForm{4, 2}}) {
@@ -896,7 +941,7 @@ int prepare_kv4_kernels() {
         });
         if (rc) return rc;
       }
-  done = true;
+  if (dev < 64) done[dev] = true;
   return DZ_OK;
 }
 
@@ -916,6 +961,8 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       dst.stats = weights ? stats : nullptr;
       dst.gate = gate;
       dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
+      // behind the records of the most chunks
+      dst.scores = weights && form.rt == 1 ? dst.rec + (most > 1 ? ((size_t)n * n_head * most * (2 + HD) + 3) / 4 * 4 : 0) : nullptr;
       const int rc = with_form(form, [&](auto R, auto P) -> int {
         constexpr int RT = decltype(R)::value, PS = decltype(P)::value;
         const unsigned wgs = (unsigned)((rows + 16 * RT - 1) / (16 * RT) * c.nkv * nch);
@@ -932,7 +979,11 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
         else kv4_merge_kernel<HD, E, 16><<<grid, 256, 0, s>>>(dst, nch, n_head, (E*)out, ldo);
         DZ_HIP_CHECK(hipGetLastError());
       }
-      if (weights) {
+      if (weights && dst.scores) {
+        kv4_few_weights_kernel<<<dim3((unsigned)((len + 1023) / 1024), (unsigned)c.nkv), 256, 0, s>>>(
+            dst.scores, c.cap, len, n_head, n_head / c.nkv, rows, stats, weights, ldw);
+        DZ_HIP_CHECK(hipGetLastError());
+      } else if (weights) {
         // as many rows of keys a wave as leave about a workgroup for each compute unit
         const int64_t units = ((int64_t)len + 63) / 64 * c.nkv;
         const int row_tiles = (rows + 15) / 16;
@@ -1025,19 +1076,16 @@ __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restric
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, up = pass == 0 ? 32 : pass == 1 ? 21 : 10;
     hist[tid] = hist[1024 + tid] = 0;
     __syncthreads();
+    // keys of 0 (rows never attended to, often many) are counted by the wave, not one after another in their bin
+    constexpr unsigned kZero = 0x80000000u;
+    const bool zeros_in = pass == 0 || (kZero >> (up & 31)) == (prefix >> (up & 31));
+    int zeros = 0;
     rows([&](int, unsigned k, bool has) {
-      const bool in = has && (pass == 0 || (k >> (up & 31)) == (prefix >> (up & 31)));
-      const unsigned long long any = __ballot(in);
-      if (!any) return;
-      const unsigned bin = (k >> sh) & (pass == 2 ? 1023u : 2047u);
-      // a wave of equal keys (rows never attended to) counts once
-      const unsigned first = (unsigned)__builtin_amdgcn_readlane((int)bin, __builtin_ctzll(any));
-      if (__ballot(in && bin == first) == any) {
-        if (lane == 0) atomicAdd(&hist[first], (unsigned)__popcll(any));
-      } else if (in) {
-        atomicAdd(&hist[bin], 1u);
-      }
+      if (zeros_in) zeros += __popcll(__ballot(has && k == kZero));
+      if (has && k != kZero && (pass == 0 || (k >> (up & 31)) == (prefix >> (up & 31))))
+        atomicAdd(&hist[(k >> sh) & (pass == 2 ? 1023u : 2047u)], 1u);
     });
+    if (zeros && lane == 0) atomicAdd(&hist[(kZero >> sh) & (pass == 2 ? 1023u : 2047u)], (unsigned)zeros);
     __syncthreads();
     // how many keys lie in the bins above a thread's two, from the top
     const unsigned hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid], own = hi + lo;
@@ -1262,6 +1310,7 @@ int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int
   if (n_head < 1 || n_head > 65535 || n_head % c->v.nkv)
     return set_error(DZ_ERR_TENSOR, "attend: %d heads on %d kv heads", n_head, c->v.nkv);
   if (n < 1 || n > c->len) return set_error(DZ_ERR_TENSOR, "attend: %d queries over %d rows", n, c->len);
+  if ((int64_t)n * n_head > 1 << 30) return set_error(DZ_ERR_UNSUPPORTED, "attend: %d queries of %d heads", n, n_head);
   int rc = check_type(type);
   if (rc) return rc;
   const int64_t row = (int64_t)n_head * c->v.hd;

@@ -1846,7 +1846,11 @@ int dz_ctx_create(dz_model* m, dz_ctx** out) {
 int dz_ctx_create_kv4(dz_model* m, int kv_rows, int track, dz_ctx** out) {
   if (!m || !out) return set_error(DZ_ERR_MODEL, "null argument");
   if (kv_rows < 0 || kv_rows > m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "4-bit cache of %d rows (max_ctx %d)", kv_rows, m->cfg.max_ctx);
-  return ctx_create(m, kv_rows ? kv_rows : m->cfg.max_ctx, track != 0, out);
+  try {
+    return ctx_create(m, kv_rows ? kv_rows : m->cfg.max_ctx, track != 0, out);
+  } catch (...) {  // an allocation on the host
+    return set_error(DZ_ERR_MODEL, "out of memory");
+  }
 }
 
 int dz_ctx_free(dz_ctx* x) {
