@@ -432,7 +432,7 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
 #pragma unroll
   for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
   unsigned qoff = (unsigned)(rt * T * QP * 64) + lane;
-  auto tiles = [&](auto Odd) {
+  auto tiles = [&](auto Odd, auto Keep) {
     for (int p0 = p_first; p0 < wend; p0 += step) {
       constexpr bool odd = decltype(Odd)::value;
       const int pn = p0 + step < wend ? p0 + step : p0;  // past the last tile: not used
@@ -479,7 +479,7 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
         for (int j = 0; j < 8; ++j)
           if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
       }
-      if constexpr (RT == 1) {
+      if constexpr (decltype(Keep)::value) {
         // every position up to the last row's is in some wave's tile, so that the rows are written whole
         if (dst.scores && rho < rows) {
           float* y = dst.scores + ((size_t)(rho / grp) * nq + g * grp + rho % grp) * c.cap + p0 + 4 * lk;
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
     }
   };
   if (__ballot(flag != 0)) {
-    tiles(std::true_type{});
+    tiles(std::true_type{}, std::integral_constant<bool, RT == 1>{});
     // rows that see a value which is not a number
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -541,13 +541,16 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
       for (int t = 0; t < T; ++t)
         if (first[t] < ci) o[2 * t][i] = o[2 * t + 1][i] = __builtin_nanf("");
     }
+  } else if (RT == 1 && dst.scores) {
+    tiles(std::false_type{}, std::integral_constant<bool, RT == 1>{});
   } else {
-    tiles(std::false_type{});
+    tiles(std::false_type{}, std::false_type{});
   }
   if constexpr (RT == 1) {
     // the waves' results of the rows that there are, [wave][row][HD + 8] (the rows of a store in different banks), over
     // the queries, which every wave has read; then each row's largest maximum and the sums at it, four dims a thread
     constexpr int LD = HD + 8;
+    const int nr = min(16, rows - row0);
     float* ms = reinterpret_cast<float*>(smem);  // m [PS][16], l [PS][16]
     float* os = ms + 32 * PS;
     __syncthreads();
@@ -557,22 +560,22 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (4 * lk + i < rows)
+      if (4 * lk + i < nr)
 #pragma unroll
         for (int t = 0; t < T; ++t)
-          *reinterpret_cast<float2*>(os + (size_t)(w * rows + 4 * lk + i) * LD + 32 * t + 2 * ln) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
+          *reinterpret_cast<float2*>(os + (size_t)(w * nr + 4 * lk + i) * LD + 32 * t + 2 * ln) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
     __syncthreads();
-    for (int u = (int)tid; u < rows * (HD / 4); u += NT) {
-      const int r = u / (HD / 4), d = 4 * (u % (HD / 4));
+    for (int u = (int)tid; u < nr * (HD / 4); u += NT) {
+      const int q = u / (HD / 4), r = row0 + q, d = 4 * (u % (HD / 4));
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int k = 0; k < PS; ++k) M = fmaxf(M, ms[16 * k + r]);
+      for (int k = 0; k < PS; ++k) M = fmaxf(M, ms[16 * k + q]);
       f32x4 O{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < PS; ++k) {
-        const float e = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ms[16 * k + r] - M) * kLog2e);
-        L = __builtin_fmaf(ms[16 * PS + 16 * k + r], e, L);
-        O += *reinterpret_cast<const f32x4*>(os + (size_t)(k * rows + r) * LD + d) * e;
+        const float e = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ms[16 * k + q] - M) * kLog2e);
+        L = __builtin_fmaf(ms[16 * PS + 16 * k + q], e, L);
+        O += *reinterpret_cast<const f32x4*>(os + (size_t)(k * nr + q) * LD + d) * e;
       }
       const size_t row = (size_t)(r / grp) * nq + g * grp + r % grp;
       if (nch == 1) {
@@ -872,21 +875,22 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     }
 }
 
-// The form of the kernel that a call takes: row tiles of a workgroup (rt), and the waves of a row tile (ps).  One row tile
-// takes eight waves, or four while 256 workgroups of four have no more than a tile each: fewer results to join, 10.4
-// against 12.1 us at 4096 positions of 4 key/value heads, 16.5 against 14.8 at 16384.
+// The form of the kernel that a call takes: row tiles of a workgroup (rt), and the waves of a row tile (ps).  Four row tiles
+// read the cache once between them; up to 192 rows one tile a workgroup, each with its own pass over the cache but more
+// waves on the same chunk, is faster (24 heads on 4 behind 8192 positions: 48 rows 19.5 against 24.0 us, 192 rows
+// 35.8 against 41.0, 384 rows 64.2 against 59.0).  It takes eight waves, or four while 256 workgroups of four
+// have no more than a tile each: fewer results to join (one token: 10.4 against 12.1 us at 4096 positions, 16.5
+// against 14.8 at 16384).
 struct AttendForm {
   int rt, ps;
 };
 static AttendForm attend_form(int rows, int nkv, int len) {
-  if (rows > 32) return AttendForm{4, 2};
-  if (rows > 16) return AttendForm{2, 4};
-  return AttendForm{1, (int64_t)len * nkv <= 256 * 128 ? 4 : 8};
+  if (rows > 192) return AttendForm{4, 2};
+  return AttendForm{1, (int64_t)len * nkv * ((rows + 15) / 16) <= 256 * 128 ? 4 : 8};
 }
 template <class F>
 static int with_form(AttendForm form, F&& f) {
   if (form.rt == 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-  if (form.rt == 2) return f(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
   if (form.ps == 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
   return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
 }
@@ -927,7 +931,7 @@ int prepare_kv4_kernels() {
   if (dev < 64 && done[dev]) return DZ_OK;
   for (int hd : {64, 128, 256})
     for (int type : {DZ_F32, DZ_F16, DZ_BF16})
-      for (AttendForm form : {AttendForm{1, 4}, AttendForm{1, 8}, AttendForm{2, 4}, AttendForm{4, 2}}) {
+      for (AttendForm form : {AttendForm{1, 4}, AttendForm{1, 8}, AttendForm{4, 2}}) {
         const int rc = with_head_dim(hd, [&](auto D) {
           return with_type(type, [&](auto* e) {
             return with_form(form, [&](auto R, auto P) -> int {
@@ -962,7 +966,7 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       dst.gate = gate;
       dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
       // behind the records of the most chunks
-      dst.scores = weights && form.rt == 1 ? dst.rec + (most > 1 ? ((size_t)n * n_head * most * (2 + HD) + 3) / 4 * 4 : 0) : nullptr;
+      dst.scores = weights && rows <= 16 ? dst.rec + (most > 1 ? ((size_t)n * n_head * most * (2 + HD) + 3) / 4 * 4 : 0) : nullptr;
       const int rc = with_form(form, [&](auto R, auto P) -> int {
         constexpr int RT = decltype(R)::value, PS = decltype(P)::value;
         const unsigned wgs = (unsigned)((rows + 16 * RT - 1) / (16 * RT) * c.nkv * nch);
