@@ -375,9 +375,9 @@ __device__ __forceinline__ float sum_over_lk(float x) {
 }
 
 // Causal attention of the n·grp query rows of a key/value head on the matrix cores.  Scores as S^T = K · Q^T: the operand
-// of the keys is the dequantised block itself (a block of 32 dims is one 16x16x32 instruction), that of the queries comes from LDS;
-// lane (ln, lk) gets the scores of row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that order, its
-// part of the operand P of O += P · V.  Dequantising is exact, queries and probabilities are sums of bf16 operands
+// of the keys is the dequantised block itself (a block of 32 dims is one 16x16x32 instruction), that of the queries comes
+// from LDS; lane (ln, lk) gets the scores of row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that
+// order, its part of the operand P of O += P · V.  Dequantising is exact, queries and probabilities are sums of bf16 operands
 // (Parts), so products are those of f32 values and the sums f32.
 //
 // A workgroup has RT tiles of 16 rows and PS waves for each, which take the chunk's tiles of 32 positions in turn, each a
@@ -706,6 +706,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, 
 __global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __restrict__ scores, int cap, int len, int nq, int grp,
                                                               int rows, const float2* __restrict__ stats,
                                                               float* __restrict__ weights, int64_t ldw) {
+  const int before = len - rows / grp;
   const int g = blockIdx.y, r = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
   if (r >= len) return;
   f32x4 s[16];
@@ -724,9 +725,8 @@ __global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __res
       const float inv = 1.f / st[k].y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        // what a row does not see has the score -inf; it adds nothing though the row's sum be a NaN
         const float p = __builtin_amdgcn_exp2f((s[k][i] - st[k].x) * kLog2e) * inv;
-        a[i] += s[k][i] == -INFINITY ? 0.f : p;
+        a[i] += r + i <= before + k / grp ? p : 0.f;  // what a row does not see gets nothing though the row's sum be a NaN
       }
     }
 #pragma unroll

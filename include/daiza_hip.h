@@ -147,13 +147,15 @@ int dz_q1_0_dequant_rows(dz_mat* m, size_t r0, size_t n, float* out);
  * cache (KvCache, cache/kv_cache.rs:17-130; the reference has no such form).  A row's head is blocks of 32 values,
  * each a 4-bit float (a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6; nearest, ties to the even code) times a power of two per
  * block: the smallest one at which the block's largest value does not round past 6, within [2^-120, 2^125] (a value
- * past 6 * 2^125 is held as that).  A block with an infinity or a NaN reads back as NaN throughout.  Writing a row that was read back gives the same row.
+ * past 6 * 2^125 is held as that).  A block with an infinity or a NaN reads back as NaN throughout.  Writing a row that
+ * was read back gives the same row.
  *
  * The calls below take device pointers and are enqueued on `stream` (a hipStream_t, NULL = default) without a host
- * synchronisation; their lengths are the host's.  A cache belongs to the device that dz_device_init selected before
- * dz_kv4_create; arrays elsewhere are refused.  Its calls must be ordered by the caller (one stream, or events).
- * Every array is [row][head][head_dim] with `ld` elements from row to row (ld >= heads * head_dim); no
- * alignment beyond the element's own is needed.
+ * synchronisation.  Rows held are counted on the host, when a call is made: a captured call replays on the rows that it
+ * was captured for, and the cache and every array must outlive the last replay.  A cache belongs to the device that
+ * dz_device_init selected before dz_kv4_create; arrays elsewhere are refused.  Its calls must be ordered by the caller
+ * (one stream, or events).  Every array is [row][head][head_dim] with `ld` elements from row to row (ld >= heads *
+ * head_dim); no alignment beyond the element's own is needed.  Outputs overlap no input.
  */
 typedef struct dz_kv4 dz_kv4;
 
@@ -307,10 +309,11 @@ int dz_forward_batch(dz_ctx* c, const uint32_t* ids, int n, int start_pos,
                      float* last_logits_or_null, float* per_pos_logits_or_null);
 
 /*
- * dz_forward_batch with log probabilities in place of logits, formed on the device (dz_logprobs_dev), where up to 1024 rows of
- * logits stay (1 MB each at the 27B vocabulary): logp[i] of targets[i] under the logits after ids[i] (targets[i] outside the vocabulary, -1 for one:
- * NaN), entropy[i], and the `top` best alternatives top_ids[i][top], top_logp[i][top].  Host arrays; logp (with
- * targets), entropy and top_logp may be NULL, top may be 0.  A prompt's score is targets[i] = ids[i + 1].
+ * dz_forward_batch with log probabilities in place of logits, formed on the device (dz_logprobs_dev), where up to 1024
+ * rows of logits stay (1 MB each at the 27B vocabulary): logp[i] of targets[i] under the logits after ids[i] (NaN for
+ * targets[i] outside the vocabulary, -1 for one), entropy[i], and the `top` best alternatives top_ids[i][top],
+ * top_logp[i][top].  Host arrays; logp (with targets), entropy and top_logp may be NULL, top may be 0.  A prompt's score
+ * is targets[i] = ids[i + 1].
  */
 int dz_forward_logprobs(dz_ctx* c, const uint32_t* ids, const int32_t* targets, int n, int start_pos, int top, float* logp,
                         float* entropy, int32_t* top_ids, float* top_logp);

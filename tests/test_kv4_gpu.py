@@ -216,6 +216,20 @@ def test_query_with_nan(dz):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("n", [2, 40])
+def test_scores_past_f32(dz, n):
+    # every score of head 0 is -inf in f32: its softmax is 0 / 0 in what each query sees, and nothing elsewhere
+    k, v = torch.full((70, 1, 64), 2.0 ** 100), _rows(54, 70, 1, 64)
+    c = _cache(dz, k, v)
+    q = _normal(55, n, 2, 64)
+    q[:, 0] = -2.0 ** 100
+    q[:, 1] = 0
+    out, w = torch.empty(n, 2, 64, device="cuda"), torch.zeros(1, 75, device="cuda")
+    c.attend_dev(q.cuda(), out, weights=w)
+    assert bool(torch.isnan(out[:, 0]).all()) and bool(torch.isfinite(out[:, 1]).all())
+    assert bool(torch.isnan(w[0, :70]).all()) and bool((w[0, 70:] == 0).all())
+
+
 def test_same_results_every_time(dz):
     k, v = _rows(60, 3000, 4, 256), _rows(61, 3000, 4, 256)
     c = _cache(dz, k, v)
