@@ -9,8 +9,8 @@
 // of what is stored 99% instead of 98%.
 //
 // Layout, per key/value head and tile of 32 rows, T = head_dim/32 blocks (lane = 16·lk + ln of a wave):
-//   keys    row r at r·head_dim/2: dword (lk, b) at 4(lk·T + b) holds dims 32b + 8lk .. +7 in nibble order: the lane's part of
-//           the 16x16x32 matrix operand of block b, a lane's T dwords contiguous
+//   keys    row r at r·head_dim/2, its dims in nibble order.  Lane (ln, lk) takes the quarter lk of row ln's dims: its part of
+//           the matrix operands, dims in an order that the queries share
 //   values  the lane's slots j = 0..7 are rows 4lk + j (j < 4) and 16 + 4lk + j - 4, the rows whose probabilities the
 //           score product leaves in that lane; byte (j, t) of its 8·T bytes holds dims 32t + 2ln (low nibble) and
 //           32t + 2ln + 1; the bytes come in chunks of 16, chunk c of all lanes one after another

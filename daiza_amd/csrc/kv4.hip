@@ -7,6 +7,7 @@
 
 #include "elem.h"
 #include "kv4.h"
+#include "q1_digits.h"
 
 struct dz_kv4 {
   dz::Kv4View v;
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(kKv4RowThreads) void kv4_append_kernel(Kv4View c, i
     if (sb == 255) c.bad[(size_t)g * (c.cap / kKv4Tile) + r / kKv4Tile] = 1;
   }
   if (!values) {
-    uint8_t* p = c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 4 * (((a % 8) / 2) * T + b) + 2 * (a & 1);
+    uint8_t* p = c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 2 * a;
     *reinterpret_cast<unsigned short*>(p) = (unsigned short)code;
   } else {
     uint8_t* p = c.vc + g * c.code_head() + kv4_value_offset<HD>(r, 2 * (a % 8)) + b;
@@ -103,8 +104,7 @@ __global__ __launch_bounds__(kKv4RowThreads) void kv4_read_kernel(Kv4View c, int
     const uint8_t* p = c.vc + g * c.code_head() + kv4_value_offset<HD>(r, 2 * (a % 8)) + b;
     code = p[0] | (unsigned)p[16] << 8;
   } else {
-    code = *reinterpret_cast<const unsigned short*>(c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 4 * (((a % 8) / 2) * T + b) +
-                                                    2 * (a & 1));
+    code = *reinterpret_cast<const unsigned short*>(c.kc + g * c.code_head() + (size_t)r * (HD / 2) + 2 * a);
   }
   const float s = kv4_scale((values ? c.vs : c.ks)[g * c.scale_head() + (size_t)r * T + b]);
   struct __attribute__((packed, aligned(4))) Four {
@@ -206,9 +206,9 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 // A lane's words of a tile of 32 rows.
 template <int HD>
 struct KeyWords {
-  static constexpr int T = HD / 32;
-  unsigned code[2][T];           // rows 16h + ln: dims 32b + 8lk .. +7
-  unsigned scale[2][(T + 3) / 4];
+  static constexpr int T = HD / 32, G = T >= 4 ? T / 4 : 1;  // words; blocks that the lane has a part of (half of one at 64)
+  unsigned code[2][T];  // rows 16h + ln: dims lk·HD/4 + 8b .. +7
+  unsigned scale[2];    // their blocks' bytes
   __device__ __forceinline__ void load(const uint8_t* kc, const uint8_t* ks, int64_t row, int ln, int lk) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -216,29 +216,33 @@ struct KeyWords {
       const unsigned* p = reinterpret_cast<const unsigned*>(kc + (size_t)r * (HD / 2) + 4 * T * lk);
 #pragma unroll
       for (int b = 0; b < T; ++b) code[h][b] = p[b];
-      if constexpr (T >= 4) {
-        const unsigned* q = reinterpret_cast<const unsigned*>(ks + (size_t)r * T);
-#pragma unroll
-        for (int b = 0; b < T / 4; ++b) scale[h][b] = q[b];
-      } else {
-        scale[h][0] = *reinterpret_cast<const unsigned short*>(ks + (size_t)r * T);
-      }
+      const uint8_t* q = ks + (size_t)r * T + (T >= 4 ? lk * G : lk / 2);
+      scale[h] = G == 2 ? *reinterpret_cast<const unsigned short*>(q) : *q;
     }
   }
-  // The matrix operand of block b of rows 16h + ln.
+  // Part b of the rows 16h + ln as a bf16 operand: a lane's dims lk·HD/4 + 8b .. +7, for the 16x16x32 instruction.
   __device__ __forceinline__ u32x4 operand(int h, int b) const {
-    const float s = scale_of(scale[h][b / 4], b % 4);
+    const float s = scale_of(scale[h], b / 4);
     const unsigned w = code[h][b];
     return u32x4{fp4_pair<0>(w, s), fp4_pair<1>(w, s), fp4_pair<2>(w, s), fp4_pair<3>(w, s)};
   }
   // Bit r of the result: row 16h + r has a block that is not a number.
   __device__ __forceinline__ unsigned bad_rows(int h) const {
-    bool bad = false;
-#pragma unroll
-    for (int b = 0; b < T; ++b) bad |= ((scale[h][b / 4] >> (8 * (b % 4))) & 255u) == 255u;
-    return (unsigned)__ballot(bad) & 0xFFFFu;  // the four lanes of a row agree
+    const unsigned long long m = __ballot((scale[h] & 255u) == 255u || (G == 2 && scale[h] >> 8 == 255u));
+    const unsigned v = (unsigned)m | (unsigned)(m >> 32);
+    return (v | v >> 16) & 0xFFFFu;  // the four lanes of a row have a quarter each
   }
 };
+// f += K · Q^T of 16 rows of keys (a lane's words and scale bytes) and a digit of 16 queries, for part g of a lane's dims (32, or
+// 16 and zeros): the 4-bit values are the 16x16x128 instruction's operand as they stand, their bytes its block scales.
+template <int HD>
+__device__ __forceinline__ f32x4 digit_scores(const unsigned (&code)[HD / 32], unsigned scale, int g, const i32x8& q, int q_scale, f32x4 f) {
+  i32x8 k{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < (HD >= 128 ? 4 : 2); ++i) k[i] = (int)code[4 * g + i];
+  return g ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, f, 4, 2, 1, (int)scale, 0, q_scale)
+           : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, f, 4, 2, 0, (int)scale, 0, q_scale);
+}
 template <int HD>
 struct ValueWords {
   static constexpr int T = HD / 32;
@@ -296,8 +300,8 @@ struct ValueWords {
   }
 };
 
-// The query rows of a workgroup, row ρ = token · grp + head of the group, as operands in LDS: [row tile][block][part]
-// [lane][16 B], lane 16·lk + ln holding dims 32b + 8lk .. +7 of the tile's row ln.  Requested and stored apart, for
+// The query rows of a workgroup, row ρ = token · grp + head of the group, as operands in LDS: [row tile][b][part]
+// [lane][16 B], lane 16·lk + ln holding dims lk·HD/4 + 8b .. +7 of the tile's row ln.  Requested and stored apart, for
 // other loads to be on their way in between.
 template <int HD, class E, int TILES, int NT>
 struct QueryStage {
@@ -311,8 +315,8 @@ struct QueryStage {
       struct __attribute__((packed, aligned(sizeof(E)))) Raw {
         E e[8];
       };
-      const Raw r = *reinterpret_cast<const Raw*>(q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD + 32 * b +
-                                                  8 * (lane >> 4));
+      const Raw r = *reinterpret_cast<const Raw*>(q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD +
+                                                  (HD / 4) * (lane >> 4) + 8 * b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[i][j] = r.e[j];
     }
@@ -332,6 +336,65 @@ struct QueryStage {
     }
   }
 };
+
+// f32 query rows as digits (q1_digits.h: a block of 32 values to 2^-29 of its largest) for the 16x16x128 instruction, which runs
+// at four times the rate of the bf16 one: six digits take half the time of three bf16 parts, and the keys need no dequantising.
+// Of a row tile: [g][digit] the first 16 bytes of the lanes, then their last 8, then [g] their block scales.  Forming them
+// takes a wave about 650 instructions, ten times the bf16 parts': for calls of many rows.
+template <int HD>
+struct DigitTile {
+  static constexpr int G = KeyWords<HD>::G, kTail = G * kDigits * 1024, kScales = kTail + G * kDigits * 512, kBytes = kScales + G * 256;
+};
+template <int HD, int TILES, int NT>
+struct DigitStage {
+  using D = DigitTile<HD>;
+  static constexpr int G = D::G, W = HD >= 128 ? 32 : 16, N = (TILES * G * 64 + NT - 1) / NT;
+  float x[N][W];
+  __device__ __forceinline__ void load(const float* __restrict__ q, int64_t ldq, int head0, int grp, int row0, int rows, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int u = tid + i * NT, lane = u & 63, g = (u >> 6) % G, tile = (u >> 6) / G;
+      const int rho = min(row0 + 16 * tile + (lane & 15), rows - 1);  // a row past the last is the last one again: not used
+      struct __attribute__((packed, aligned(4))) Raw {
+        float e[W];
+      };
+      const Raw r = *reinterpret_cast<const Raw*>(q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD +
+                                                  (HD / 4) * (lane >> 4) + 32 * g);
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[i][j] = r.e[j];
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* to, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int u = tid + i * NT, lane = u & 63, g = (u >> 6) % G, tile = (u >> 6) / G;
+      if (N * NT != TILES * G * 64 && u >= TILES * G * 64) break;
+      float v[32];  // pack_digits' element 2i is its argument 8 (i & 3) + (i >> 2), 2i + 1 the fourth after it
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int c = 8 * (j & 3) + (j >> 2);
+        v[c] = 2 * j < W ? x[i][2 * j < W ? 2 * j : 0] : 0.f;
+        v[c + 4] = 2 * j < W ? x[i][2 * j < W ? 2 * j + 1 : 0] : 0.f;
+      }
+      u32x6 d[kDigits];
+      const unsigned e = pack_digits(v, d);
+      uint8_t* p = to + tile * D::kBytes;
+#pragma unroll
+      for (int k = 0; k < kDigits; ++k) {
+        *reinterpret_cast<u32x4*>(p + (g * kDigits + k) * 1024 + lane * 16) = u32x4{d[k][0], d[k][1], d[k][2], d[k][3]};
+        *reinterpret_cast<u32x2*>(p + D::kTail + (g * kDigits + k) * 512 + lane * 8) = u32x2{d[k][4], d[k][5]};
+      }
+      *reinterpret_cast<unsigned*>(p + D::kScales + g * 256 + lane * 4) = e;
+    }
+  }
+};
+// Digit k of part g of a lane's dims.
+template <int HD>
+__device__ __forceinline__ i32x8 digit_operand(const uint8_t* tile, int g, int k, int lane) {
+  const u32x4 a = *reinterpret_cast<const u32x4*>(tile + (g * kDigits + k) * 1024 + lane * 16);
+  const u32x2 b = *reinterpret_cast<const u32x2*>(tile + DigitTile<HD>::kTail + (g * kDigits + k) * 512 + lane * 8);
+  return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -384,11 +447,14 @@ __device__ __forceinline__ float sum_over_lk(float x) {
 // tile ahead with its loads; their results meet in LDS at the end.  Two waves a SIMD, so that one's dequantising (about 400
 // vector instructions a tile) runs beside the other's matrix instructions (96 of 16 cycles with f32 queries).
 // Grid: row tiles x key/value heads x chunks; 64 RT PS threads.
+template <class E, int RT>
+constexpr bool attend_digits() { return RT == 4 && std::is_same<E, float>::value; }
 template <int HD, class E, int RT, int PS>
 __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq,
                                                                      int n, float scale, int csz, int nch, AttendOut dst,
                                                                      E* __restrict__ out, int64_t ldo) {
   constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p, NT = 64 * RT * PS;
+  constexpr bool kDig = attend_digits<E, RT>();
   extern __shared__ __align__(16) uint8_t smem[];
   u32x4* qs = reinterpret_cast<u32x4*>(smem);
   const int grp = nq / c.nkv, rows = n * grp, ntile = (rows + 16 * RT - 1) / (16 * RT);
@@ -413,7 +479,7 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
   const int p_first = pbeg + 32 * turn;
   KeyWords<HD> kw;
   ValueWords<HD> vw;
-  QueryStage<HD, E, RT, NT> queries;
+  typename std::conditional<kDig, DigitStage<HD, RT, NT>, QueryStage<HD, E, RT, NT>>::type queries;
   queries.load(q, ldq, g * grp, grp, row0, rows, (int)tid);
   // whether a tile of the chunk may hold blocks that are not numbers: such chunks take a loop of their own
   unsigned flag = 0;
@@ -422,7 +488,8 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
     kw.load(kc, ks, p_first, ln, lk);
     vw.load(vc, vs, p_first, (int)lane);
   }
-  queries.store(qs, (int)tid);
+  if constexpr (kDig) queries.store(smem, (int)tid);
+  else queries.store(qs, (int)tid);
   __syncthreads();
   f32x4 o[2 * T];
 #pragma unroll
@@ -431,38 +498,54 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
   int first[T];  // first position seen whose value block t is not a number
 #pragma unroll
   for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
-  unsigned qoff = (unsigned)(rt * T * QP * 64) + lane;
+  unsigned qoff = kDig ? (unsigned)(rt * DigitTile<HD>::kBytes) : (unsigned)(rt * T * QP * 64) + lane;
   auto tiles = [&](auto Odd, auto Keep) {
     for (int p0 = p_first; p0 < wend; p0 += step) {
       constexpr bool odd = decltype(Odd)::value;
       const int pn = p0 + step < wend ? p0 + step : p0;  // past the last tile: not used
       // the queries are read from LDS anew for every tile: in registers they would cost the second wave its place
       asm volatile("" : "+v"(qoff));
-      // matrix instructions of block b among the next block's dequantising
       f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-      u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QP];
+      if constexpr (kDig) {
+        constexpr int G = DigitTile<HD>::G;
+        const uint8_t* qt = smem + qoff;
+        int qe[G];
 #pragma unroll
-      for (int k = 0; k < QP; ++k) qq[k] = qs[qoff + k * 64];
+        for (int g2 = 0; g2 < G; ++g2) qe[g2] = *reinterpret_cast<const int*>(qt + DigitTile<HD>::kScales + g2 * 256 + lane * 4);
 #pragma unroll
-      for (int b = 0; b < T; ++b) {
-        u32x4 n0 = k0, n1 = k1, qn[QP];
-        if (b + 1 < T) {
+        for (int k = kDigits - 1; k >= 0; --k)
 #pragma unroll
-          for (int k = 0; k < QP; ++k) qn[k] = qs[qoff + ((b + 1) * QP + k) * 64];
-          n0 = kw.operand(0, b + 1);
-          n1 = kw.operand(1, b + 1);
+          for (int g2 = 0; g2 < G; ++g2) {
+            const i32x8 d = digit_operand<HD>(qt, g2, k, (int)lane);
+            s[0] = digit_scores<HD>(kw.code[0], kw.scale[0], g2, d, qe[g2] - 5 * k, s[0]);
+            s[1] = digit_scores<HD>(kw.code[1], kw.scale[1], g2, d, qe[g2] - 5 * k, s[1]);
+          }
+      } else {
+        // matrix instructions of block b among the next block's dequantising
+        u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QP];
+#pragma unroll
+        for (int k = 0; k < QP; ++k) qq[k] = qs[qoff + k * 64];
+#pragma unroll
+        for (int b = 0; b < T; ++b) {
+          u32x4 n0 = k0, n1 = k1, qn[QP];
+          if (b + 1 < T) {
+#pragma unroll
+            for (int k = 0; k < QP; ++k) qn[k] = qs[qoff + ((b + 1) * QP + k) * 64];
+            n0 = kw.operand(0, b + 1);
+            n1 = kw.operand(1, b + 1);
+          }
+#pragma unroll
+          for (int k = 0; k < QP; ++k) {
+            s[0] = mfma(k0, qq[k], s[0]);
+            s[1] = mfma(k1, qq[k], s[1]);
+          }
+          interleave<2 * QP, 10>();
+          __builtin_amdgcn_sched_barrier(0);
+          k0 = n0;
+          k1 = n1;
+#pragma unroll
+          for (int k = 0; k < QP; ++k) qq[k] = qn[k];
         }
-#pragma unroll
-        for (int k = 0; k < QP; ++k) {
-          s[0] = mfma(k0, qq[k], s[0]);
-          s[1] = mfma(k1, qq[k], s[1]);
-        }
-        interleave<2 * QP, 10>();
-        __builtin_amdgcn_sched_barrier(0);
-        k0 = n0;
-        k1 = n1;
-#pragma unroll
-        for (int k = 0; k < QP; ++k) qq[k] = qn[k];
       }
       float x[8];
 #pragma unroll
@@ -734,15 +817,21 @@ __global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __res
     if (r + i < len) weights[(size_t)g * ldw + r + i] += a[i];
 }
 
-// The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile][block][part][lane].
+// Bytes of a row tile of the operands that the weights' pass takes ready.
+template <int HD, class E>
+constexpr int ready_bytes() { return std::is_same<E, float>::value ? DigitTile<HD>::kBytes : HD / 32 * Parts<E>::q * 1024; }
+
+// The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile].
 // Grid (row tiles, nkv), 256 threads.
 template <int HD, class E>
 __global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q, int64_t ldq, int nkv, int nq, int n,
-                                                        u32x4* __restrict__ split) {
+                                                        uint8_t* __restrict__ split) {
   const int g = blockIdx.y, grp = nq / nkv;
-  QueryStage<HD, E, 1, 256> queries;
+  uint8_t* to = split + ((size_t)g * gridDim.x + blockIdx.x) * ready_bytes<HD, E>();
+  typename std::conditional<std::is_same<E, float>::value, DigitStage<HD, 1, 256>, QueryStage<HD, E, 1, 256>>::type queries;
   queries.load(q, ldq, g * grp, grp, 16 * (int)blockIdx.x, n * grp, (int)threadIdx.x);
-  queries.store(split + ((size_t)g * gridDim.x + blockIdx.x) * (HD / 32 * Parts<E>::q * 64), (int)threadIdx.x);
+  if constexpr (std::is_same<E, float>::value) queries.store(to, (int)threadIdx.x);
+  else queries.store(reinterpret_cast<u32x4*>(to), (int)threadIdx.x);
 }
 
 // weights[g][r] += Σ over the group's query rows ρ of exp(s_ρr - m_ρ) / l_ρ: a wave holds the operands of 16·PT rows of keys and
@@ -757,14 +846,16 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
                                                              float scale, const u32x4* __restrict__ split,
                                                              const float2* __restrict__ stats, float* __restrict__ weights,
                                                              int64_t ldw) {
-  constexpr int T = HD / 32, QP = Parts<E>::q, TILE = T * QP * 64, N = (TILE + 255) / 256;
+  constexpr bool kDig = READY && std::is_same<E, float>::value;
+  constexpr int T = HD / 32, QP = Parts<E>::q, TILE = (READY ? ready_bytes<HD, E>() : T * QP * 1024) / 16, N = (TILE + 255) / 256;
   __shared__ u32x4 qs[(READY ? 2 : 1) * TILE];
   const int g = blockIdx.y, grp = nq / c.nkv, rows = n * grp, before = len - n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int ln = lane & 15, lk = lane >> 4;
   const int pblk = (int)blockIdx.x * 64 * PT, pw = pblk + 16 * PT * w;  // the workgroup's and the wave's first position
   const uint8_t *kc = c.kc + g * c.code_head(), *ks = c.ks + g * c.scale_head();
-  u32x4 kop[PT][T];
+  u32x4 kop[kDig ? 1 : PT][T];
+  unsigned kcode[kDig ? PT : 1][T], kscale[kDig ? PT : 1];
   unsigned nan[PT];
 #pragma unroll
   for (int u = 0; u < PT; u += (PT == 1 ? 1 : 2)) {
@@ -773,8 +864,16 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     const int r = pw + 16 * u, base = r < len ? r & ~31 : 0;
     kw.load(kc, ks, base, ln, lk);
     const int h0 = r < len ? (r >> 4) & 1 : 0;
+    if constexpr (kDig) {
 #pragma unroll
-    for (int b = 0; b < T; ++b) {
+      for (int h = 0; h < (PT == 1 ? 1 : 2); ++h) {
+        kscale[u + h] = PT == 1 && h0 ? kw.scale[1] : kw.scale[h];
+#pragma unroll
+        for (int b = 0; b < T; ++b) kcode[u + h][b] = PT == 1 && h0 ? kw.code[1][b] : kw.code[h][b];
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < (kDig ? 0 : T); ++b) {
       if constexpr (PT == 1) {
         kop[u][b] = h0 ? kw.operand(1, b) : kw.operand(0, b);
       } else {
@@ -835,14 +934,30 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     f32x4 s[PT];
 #pragma unroll
     for (int u = 0; u < PT; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (kDig) {
+      constexpr int G = DigitTile<HD>::G;
+      const uint8_t* qd = reinterpret_cast<const uint8_t*>(qt);
+      int qe[G];
 #pragma unroll
-    for (int b = 0; b < T; ++b)
+      for (int g2 = 0; g2 < G; ++g2) qe[g2] = *reinterpret_cast<const int*>(qd + DigitTile<HD>::kScales + g2 * 256 + lane * 4);
 #pragma unroll
-      for (int k = 0; k < QP; ++k) {
-        const u32x4 qq = qt[(b * QP + k) * 64 + lane];
+      for (int k = kDigits - 1; k >= 0; --k)
 #pragma unroll
-        for (int u = 0; u < PT; ++u) s[u] = mfma(kop[u][b], qq, s[u]);
-      }
+        for (int g2 = 0; g2 < G; ++g2) {
+          const i32x8 d = digit_operand<HD>(qd, g2, k, lane);
+#pragma unroll
+          for (int u = 0; u < PT; ++u) s[u] = digit_scores<HD>(kcode[u], kscale[u], g2, d, qe[g2] - 5 * k, s[u]);
+        }
+    } else {
+#pragma unroll
+      for (int b = 0; b < T; ++b)
+#pragma unroll
+        for (int k = 0; k < QP; ++k) {
+          const u32x4 qq = qt[(b * QP + k) * 64 + lane];
+#pragma unroll
+          for (int u = 0; u < PT; ++u) s[u] = mfma(kop[u][b], qq, s[u]);
+        }
+    }
     const float inv = 1.f / st.y;
     if (any_nan) {
 #pragma unroll
@@ -909,14 +1024,17 @@ size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   const size_t rec = nch > 1 ? (rows * nch * (size_t)(2 + c.hd) * sizeof(float) + 15) / 16 * 16 : 0;
   const int tiles = (n * (n_head / c.nkv) + 15) / 16;
   if (tiles == 1) return (rows * sizeof(float2) + 15) / 16 * 16 + rec + rows * (size_t)c.cap * sizeof(float);
-  const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * 16 * c.nkv * c.hd * 2 * Parts<float>::q : 0;  // over the records
+  // over the records; the f32 queries' are the largest
+  const size_t ready = c.hd == 256 ? DigitTile<256>::kBytes : DigitTile<128>::kBytes;
+  static_assert(ready_bytes<256, __half>() <= DigitTile<256>::kBytes && DigitTile<64>::kBytes <= DigitTile<128>::kBytes);
+  const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * c.nkv * ready : 0;
   return (rows * sizeof(float2) + 15) / 16 * 16 + std::max(rec, split);
 }
 
 // Dynamic LDS of a workgroup for a call of `rows` rows a key/value head.
 template <int HD, class E, int RT, int PS>
 constexpr size_t attend_lds(int rows) {
-  const size_t queries = (size_t)RT * (HD / 32) * Parts<E>::q * 1024;
+  const size_t queries = (size_t)RT * (attend_digits<E, RT>() ? DigitTile<HD>::kBytes : HD / 32 * Parts<E>::q * 1024);
   const size_t join = RT == 1 ? (size_t)PS * (128 + (rows < 16 ? rows : 16) * (HD + 8) * 4) : (size_t)(RT * PS / 2) * (HD / 32 * 2 * 1024 + 512);
   return queries > join ? queries : join;
 }
@@ -993,7 +1111,8 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
         const int row_tiles = (rows + 15) / 16;
         u32x4* split = row_tiles >= kKv4SplitTiles ? reinterpret_cast<u32x4*>(dst.rec) : nullptr;
         if (split) {
-          kv4_split_kernel<HD, E><<<dim3((unsigned)row_tiles, (unsigned)c.nkv), 256, 0, s>>>((const E*)q, ldq, c.nkv, n_head, n, split);
+          kv4_split_kernel<HD, E><<<dim3((unsigned)row_tiles, (unsigned)c.nkv), 256, 0, s>>>((const E*)q, ldq, c.nkv, n_head, n,
+                                                                                          reinterpret_cast<uint8_t*>(split));
           DZ_HIP_CHECK(hipGetLastError());
         }
         auto run = [&](auto P, auto R) {

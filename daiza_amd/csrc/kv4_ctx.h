@@ -88,10 +88,9 @@ __global__ __launch_bounds__(256) void kv4_prep_kernel(Src src, int nq, int nkv,
   }
   __syncthreads();
   if (tid < HD / 8) {
-    const int lk = (int)tid / T, b = (int)tid % T;
     unsigned w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (unsigned)code[0][32 * b + 8 * lk + i] << (4 * i);
+    for (int i = 0; i < 8; ++i) w |= (unsigned)code[0][8 * tid + i] << (4 * i);
     *reinterpret_cast<unsigned*>(c.kc + ch + (size_t)r * (HD / 2) + 4 * tid) = w;
   } else if (tid < HD / 8 + 16) {
     const int ln = (int)tid - HD / 8;
