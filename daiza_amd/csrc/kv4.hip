@@ -838,14 +838,16 @@ __global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q,
 // walks the query rows 16 at a time, in LDS for the workgroup's four waves, a lane adding up its four positions
 // of each 16 over the query rows ln, in order; the sixteen lanes of a position are summed at the end.
 // READY: the queries come as operands (kv4_split_kernel), the next tile's requested ahead and LDS in two halves, one
-// barrier a tile; else the workgroup forms them (few rows, where a launch more would cost more).
-// Bound by the matrix instructions (24 PT of 16 cycles with f32 queries) and the LDS reads beside them (24 KB a wave).
-// Grid (ceil(len / 64PT), nkv), 256 threads.
+// barrier a tile, and the row tiles may be spread over gridDim.z workgroups whose sums kv4_join_weights_kernel adds; else
+// the workgroup forms them (few rows, where a launch more would cost more).
+// Bound by the matrix instructions of a wave's tile (48 of 9.1 ns with f32 queries as digits and PT = 4), the exponentials and
+// LDS reads (19 KB) that follow them between two barriers: 2.06 us a tile of two workgroups on a compute unit.
+// Grid (ceil(len / 64PT), nkv, parts), 256 threads.
 template <int HD, class E, int PT, bool READY>
 __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq, int n,
                                                              float scale, const u32x4* __restrict__ split,
                                                              const float2* __restrict__ stats, float* __restrict__ weights,
-                                                             int64_t ldw) {
+                                                             int64_t ldw, float* __restrict__ parts) {
   constexpr bool kDig = READY && std::is_same<E, float>::value;
   constexpr int T = HD / 32, QP = Parts<E>::q, TILE = (READY ? ready_bytes<HD, E>() : T * QP * 1024) / 16, N = (TILE + 255) / 256;
   __shared__ u32x4 qs[(READY ? 2 : 1) * TILE];
@@ -897,7 +899,9 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[u][i] = 0.f;
   // from the tile of the first query row that sees the workgroup's first position
-  const int t0 = max(0, pblk - before) * grp / 16, tn = (rows + 15) / 16;
+  const int ts = max(0, pblk - before) * grp / 16, tn = (rows + 15) / 16;
+  const int z = READY ? (int)blockIdx.z : 0, nz = READY ? (int)gridDim.z : 1;
+  const int t0 = ts + (int)((int64_t)(tn - ts) * z / nz), te = ts + (int)((int64_t)(tn - ts) * (z + 1) / nz);
   u32x4 next[READY ? N : 1];
   float2 st_next = make_float2(0.f, 1.f);
   const u32x4* tiles = split + (size_t)g * tn * TILE;
@@ -911,8 +915,8 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
       for (int i = 0; i < N; ++i) next[i] = tiles[(size_t)t * TILE + (TILE % 256 ? min(tid + 256 * i, TILE - 1) : tid + 256 * i)];
     st_next = stat(t);
   };
-  if (t0 < tn) request(t0);
-  for (int t = t0; t < tn; ++t) {
+  if (t0 < te) request(t0);
+  for (int t = t0; t < te; ++t) {
     const u32x4* qt = qs;
     if constexpr (READY) {
       u32x4* to = qs + (t & 1) * TILE;
@@ -928,7 +932,7 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     }
     const float2 st = st_next;
     __syncthreads();
-    request(min(t + 1, tn - 1));
+    request(min(t + 1, te - 1));
     const int rho = 16 * t + ln;
     const int ctx = rho < rows ? before + rho / grp + 1 : 0;
     f32x4 s[PT];
@@ -986,8 +990,28 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
       a += __shfl_xor(a, 4);
       a += __shfl_xor(a, 8);
       const int r = pw + 16 * u + 4 * lk + i;
-      if (ln == 0 && r < len) weights[(size_t)g * ldw + r] += a;
+      if (ln != 0 || r >= len) continue;
+      if (READY && nz > 1) parts[((size_t)(g * gridDim.x + blockIdx.x) * nz + z) * (64 * PT) + (r - pblk)] = a;
+      else weights[(size_t)g * ldw + r] += a;
     }
+}
+
+// weights[g][r] += the sums of its nz parts [kv head][block of 64 PT positions][part][64 PT], in order.
+// Grid (ceil(len / 64PT), nkv), 64 PT threads.
+__global__ __launch_bounds__(256) void kv4_join_weights_kernel(const float* __restrict__ parts, int nz, int len,
+                                                               float* __restrict__ weights, int64_t ldw) {
+  const int g = blockIdx.y, n = (int)blockDim.x, r = (int)blockIdx.x * n + (int)threadIdx.x;
+  if (r >= len) return;
+  const float* p = parts + (size_t)(g * gridDim.x + blockIdx.x) * nz * n + threadIdx.x;
+  float a = 0.f;
+  for (int z = 0; z < nz; z += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[(size_t)min(z + i, nz - 1) * n];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a += z + i < nz ? v[i] : 0.f;
+  }
+  weights[(size_t)g * ldw + r] += a;
 }
 
 // The form of the kernel that a call takes: row tiles of a workgroup (rt), and the waves of a row tile (ps).  Four row tiles
@@ -1016,8 +1040,13 @@ static int attend_max_chunks(int n, int n_head, int nkv) {
   return std::max(1, std::min(kKv4MaxChunks, 256 / tiles));
 }
 
-// From this many tiles of 16 query rows on the weights' pass takes its queries as operands formed once.
-constexpr int kKv4SplitTiles = 4;
+// From this many tiles of 16 query rows on the weights' pass takes its queries as operands formed once (attention and pass of
+// 5 tiles 25.7 against 22.3 us behind 600 positions, 66.2 against 67.6 behind 32768; of 8 tiles 27.1 against 28.1, 87.7
+// against 93.5; of 12 28.9 against 35.4).
+constexpr int kKv4SplitTiles = 8;
+// It has 4 tiles of 16 positions a wave then, and its query rows over as many workgroups as make up this number (333 tokens,
+// the pass alone: 26 us behind 600 positions and 74 behind 7333; each with all the rows: 110 and 129).
+constexpr int kKv4WeightGroups = 512, kKv4WeightTiles = 4;
 
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   const size_t rows = (size_t)n * n_head, nch = (size_t)attend_max_chunks(n, n_head, c.nkv);
@@ -1027,7 +1056,7 @@ size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   // over the records; the f32 queries' are the largest
   const size_t ready = c.hd == 256 ? DigitTile<256>::kBytes : DigitTile<128>::kBytes;
   static_assert(ready_bytes<256, __half>() <= DigitTile<256>::kBytes && DigitTile<64>::kBytes <= DigitTile<128>::kBytes);
-  const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * c.nkv * ready : 0;
+  const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * c.nkv * ready + kKv4WeightGroups * 64 * kKv4WeightTiles * sizeof(float) : 0;
   return (rows * sizeof(float2) + 15) / 16 * 16 + std::max(rec, split);
 }
 
@@ -1106,27 +1135,34 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
             dst.scores, c.cap, len, n_head, n_head / c.nkv, rows, stats, weights, ldw);
         DZ_HIP_CHECK(hipGetLastError());
       } else if (weights) {
-        // as many rows of keys a wave as leave about a workgroup for each compute unit
-        const int64_t units = ((int64_t)len + 63) / 64 * c.nkv;
         const int row_tiles = (rows + 15) / 16;
         u32x4* split = row_tiles >= kKv4SplitTiles ? reinterpret_cast<u32x4*>(dst.rec) : nullptr;
+        auto run = [&](auto P, auto R, int parts_n, float* parts) {
+          constexpr int PT = decltype(P)::value;
+          kv4_weights_kernel<HD, E, PT, decltype(R)::value>
+              <<<dim3((unsigned)((len + 64 * PT - 1) / (64 * PT)), (unsigned)c.nkv, (unsigned)parts_n), 256, 0, s>>>(
+                  c, len, (const E*)q, ldq, n_head, n, scale, split, stats, weights, ldw, parts);
+        };
         if (split) {
+          constexpr int PT = kKv4WeightTiles;
           kv4_split_kernel<HD, E><<<dim3((unsigned)row_tiles, (unsigned)c.nkv), 256, 0, s>>>((const E*)q, ldq, c.nkv, n_head, n,
                                                                                           reinterpret_cast<uint8_t*>(split));
           DZ_HIP_CHECK(hipGetLastError());
+          const int blocks = (len + 64 * PT - 1) / (64 * PT);
+          const int nz = (int)std::max<int64_t>(1, std::min<int64_t>(row_tiles, kKv4WeightGroups / ((int64_t)blocks * c.nkv)));
+          float* parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(split) + (size_t)row_tiles * c.nkv * ready_bytes<HD, E>());
+          run(std::integral_constant<int, PT>{}, std::true_type{}, nz, parts);
+          if (nz > 1) {
+            DZ_HIP_CHECK(hipGetLastError());
+            kv4_join_weights_kernel<<<dim3((unsigned)blocks, (unsigned)c.nkv), 64 * PT, 0, s>>>(parts, nz, len, weights, ldw);
+          }
+        } else {
+          // as many rows of keys a wave as leave about a workgroup for each compute unit
+          const int64_t units = ((int64_t)len + 63) / 64 * c.nkv;
+          if (units >= 4 * 200) run(std::integral_constant<int, 4>{}, std::false_type{}, 1, nullptr);
+          else if (units >= 2 * 200) run(std::integral_constant<int, 2>{}, std::false_type{}, 1, nullptr);
+          else run(std::integral_constant<int, 1>{}, std::false_type{}, 1, nullptr);
         }
-        auto run = [&](auto P, auto R) {
-          constexpr int PT = decltype(P)::value;
-          kv4_weights_kernel<HD, E, PT, decltype(R)::value><<<dim3((unsigned)((len + 64 * PT - 1) / (64 * PT)), (unsigned)c.nkv), 256, 0, s>>>(
-              c, len, (const E*)q, ldq, n_head, n, scale, split, stats, weights, ldw);
-        };
-        auto with_rows = [&](auto P) {
-          if (split) run(P, std::true_type{});
-          else run(P, std::false_type{});
-        };
-        if (units >= 4 * 200) with_rows(std::integral_constant<int, 4>{});
-        else if (units >= 2 * 200) with_rows(std::integral_constant<int, 2>{});
-        else with_rows(std::integral_constant<int, 1>{});
         DZ_HIP_CHECK(hipGetLastError());
       }
       return DZ_OK;

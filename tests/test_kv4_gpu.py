@@ -147,6 +147,51 @@ def test_attend_types(dz, dtype):
     _check_attend(dz, 4, 2, 64, 100, 9, dtype, True)
 
 
+@pytest.mark.parametrize("nq,nkv,hd,length,n", [(24, 4, 256, 700, 60), (6, 1, 256, 250, 250), (8, 2, 128, 600, 77), (16, 1, 128, 41, 13),
+                                                (4, 2, 64, 260, 129), (12, 1, 64, 90, 33)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attend_many_rows(dz, nq, nkv, hd, length, n, dtype):
+    _check_attend(dz, nq, nkv, hd, length, n, dtype, True)
+
+
+@pytest.mark.parametrize("n", [1, 30, 70])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_attend_queries_of_uneven_size(dz, n, hd):
+    # one dim in every 32 a thousand times the others, whose keys are small: a query of many rows is held to 2^-29 of its
+    # block's largest (the bound below), a key's 4 bits take the rest
+    k, v = _rows(56, 150, 1, hd), _rows(57, 150, 1, hd)
+    k[:, :, 7::32] *= 1e-3
+    q = _normal(58, n, 4, hd)
+    q[:, :, 7::32] *= 1e3
+    c = _cache(dz, k, v)
+    out, w = torch.empty(n, 4, hd, device="cuda"), torch.zeros(1, 150, device="cuda")
+    c.attend_dev(q.cuda(), out, weights=w)
+    ks, vs = ref.stored(k), ref.stored(v)
+    want, ww, bound, wb = ref.attend(q, ks, vs)
+    big = q.double().abs().reshape(n, 4, -1, 32).amax(-1)  # [n][heads][blocks]
+    held = (big @ ks[0].abs().reshape(150, -1, 32).sum(-1).T).amax(-1) * 2.0 ** -29 / math.sqrt(hd)  # of a score, absolute
+    more = 2 * held[..., None] * vs.abs().amax()
+    assert bool(((out.cpu().double() - want).abs() <= bound + more + 2.0 ** -24 * want.abs()).all())
+    assert bool(((w.cpu().double() - ww).abs() <= wb + 4 * held.amax() * ww + 2.0 ** -24 * ww).all())
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_query_that_is_not_a_number_among_many(dz, value, hd):
+    k, v = _rows(50, 110, 1, hd), _rows(51, 110, 1, hd)
+    q = _normal(52, 90, 3, hd)
+    c = _cache(dz, k, v)
+    want, got = torch.empty(90, 3, hd, device="cuda"), torch.empty(90, 3, hd, device="cuda")
+    ww, gw = torch.zeros(1, 110, device="cuda"), torch.zeros(1, 110, device="cuda")
+    c.attend_dev(q.cuda(), want, weights=ww)
+    q[41, 1, hd - 3] = value
+    c.attend_dev(q.cuda(), got, weights=gw)
+    assert bool(torch.isnan(got[41, 1]).all())
+    got[41, 1] = want[41, 1]
+    assert torch.equal(got, want)
+    assert bool(torch.isnan(gw[0, :20 + 42]).all()) and torch.equal(gw[0, 20 + 42:], ww[0, 20 + 42:])
+
+
 @pytest.mark.parametrize("kscale", [1e-6, 30.0])
 def test_attend_flat_and_peaked(dz, kscale):
     """Scores all but equal, and scores whose largest takes all the weight."""
