@@ -48,6 +48,8 @@ constexpr int kv4_wg_rows() { return kKv4RowThreads / (HD / 4); }
 
 // Rows of keys (z = 0) or values (z = 1) of a head into the cache, a thread per four dims: the eight threads of a block
 // find its largest value; a thread's four codes are half a word of keys, or a byte of values for each of two lanes.
+// Bound by the rows read, at 4 x 256: 1024 rows 5.1 us (8.4 MB in, 1.1 MB out), 32768 rows 89 us (3.4 TB/s; the codes are
+// stores of one and two bytes); one row 2.9 us, a launch.
 // Grid (ceil(n / kv4_wg_rows), nkv, 2), 256 threads.
 template <int HD, class E>
 __global__ __launch_bounds__(kKv4RowThreads) void kv4_append_kernel(Kv4View c, int row0, int n, const E* __restrict__ k, int64_t ldk,
@@ -88,7 +90,8 @@ __device__ __forceinline__ float kv4_grid(unsigned code) {
   return code & 8u ? -a : a;
 }
 
-// The values of rows start .. start + n, f32 [kv head][n][HD], a thread per four dims.
+// The values of rows start .. start + n, f32 [kv head][n][HD], a thread per four dims.  Bound by the stores: 8192 rows of 4 x 256
+// 15.2 us (67 MB, 4.4 TB/s).
 // Grid (ceil(n / kv4_wg_rows), nkv, 2), 256 threads.
 template <int HD>
 __global__ __launch_bounds__(kKv4RowThreads) void kv4_read_kernel(Kv4View c, int start, int n, float* __restrict__ k,
@@ -437,23 +440,41 @@ __device__ __forceinline__ float sum_over_lk(float x) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// Causal attention of the n·grp query rows of a key/value head on the matrix cores.  Scores as S^T = K · Q^T: the operand
-// of the keys is the dequantised block itself (a block of 32 dims is one 16x16x32 instruction), that of the queries comes
-// from LDS; lane (ln, lk) gets the scores of row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that
-// order, its part of the operand P of O += P · V.  Dequantising is exact, queries and probabilities are sums of bf16 operands
-// (Parts), so products are those of f32 values and the sums f32.
+// Causal attention of the n·grp query rows of a key/value head on the matrix cores, in one pass with the running maximum m and
+// sum l of each row's softmax.  Scores as S^T = K · Q^T, the operand of the queries from LDS; lane (ln, lk) gets the scores of
+// row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that order, its part of the operand P of O += P · V.
+// Dequantising is exact, queries are sums of bf16 operands (Parts) or digits of the 4-bit instruction (attend_digits),
+// probabilities sums of bf16 operands: products are those of f32 values, and the sums f32.
 //
 // A workgroup has RT tiles of 16 rows and PS waves for each, which take the chunk's tiles of 32 positions in turn, each a
-// tile ahead with its loads; their results meet in LDS at the end.  Two waves a SIMD, so that one's dequantising (about 400
-// vector instructions a tile) runs beside the other's matrix instructions (96 of 16 cycles with f32 queries).
+// tile ahead with its loads; their results meet in LDS at the end.  Two waves a SIMD, so that one's dequantising runs beside
+// the other's matrix instructions.  At 24 heads on 4 x 256, f32:
+//   RT = 1 (up to 192 rows)  bound by latency to about 16384 positions (one token behind 4096: 7.8 us and the merge's 2.7)
+//                            and by the cache's bytes beyond (262144: 61 us, 4.7 TB/s, of 285 MB)
+//   RT = 4                   bound by the vector instructions (of which a wave dequantises its values with about 190 a tile, 32
+//                            positions) and the matrix instructions (24 of 9.1 ns for scores by six digits, 48 of 6.7 ns for
+//                            three parts of P) that do not run beside each other well enough: 0.67 and 0.54 us of the 1.6 us
+//                            of a tile.  333 tokens behind 7000 positions, 59 GFLOP, 175 us; with three bf16 parts for the
+//                            queries, 96 matrix instructions and the keys' dequantising beside them, 206 us.
+// Tiles with blocks that are not numbers, and calls that keep their scores, take loops of their own: in the common one
+// the bookkeeping cost 40 registers that it does not have.
 // Grid: row tiles x key/value heads x chunks; 64 RT PS threads.
 template <class E, int RT>
 constexpr bool attend_digits() { return RT == 4 && std::is_same<E, float>::value; }
+// Row tiles of a wave, and threads of a workgroup.  Two tiles share the values' dequantising, where registers hold two and the
+// other wave of the SIMD stays: 1024 tokens of 32 heads on 8 x 128 bf16 behind 8192 positions 290 us for 350, 333 tokens 121
+// for 190 (16-bit types).  f32 gains as much there but loses on short calls (300 tokens behind 3700 positions 52 us for 45);
+// at 256 dims two tiles leave one wave a SIMD, and 1024 f32 tokens took 745 us for 659.
+template <int HD, class E, int RT>
+constexpr int attend_wave_tiles() { return RT == 4 && HD <= 128 && sizeof(E) == 2 ? 2 : 1; }
 template <int HD, class E, int RT, int PS>
-__global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq,
+constexpr int attend_threads() { return 64 * RT / attend_wave_tiles<HD, E, RT>() * PS; }
+template <int HD, class E, int RT, int PS>
+__global__ __launch_bounds__((attend_threads<HD, E, RT, PS>()), 2) void kv4_attend_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq,
                                                                      int n, float scale, int csz, int nch, AttendOut dst,
                                                                      E* __restrict__ out, int64_t ldo) {
-  constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p, NT = 64 * RT * PS;
+  constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p, QT = attend_wave_tiles<HD, E, RT>(),
+                NT = attend_threads<HD, E, RT, PS>();
   constexpr bool kDig = attend_digits<E, RT>();
   extern __shared__ __align__(16) uint8_t smem[];
   u32x4* qs = reinterpret_cast<u32x4*>(smem);
@@ -461,17 +482,21 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
   const int pairs = c.nkv * nch, pair = (int)blockIdx.x % pairs;
   const int tile = ntile - 1 - (int)blockIdx.x / pairs, g = pair % c.nkv, z = pair / c.nkv;
   const unsigned tid = threadIdx.x, lane = tid & 63u;
-  const int w = __builtin_amdgcn_readfirstlane((int)(tid >> 6)), rt = w % RT, turn = w / RT;
+  const int w = __builtin_amdgcn_readfirstlane((int)(tid >> 6)), rt = w % (RT / QT) * QT, turn = w / (RT / QT);
   const int ln = (int)(lane & 15u), lk = (int)(lane >> 4);
   const int row0 = 16 * RT * tile, wrow = row0 + 16 * rt;
   const int before = len - n;
   // the positions that any row of the workgroup (of the wave) sees in the chunk
-  const int last_row = min(row0 + 16 * RT, rows) - 1, wlast = min(wrow + 16, rows) - 1;
+  const int last_row = min(row0 + 16 * RT, rows) - 1, wlast = min(wrow + 16 * QT, rows) - 1;
   const int pbeg = z * csz, pend = min(min((z + 1) * csz, len), before + last_row / grp + 1);
   const int wend = wrow < rows ? min(pend, before + wlast / grp + 1) : pbeg;
   const int wmin = wrow < rows ? before + wrow / grp + 1 : 0;  // what the wave's first row sees
-  const int rho = wrow + ln;
-  const int ctx = rho < rows ? before + rho / grp + 1 : 0;
+  int rho[QT], ctx[QT];
+#pragma unroll
+  for (int u = 0; u < QT; ++u) {
+    rho[u] = wrow + 16 * u + ln;
+    ctx[u] = rho[u] < rows ? before + rho[u] / grp + 1 : 0;
+  }
   const uint8_t *kc = c.kc + g * c.code_head(), *vc = c.vc + g * c.code_head();
   const uint8_t *ks = c.ks + g * c.scale_head(), *vs = c.vs + g * c.scale_head();
   const uint8_t* bad = c.bad + (size_t)g * (c.cap / kKv4Tile);
@@ -491,10 +516,15 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
   if constexpr (kDig) queries.store(smem, (int)tid);
   else queries.store(qs, (int)tid);
   __syncthreads();
-  f32x4 o[2 * T];
+  f32x4 o[QT][2 * T];
+  float m[QT], l[QT];
 #pragma unroll
-  for (int t = 0; t < 2 * T; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int u = 0; u < QT; ++u) {
+#pragma unroll
+    for (int t = 0; t < 2 * T; ++t) o[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+  }
   int first[T];  // first position seen whose value block t is not a number
 #pragma unroll
   for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
@@ -505,95 +535,117 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
       const int pn = p0 + step < wend ? p0 + step : p0;  // past the last tile: not used
       // the queries are read from LDS anew for every tile: in registers they would cost the second wave its place
       asm volatile("" : "+v"(qoff));
-      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      f32x4 s[QT][2];
+#pragma unroll
+      for (int u = 0; u < QT; ++u) s[u][0] = s[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
       if constexpr (kDig) {
         constexpr int G = DigitTile<HD>::G;
         const uint8_t* qt = smem + qoff;
-        int qe[G];
+        int qe[QT][G];
 #pragma unroll
-        for (int g2 = 0; g2 < G; ++g2) qe[g2] = *reinterpret_cast<const int*>(qt + DigitTile<HD>::kScales + g2 * 256 + lane * 4);
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int g2 = 0; g2 < G; ++g2)
+            qe[u][g2] = *reinterpret_cast<const int*>(qt + u * DigitTile<HD>::kBytes + DigitTile<HD>::kScales + g2 * 256 + lane * 4);
 #pragma unroll
         for (int k = kDigits - 1; k >= 0; --k)
 #pragma unroll
-          for (int g2 = 0; g2 < G; ++g2) {
-            const i32x8 d = digit_operand<HD>(qt, g2, k, (int)lane);
-            s[0] = digit_scores<HD>(kw.code[0], kw.scale[0], g2, d, qe[g2] - 5 * k, s[0]);
-            s[1] = digit_scores<HD>(kw.code[1], kw.scale[1], g2, d, qe[g2] - 5 * k, s[1]);
-          }
+          for (int g2 = 0; g2 < G; ++g2)
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+              const i32x8 d = digit_operand<HD>(qt + u * DigitTile<HD>::kBytes, g2, k, (int)lane);
+              s[u][0] = digit_scores<HD>(kw.code[0], kw.scale[0], g2, d, qe[u][g2] - 5 * k, s[u][0]);
+              s[u][1] = digit_scores<HD>(kw.code[1], kw.scale[1], g2, d, qe[u][g2] - 5 * k, s[u][1]);
+            }
       } else {
         // matrix instructions of block b among the next block's dequantising
-        u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QP];
+        u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QT][QP];
 #pragma unroll
-        for (int k = 0; k < QP; ++k) qq[k] = qs[qoff + k * 64];
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int k = 0; k < QP; ++k) qq[u][k] = qs[qoff + (u * T * QP + k) * 64];
 #pragma unroll
         for (int b = 0; b < T; ++b) {
-          u32x4 n0 = k0, n1 = k1, qn[QP];
+          u32x4 n0 = k0, n1 = k1, qn[QT][QP];
           if (b + 1 < T) {
 #pragma unroll
-            for (int k = 0; k < QP; ++k) qn[k] = qs[qoff + ((b + 1) * QP + k) * 64];
+            for (int u = 0; u < QT; ++u)
+#pragma unroll
+              for (int k = 0; k < QP; ++k) qn[u][k] = qs[qoff + ((u * T + b + 1) * QP + k) * 64];
             n0 = kw.operand(0, b + 1);
             n1 = kw.operand(1, b + 1);
           }
 #pragma unroll
-          for (int k = 0; k < QP; ++k) {
-            s[0] = mfma(k0, qq[k], s[0]);
-            s[1] = mfma(k1, qq[k], s[1]);
-          }
-          interleave<2 * QP, 10>();
+          for (int k = 0; k < QP; ++k)
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+              s[u][0] = mfma(k0, qq[u][k], s[u][0]);
+              s[u][1] = mfma(k1, qq[u][k], s[u][1]);
+            }
+          interleave<2 * QP * QT, 10>();
           __builtin_amdgcn_sched_barrier(0);
           k0 = n0;
           k1 = n1;
 #pragma unroll
-          for (int k = 0; k < QP; ++k) qq[k] = qn[k];
+          for (int u = 0; u < QT; ++u)
+#pragma unroll
+            for (int k = 0; k < QP; ++k) qq[u][k] = qn[u][k];
         }
       }
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * scale;
+      unsigned b0 = 0, b1 = 0;
       if constexpr (odd) {
-        const unsigned b0 = kw.bad_rows(0), b1 = kw.bad_rows(1);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (((j < 4 ? b0 : b1) >> (4 * lk + (j & 3))) & 1u) x[j] = __builtin_nanf("");
+        b0 = kw.bad_rows(0);
+        b1 = kw.bad_rows(1);
       }
       kw.load(kc, ks, pn, ln, lk);
-      if (p0 + 32 > wmin) {
+      u32x4 pp[QT][PP];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx) x[j] = -INFINITY;
-      }
-      if constexpr (decltype(Keep)::value) {
-        // every position up to the last row's is in some wave's tile, so that the rows are written whole
-        if (dst.scores && rho < rows) {
-          float* y = dst.scores + ((size_t)(rho / grp) * nq + g * grp + rho % grp) * c.cap + p0 + 4 * lk;
-          *reinterpret_cast<f32x4*>(y) = f32x4{x[0], x[1], x[2], x[3]};
-          *reinterpret_cast<f32x4*>(y + 16) = f32x4{x[4], x[5], x[6], x[7]};
+      for (int u = 0; u < QT; ++u) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s[u][j >> 2][j & 3] * scale;
+        if constexpr (odd) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (((j < 4 ? b0 : b1) >> (4 * lk + (j & 3))) & 1u) x[j] = __builtin_nanf("");
         }
-      }
-      const float bm = max_over_lk(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
-      const float mn = fmaxf(m, bm);
-      // a row that has seen nothing keeps m = -inf: its factor is 1 by definition, and its probabilities 0
-      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-      const float base = mn == -INFINITY ? 0.f : mn;
-      float p[8], ps = 0.f;
+        if (p0 + 32 > wmin) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
-        ps += p[j];
-      }
-      l = l * al + sum_over_lk(ps);
-      m = mn;
-      // the O rows of this lane are 4lk + i: their factors live in lanes 4lk + i
-      if (__ballot(al != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = __shfl(al, 4 * lk + i);
-#pragma unroll
-          for (int t = 0; t < 2 * T; ++t) o[t][i] *= a;
+          for (int j = 0; j < 8; ++j)
+            if (p0 + 16 * (j >> 2) + 4 * lk + (j & 3) >= ctx[u]) x[j] = -INFINITY;
         }
+        if constexpr (decltype(Keep)::value) {
+          // every position up to the last row's is in some wave's tile, so that the rows are written whole
+          if (dst.scores && rho[u] < rows) {
+            float* y = dst.scores + ((size_t)(rho[u] / grp) * nq + g * grp + rho[u] % grp) * c.cap + p0 + 4 * lk;
+            *reinterpret_cast<f32x4*>(y) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(y + 16) = f32x4{x[4], x[5], x[6], x[7]};
+          }
+        }
+        const float bm = max_over_lk(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))));
+        const float mn = fmaxf(m[u], bm);
+        // a row that has seen nothing keeps m = -inf: its factor is 1 by definition, and its probabilities 0
+        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[u] - mn) * kLog2e);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        float p[8], ps = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = __builtin_amdgcn_exp2f((x[j] - base) * kLog2e);
+          ps += p[j];
+        }
+        l[u] = l[u] * al + sum_over_lk(ps);
+        m[u] = mn;
+        // the O rows of this lane are 4lk + i: their factors live in lanes 4lk + i
+        if (__ballot(al != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = __shfl(al, 4 * lk + i);
+#pragma unroll
+            for (int t = 0; t < 2 * T; ++t) o[u][t][i] *= a;
+          }
+        }
+        split8<PP>(p, pp[u]);
       }
-      u32x4 pp[PP];
-      split8<PP>(p, pp);
       if constexpr (odd) vw.take_bad(p0, lk, first);
       u32x4 lo, hi;
       vw.operands(0, lo, hi);
@@ -602,11 +654,13 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
         u32x4 nlo = lo, nhi = hi;
         if (t + 1 < T) vw.operands(t + 1, nlo, nhi);
 #pragma unroll
-        for (int k = 0; k < PP; ++k) {
-          o[2 * t] = mfma(pp[k], lo, o[2 * t]);
-          o[2 * t + 1] = mfma(pp[k], hi, o[2 * t + 1]);
-        }
-        interleave<2 * PP, 24>();
+        for (int k = 0; k < PP; ++k)
+#pragma unroll
+          for (int u = 0; u < QT; ++u) {
+            o[u][2 * t] = mfma(pp[u][k], lo, o[u][2 * t]);
+            o[u][2 * t + 1] = mfma(pp[u][k], hi, o[u][2 * t + 1]);
+          }
+        interleave<2 * PP * QT, 24>();
         __builtin_amdgcn_sched_barrier(0);
         lo = nlo;
         hi = nhi;
@@ -618,12 +672,14 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
     tiles(std::true_type{}, std::integral_constant<bool, RT == 1>{});
     // rows that see a value which is not a number
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int ci = __shfl(ctx, 4 * lk + i);
+    for (int u = 0; u < QT; ++u)
 #pragma unroll
-      for (int t = 0; t < T; ++t)
-        if (first[t] < ci) o[2 * t][i] = o[2 * t + 1][i] = __builtin_nanf("");
-    }
+      for (int i = 0; i < 4; ++i) {
+        const int ci = __shfl(ctx[u], 4 * lk + i);
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+          if (first[t] < ci) o[u][2 * t][i] = o[u][2 * t + 1][i] = __builtin_nanf("");
+      }
   } else if (RT == 1 && dst.scores) {
     tiles(std::false_type{}, std::integral_constant<bool, RT == 1>{});
   } else {
@@ -638,15 +694,15 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
     float* os = ms + 32 * PS;
     __syncthreads();
     if (lk == 0) {
-      ms[16 * w + ln] = m;
-      ms[16 * PS + 16 * w + ln] = l;
+      ms[16 * w + ln] = m[0];
+      ms[16 * PS + 16 * w + ln] = l[0];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (4 * lk + i < nr)
 #pragma unroll
         for (int t = 0; t < T; ++t)
-          *reinterpret_cast<float2*>(os + (size_t)(w * nr + 4 * lk + i) * LD + 32 * t + 2 * ln) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
+          *reinterpret_cast<float2*>(os + (size_t)(w * nr + 4 * lk + i) * LD + 32 * t + 2 * ln) = make_float2(o[0][2 * t][i], o[0][2 * t + 1][i]);
     __syncthreads();
     for (int u = (int)tid; u < nr * (HD / 4); u += NT) {
       const int q = u / (HD / 4), r = row0 + q, d = 4 * (u % (HD / 4));
@@ -681,65 +737,74 @@ __global__ __launch_bounds__(64 * RT * PS, 2) void kv4_attend_kernel(Kv4View c, 
 #pragma unroll
   for (int half = PS / 2; half > 0; half /= 2) {
     __syncthreads();
-    const int slot = (turn - half) * RT + rt;
     if (turn >= half && turn < 2 * half) {
 #pragma unroll
-      for (int t = 0; t < 2 * T; ++t) os[(slot * 2 * T + t) * 64 + lane] = o[t];
-      mls[slot * 64 + lane] = make_float2(m, l);
+      for (int u = 0; u < QT; ++u) {
+        const int slot = (turn - half) * RT + rt + u;
+#pragma unroll
+        for (int t = 0; t < 2 * T; ++t) os[(slot * 2 * T + t) * 64 + lane] = o[u][t];
+        mls[slot * 64 + lane] = make_float2(m[u], l[u]);
+      }
     }
     __syncthreads();
     if (turn < half) {
-      const int from = turn * RT + rt;
-      const float2 ml = mls[from * 64 + lane];
-      const float M = fmaxf(m, ml.x);
-      const float ea = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - M) * kLog2e);
-      const float eb = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ml.x - M) * kLog2e);
-      l = l * ea + ml.y * eb;
-      m = M;
-      float fa[4], fb[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = __shfl(ea, 4 * lk + i);
-        fb[i] = __shfl(eb, 4 * lk + i);
-      }
+      for (int u = 0; u < QT; ++u) {
+        const int from = turn * RT + rt + u;
+        const float2 ml = mls[from * 64 + lane];
+        const float M = fmaxf(m[u], ml.x);
+        const float ea = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[u] - M) * kLog2e);
+        const float eb = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((ml.x - M) * kLog2e);
+        l[u] = l[u] * ea + ml.y * eb;
+        m[u] = M;
+        float fa[4], fb[4];
 #pragma unroll
-      for (int t = 0; t < 2 * T; ++t) {
-        const f32x4 v = os[(from * 2 * T + t) * 64 + lane];
+        for (int i = 0; i < 4; ++i) {
+          fa[i] = __shfl(ea, 4 * lk + i);
+          fb[i] = __shfl(eb, 4 * lk + i);
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[t][i] = o[t][i] * fa[i] + v[i] * fb[i];
+        for (int t = 0; t < 2 * T; ++t) {
+          const f32x4 v = os[(from * 2 * T + t) * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[u][t][i] = o[u][t][i] * fa[i] + v[i] * fb[i];
+        }
       }
     }
   }
   if (turn) return;
-  if (lk == 0 && rho < rows) {
-    const size_t row = (size_t)(rho / grp) * nq + g * grp + rho % grp;
-    if (nch > 1) *reinterpret_cast<float2*>(dst.rec + (row * nch + z) * (2 + HD)) = make_float2(m, l);
-    else if (dst.stats) dst.stats[row] = make_float2(m, l);
-  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = wrow + 4 * lk + i;
-    const float li = __shfl(l, 4 * lk + i);
-    if (r >= rows) continue;
-    if (nch == 1) {
+  for (int u = 0; u < QT; ++u) {
+    if (lk == 0 && rho[u] < rows) {
+      const size_t row = (size_t)(rho[u] / grp) * nq + g * grp + rho[u] % grp;
+      if (nch > 1) *reinterpret_cast<float2*>(dst.rec + (row * nch + z) * (2 + HD)) = make_float2(m[u], l[u]);
+      else if (dst.stats) dst.stats[row] = make_float2(m[u], l[u]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = wrow + 16 * u + 4 * lk + i;
+      const float li = __shfl(l[u], 4 * lk + i);
+      if (r >= rows) continue;
       const size_t row = (size_t)(r / grp) * nq + g * grp + r % grp;
-      E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + 2 * ln;
+      if (nch == 1) {
+        E* y = out + (size_t)(r / grp) * ldo + (size_t)(g * grp + r % grp) * HD + 2 * ln;
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        y[32 * t] = dst.value<E, HD>(o[2 * t][i], li, row, 32 * t + 2 * ln);
-        y[32 * t + 1] = dst.value<E, HD>(o[2 * t + 1][i], li, row, 32 * t + 2 * ln + 1);
+        for (int t = 0; t < T; ++t) {
+          y[32 * t] = dst.value<E, HD>(o[u][2 * t][i], li, row, 32 * t + 2 * ln);
+          y[32 * t + 1] = dst.value<E, HD>(o[u][2 * t + 1][i], li, row, 32 * t + 2 * ln + 1);
+        }
+      } else {
+        float* rr = dst.rec + (row * nch + z) * (2 + HD) + 2 + 2 * ln;
+#pragma unroll
+        for (int t = 0; t < T; ++t) *reinterpret_cast<float2*>(rr + 32 * t) = make_float2(o[u][2 * t][i], o[u][2 * t + 1][i]);
       }
-    } else {
-      float* rr = dst.rec + (((size_t)(r / grp) * nq + g * grp + r % grp) * nch + z) * (2 + HD) + 2 + 2 * ln;
-#pragma unroll
-      for (int t = 0; t < T; ++t) *reinterpret_cast<float2*>(rr + 32 * t) = make_float2(o[2 * t][i], o[2 * t + 1][i]);
     }
   }
 }
 
 // The chunks' records of a row (query blockIdx.x, head blockIdx.y) as 64 dims (blockIdx.z) of its output, and its
 // statistics: 256 threads, wave w for the w-th quarter of the chunks, N of its records requested at a time.  A chunk whose
-// positions the row does not see has l = 0, m = -inf and zeros.
+// positions the row does not see has l = 0, m = -inf and zeros.  Bound by latency: one token of 24 heads in 64 chunks 2.5 us.
 template <int HD, class E, int N>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(AttendOut src, int nch, int nq, E* __restrict__ out, int64_t ldo) {
   __shared__ float fac[kKv4MaxChunks], red[4][65], mx[4];
@@ -820,7 +885,7 @@ __global__ __launch_bounds__(256) void kv4_merge_few_kernel(AttendOut src, int n
 }
 
 // weights[g][r] += Σ exp(s_ρr - m_ρ) / l_ρ over the group's query rows ρ in order, from the scores that the attention left
-// (few rows): four positions a thread.  Grid (ceil(len / 1024), nkv), 256 threads.
+// (few rows): four positions a thread.  Bound by the launch: 32768 positions of 24 heads 5.1 us (3.1 MB).  Grid (ceil(len / 1024), nkv), 256 threads.
 __global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __restrict__ scores, int cap, int len, int nq, int grp,
                                                               int rows, const float2* __restrict__ stats,
                                                               float* __restrict__ weights, int64_t ldw) {
@@ -856,7 +921,8 @@ __global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __res
 template <int HD, class E>
 constexpr int ready_bytes() { return std::is_same<E, float>::value ? DigitTile<HD>::kBytes : HD / 32 * Parts<E>::q * 1024; }
 
-// The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile].
+// The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile].  500 tiles of f32
+// rows 9 us.
 // Grid (row tiles, nkv), 256 threads.
 template <int HD, class E>
 __global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q, int64_t ldq, int nkv, int nq, int n,
@@ -1068,11 +1134,23 @@ static int with_form(AttendForm form, F&& f) {
   if (form.ps == 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
   return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
 }
-// Chunks of positions that a call's row tiles are spread over, at most: as many workgroups as are resident at once.
-static int attend_max_chunks(int n, int n_head, int nkv) {
+// Chunks of positions that a call's row tiles are spread over: as many workgroups as are resident at once (one a compute unit, of
+// two waves a SIMD; two where a wave has two row tiles and each gets 512 positions, below which 16 tiles behind 4000
+// positions took 16.7 us for 13.4); or, where that leaves a good part of them idle in the last round, up to three chunks, if
+// each is long enough to be worth a merge (1024 tokens of 24 heads on 4 behind 8192 positions, 384 row tiles: 581 us in two
+// chunks, 659 in one).  len = 0: the most chunks that any length takes.
+constexpr int kKv4LongChunk = 2048;
+static int attend_chunks(int n, int n_head, int nkv, bool pairs, int len) {
   const int rows = n * (n_head / nkv), rt = attend_form(rows, nkv, 0).rt;
-  const int tiles = (rows + 16 * rt - 1) / (16 * rt) * nkv;
-  return std::max(1, std::min(kKv4MaxChunks, 256 / tiles));
+  const int64_t tiles = (int64_t)((rows + 16 * rt - 1) / (16 * rt)) * nkv;
+  const int resident = pairs && rt == 4 && (len == 0 || len * tiles >= 512 * 512) ? 512 : 256;
+  int best = (int)std::max<int64_t>(1, std::min<int64_t>(kKv4MaxChunks, resident / tiles));
+  if (tiles >= 4 * resident) return best;  // the last round is a small part of the work, the chunks' records would be large
+  if (len == 0) return std::max(best, 3);
+  auto rounds = [&](int k) { return (tiles * k + resident - 1) / resident; };
+  for (int k = best + 1; k <= 3 && len / k >= kKv4LongChunk; ++k)
+    if (10 * rounds(k) * best < 9 * rounds(best) * k) best = k;
+  return best;
 }
 
 // From this many tiles of 16 query rows on the weights' pass takes its queries as operands formed once (attention and pass of
@@ -1084,7 +1162,7 @@ constexpr int kKv4SplitTiles = 8;
 constexpr int kKv4WeightGroups = 512, kKv4WeightTiles = 4;
 
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
-  const size_t rows = (size_t)n * n_head, nch = (size_t)attend_max_chunks(n, n_head, c.nkv);
+  const size_t rows = (size_t)n * n_head, nch = (size_t)attend_chunks(n, n_head, c.nkv, c.hd <= 128, 0);
   const size_t rec = nch > 1 ? (rows * nch * (size_t)(2 + c.hd) * sizeof(float) + 15) / 16 * 16 : 0;
   const int tiles = (n * (n_head / c.nkv) + 15) / 16;
   if (tiles == 1) return (rows * sizeof(float2) + 15) / 16 * 16 + rec + rows * (size_t)c.cap * sizeof(float);
@@ -1136,8 +1214,9 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
   const int rows = n * (n_head / c.nkv);
   const AttendForm form = attend_form(rows, c.nkv, len);
   const int unit = 32 * form.ps;  // a tile for every wave
-  const int most = attend_max_chunks(n, n_head, c.nkv);
-  const int csz = ((len + most - 1) / most + unit - 1) / unit * unit, nch = (len + csz - 1) / csz;
+  const bool pairs = c.hd <= 128 && type != DZ_F32;
+  const int most = attend_chunks(n, n_head, c.nkv, pairs, len);
+  const int csz = ((len + most - 1) / most + unit - 1) / unit * unit, nch = (int)(((int64_t)len + csz - 1) / csz);
   return with_head_dim(c.hd, [&](auto D) {
     constexpr int HD = decltype(D)::value;
     return with_type(type, [&](auto* e) -> int {
@@ -1147,12 +1226,12 @@ int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, 
       dst.stats = weights ? stats : nullptr;
       dst.gate = gate;
       dst.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + ((size_t)n * n_head * sizeof(float2) + 15) / 16 * 16);
-      // behind the records of the most chunks
-      dst.scores = weights && rows <= 16 ? dst.rec + (most > 1 ? ((size_t)n * n_head * most * (2 + HD) + 3) / 4 * 4 : 0) : nullptr;
+      // behind the records
+      dst.scores = weights && rows <= 16 ? dst.rec + (nch > 1 ? ((size_t)n * n_head * nch * (2 + HD) + 3) / 4 * 4 : 0) : nullptr;
       const int rc = with_form(form, [&](auto R, auto P) -> int {
         constexpr int RT = decltype(R)::value, PS = decltype(P)::value;
         const unsigned wgs = (unsigned)((rows + 16 * RT - 1) / (16 * RT) * c.nkv * nch);
-        kv4_attend_kernel<HD, E, RT, PS><<<dim3(wgs), 64 * RT * PS, attend_lds<HD, E, RT, PS>(rows), s>>>(
+        kv4_attend_kernel<HD, E, RT, PS><<<dim3(wgs), attend_threads<HD, E, RT, PS>(), attend_lds<HD, E, RT, PS>(rows), s>>>(
             c, len, (const E*)q, ldq, n_head, n, scale, csz, nch, dst, (E*)out, ldo);
         DZ_HIP_CHECK(hipGetLastError());
         return DZ_OK;
@@ -1222,7 +1301,8 @@ constexpr int kKv4Held = 32;  // keys a thread of the selection holds
 // [old, old + recent), in ascending order.  Each wave has a span of the rows; the key of the take-th largest is
 // found 11, 11 and 10 bits at a time from the top, by a histogram of the keys that share the bits found so far; then every
 // wave counts and writes its span in order.  HELD: the keys stay in registers (old <= 32768), else they are read anew.
-// Bound by latency: one workgroup a head.  Grid (nkv), 1024 threads.
+// Bound by latency, one workgroup a head: 32768 rows 25.8 us, 1100 rows 9.3 us.  The rows whose key is that of 0 are counted
+// by the wave: where most rows are such, one bin took 35 us of atomics.  Grid (nkv), 1024 threads.
 template <bool HELD>
 __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restrict__ w, int64_t ldw, int old, int take, int recent,
                                                           int32_t* __restrict__ kept) {
@@ -1336,7 +1416,8 @@ __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restric
 }
 
 // Rows kept[g] of c -> the rows of dst, with their weights: a tile of 32 rows of dst per workgroup, its loads all under way
-// at once.  Grid (ceil(m / 32), nkv), 256 threads.
+// at once.  Bound by latency of two dependent loads: 8192 rows of 4 x 256 6.6 us (18 MB read and written, 2.7 TB/s).
+// Grid (ceil(m / 32), nkv), 256 threads.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_gather_kernel(Kv4View c, Kv4View dst, const int32_t* __restrict__ kept, int m,
                                                          const float* __restrict__ w, int64_t ldw, float* __restrict__ dw,

@@ -148,10 +148,16 @@ def test_attend_types(dz, dtype):
 
 
 @pytest.mark.parametrize("nq,nkv,hd,length,n", [(24, 4, 256, 700, 60), (6, 1, 256, 250, 250), (8, 2, 128, 600, 77), (16, 1, 128, 41, 13),
-                                                (4, 2, 64, 260, 129), (12, 1, 64, 90, 33)])
+                                                (4, 2, 64, 260, 129), (12, 1, 64, 90, 33), (2, 2, 64, 2400, 200), (16, 2, 128, 4200, 30)])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_attend_many_rows(dz, nq, nkv, hd, length, n, dtype):
     _check_attend(dz, nq, nkv, hd, length, n, dtype, True)
+
+
+def test_attend_in_chunks_to_fill_the_last_round(dz):
+    # 300 row tiles of 64 rows for 256 workgroups, 600 for 512, behind positions enough for chunks of their own
+    _check_attend(dz, 75, 75, 64, 4200, 193, "f32", False)
+    _check_attend(dz, 150, 150, 64, 4200, 193, "bf16", True)
 
 
 @pytest.mark.parametrize("n", [1, 30, 70])
