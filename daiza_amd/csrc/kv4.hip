@@ -449,12 +449,12 @@ __device__ __forceinline__ float sum_over_lk(float x) {
 // A workgroup has RT tiles of 16 rows and PS waves for each, which take the chunk's tiles of 32 positions in turn, each a
 // tile ahead with its loads; their results meet in LDS at the end.  Two waves a SIMD, so that one's dequantising runs beside
 // the other's matrix instructions.  At 24 heads on 4 x 256, f32:
-//   RT = 1 (up to 192 rows)  bound by latency to about 16384 positions (one token behind 4096: 7.8 us and the merge's 2.7)
-//                            and by the cache's bytes beyond (262144: 61 us, 4.7 TB/s, of 285 MB)
+//   RT = 1 (up to 192 rows)  bound by latency to about 16384 positions (one token behind 4096: 8.0 us and the merge's 2.7)
+//                            and by the cache's bytes beyond (262144: 62 us, 4.6 TB/s, of 285 MB)
 //   RT = 4                   bound by the vector instructions (of which a wave dequantises its values with about 190 a tile, 32
 //                            positions) and the matrix instructions (24 of 9.1 ns for scores by six digits, 48 of 6.7 ns for
 //                            three parts of P) that do not run beside each other well enough: 0.67 and 0.54 us of the 1.6 us
-//                            of a tile.  333 tokens behind 7000 positions, 59 GFLOP, 175 us; with three bf16 parts for the
+//                            of a tile.  333 tokens behind 7000 positions, 59 GFLOP, 169 us; with three bf16 parts for the
 //                            queries, 96 matrix instructions and the keys' dequantising beside them, 206 us.
 // Tiles with blocks that are not numbers, and calls that keep their scores, take loops of their own: in the common one
 // the bookkeeping cost 40 registers that it does not have.
@@ -1158,7 +1158,7 @@ static int attend_chunks(int n, int n_head, int nkv, bool pairs, int len) {
 // against 93.5; of 12 28.9 against 35.4).
 constexpr int kKv4SplitTiles = 8;
 // It has 4 tiles of 16 positions a wave then, and its query rows over as many workgroups as make up this number (333 tokens,
-// the pass alone: 26 us behind 600 positions and 74 behind 7333; each with all the rows: 110 and 129).
+// the pass alone: 26 us behind 600 positions and 72 behind 7333; each with all the rows: 110 and 129).
 constexpr int kKv4WeightGroups = 512, kKv4WeightTiles = 4;
 
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
