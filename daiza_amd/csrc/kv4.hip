@@ -1295,13 +1295,18 @@ __device__ __forceinline__ unsigned weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// n plus the number of set bits of m below the lane's own.
+__device__ __forceinline__ unsigned lanes_below(unsigned long long m, unsigned n) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, n));
+}
+
 constexpr int kKv4Held = 32;  // keys a thread of the selection holds
 
 // kept[g] of head g: the `take` rows of [0, old) with the largest keys (the lower row first among equal ones), then the rows
 // [old, old + recent), in ascending order.  Each wave has a span of the rows; the key of the take-th largest is
 // found 11, 11 and 10 bits at a time from the top, by a histogram of the keys that share the bits found so far; then every
 // wave counts and writes its span in order.  HELD: the keys stay in registers (old <= 32768), else they are read anew.
-// Bound by latency, one workgroup a head: 32768 rows 25.8 us, 1100 rows 9.3 us.  The rows whose key is that of 0 are counted
+// Bound by latency, one workgroup a head: 32768 rows 24.6 us, 1100 rows 9.3 us.  The rows whose key is that of 0 are counted
 // by the wave: where most rows are such, one bin took 35 us of atomics.  Grid (nkv), 1024 threads.
 template <bool HELD>
 __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restrict__ w, int64_t ldw, int old, int take, int recent,
@@ -1347,21 +1352,20 @@ __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restric
     }
   };
   unsigned prefix = 0, left = (unsigned)take;  // the key's bits so far; how many rows come from the keys that share them
+  constexpr unsigned kZero = 0x80000000u;      // the key of 0
+  int zeros = 0;                               // how many the wave has
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, up = pass == 0 ? 32 : pass == 1 ? 21 : 10;
     hist[tid] = hist[1024 + tid] = 0;
     __syncthreads();
     // keys of 0 (rows never attended to, often many) are counted by the wave, not one after another in their bin
-    constexpr unsigned kZero = 0x80000000u;
-    const bool zeros_in = pass == 0 || (kZero >> (up & 31)) == (prefix >> (up & 31));
-    int zeros = 0;
     rows([&](int, unsigned k, bool has) {
-      if (zeros_in) zeros += __popcll(__ballot(has && k == kZero));
-      if (has && k != kZero && (pass == 0 || (k >> (up & 31)) == (prefix >> (up & 31))))
+      if (pass == 0) zeros += __popcll(__ballot(has && k == kZero));
+      if (has && (pass == 0 || (k >> (up & 31)) == (prefix >> (up & 31))) && k != kZero)
         atomicAdd(&hist[(k >> sh) & (pass == 2 ? 1023u : 2047u)], 1u);
     });
-    if (zeros && lane == 0) atomicAdd(&hist[(kZero >> sh) & (pass == 2 ? 1023u : 2047u)], (unsigned)zeros);
+    if (zeros && lane == 0 && (pass == 0 || (kZero >> (up & 31)) == (prefix >> (up & 31)))) atomicAdd(&hist[(kZero >> sh) & (pass == 2 ? 1023u : 2047u)], (unsigned)zeros);
     __syncthreads();
     // how many keys lie in the bins above a thread's two, from the top
     const unsigned hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid], own = hi + lo;
@@ -1407,11 +1411,15 @@ __global__ __launch_bounds__(1024) void kv4_select_kernel(const float* __restric
   }
   rows([&](int r, unsigned k, bool has) {
     const unsigned long long ba = __ballot(has && k > prefix), bt = __ballot(has && k == prefix);
-    const unsigned long long below = (1ull << lane) - 1;
-    const unsigned ra = above + (unsigned)__popcll(ba & below), rt = at + (unsigned)__popcll(bt & below);
-    if (has && (k > prefix || (k == prefix && rt < left))) kept[ra + min(rt, left)] = r;
+    const unsigned ra = lanes_below(ba, above);
+    if (bt) {
+      const unsigned rt = lanes_below(bt, at);
+      if (has && (k > prefix || (k == prefix && rt < left))) kept[ra + min(rt, left)] = r;
+      at += (unsigned)__popcll(bt);
+    } else if (has && k > prefix) {
+      kept[ra + min(at, left)] = r;
+    }
     above += (unsigned)__popcll(ba);
-    at += (unsigned)__popcll(bt);
   });
 }
 
@@ -1583,7 +1591,8 @@ int dz_kv4_read_dev(const dz_kv4* c, int start, int n, float* k, float* v, void*
 }
 
 size_t dz_kv4_attend_work_bytes(const dz_kv4* c, int n_head, int n) {
-  return !c || n_head < 1 || n < 1 || n_head % c->v.nkv ? 0 : kv4_attend_work(c->v, n_head, n);
+  if (!c || n_head < 1 || n < 1 || n_head % c->v.nkv || (int64_t)n * n_head > 1 << 30) return 0;  // refused calls
+  return kv4_attend_work(c->v, n_head, n);
 }
 
 int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
