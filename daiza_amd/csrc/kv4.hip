@@ -941,8 +941,9 @@ __global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q,
 // READY: the queries come as operands (kv4_split_kernel), the next tile's requested ahead and LDS in two halves, one
 // barrier a tile, and the row tiles may be spread over gridDim.z workgroups whose sums kv4_join_weights_kernel adds; else
 // the workgroup forms them (few rows, where a launch more would cost more).
-// Bound by the matrix instructions of a wave's tile (48 of 9.1 ns with f32 queries as digits and PT = 4), the exponentials and
-// LDS reads (19 KB) that follow them between two barriers: 2.06 us a tile of two workgroups on a compute unit.
+// Bound by the matrix instructions (48 of 9.1 ns a wave and tile with f32 queries as digits and PT = 4) and the vector ones
+// (about 350, 0.7 us), which add up to the 2.3 us that a tile of two waves a SIMD takes; a tile's exponentials among the next
+// one's matrix instructions measured the same.
 // Grid (ceil(len / 64PT), nkv, parts), 256 threads.
 template <int HD, class E, int PT, bool READY>
 __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len, const E* __restrict__ q, int64_t ldq, int nq, int n,

@@ -424,6 +424,35 @@ def test_captured_calls_replay(dz):
         assert all(torch.equal(a, b) for a, b in zip(got, (out, w, kept, dw, rk, rv))), i
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_captured_attention_of_many_rows(dz, dtype):
+    """Two captured calls of many query rows, replayed at once on two streams, against the eager calls."""
+    nq, nkv, hd, n, length = 8, 2, 128, 80, 900
+    c = _cache(dz, _rows(210, length, nkv, hd), _rows(211, length, nkv, hd))
+    q = [torch.zeros(n, nq, hd, dtype=TYPES[dtype], device="cuda") for _ in range(2)]
+    out, w = [torch.empty_like(x) for x in q], [torch.zeros(nkv, length, device="cuda") for _ in range(2)]
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i in range(2):
+        c.attend_dev(q[i], out[i], weights=w[i])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[i]):
+            c.attend_dev(q[i], out[i], weights=w[i])
+    for r in range(3):
+        for i in range(2):
+            q[i].copy_(_normal(330 + 2 * r + i, n, nq, hd))
+            w[i].zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            want, ww = torch.empty_like(q[i]), torch.zeros_like(w[i])
+            c.attend_dev(q[i], want, weights=ww)
+            torch.cuda.synchronize()
+            assert torch.equal(out[i], want) and torch.equal(w[i], ww), (r, i)
+
+
 def test_on_another_stream(dz):
     """Calls given a stream explicitly run there, in order, and their work memory outlives the call."""
     k, v = _rows(400, 500, 4, 256).cuda(), _rows(401, 500, 4, 256).cuda()
