@@ -732,11 +732,14 @@ def _current_stream(t):
 
 
 def _work(t, n_bytes, stream):
-    """Device memory for one call, from torch's allocator: it goes back when the call has run on its stream."""
-    w = _torch.empty(max(16, n_bytes), dtype=_torch.uint8, device=t.device)
-    if stream != _current_stream(t):
-        w.record_stream(_torch.cuda.ExternalStream(stream, device=t.device))
-    return w
+    """Device memory for one call, from torch's allocator and of the call's own stream: work queued earlier on another stream may
+    still use a block that its owner has freed there, and on this stream the block goes back when the call has run."""
+    n = max(16, n_bytes)
+    if stream == _current_stream(t):
+        return _torch.empty(n, dtype=_torch.uint8, device=t.device)
+    cuda = _torch.cuda
+    with cuda.stream(cuda.ExternalStream(stream, device=t.device) if stream else cuda.default_stream(t.device)):
+        return _torch.empty(n, dtype=_torch.uint8, device=t.device)
 
 
 class Kv4Cache:

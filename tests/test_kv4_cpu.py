@@ -1,6 +1,8 @@
 """CPU checks of the 4-bit cache and the log probabilities: refusals that need no device, and the reference form itself."""
+import contextlib
 import ctypes
 import math
+import types
 
 import pytest
 import torch
@@ -61,3 +63,43 @@ def test_reference_of_stored_values():
     x[0, 0, 3] = math.inf
     got = ref.stored(x)[0, 0]
     assert bool(torch.isnan(got[:32]).all()) and bool(torch.isfinite(got[32:]).all())
+
+
+class _Torch:
+    """What _work uses of torch, keeping account of the stream that each block is allocated on."""
+    uint8 = "uint8"
+
+    def __init__(self, current):
+        self.current, self.blocks, self.cuda = current, [], self
+
+    def empty(self, n, dtype, device):
+        self.blocks.append((n, self.current))
+        return self
+
+    def record_stream(self, stream):  # says when a block is free again, nothing of when it was
+        pass
+
+    class ExternalStream(int):
+        def __new__(cls, handle, device=None):
+            assert handle, "torch takes 0 for a stream of its pool"
+            return int.__new__(cls, handle)
+
+    def default_stream(self, device):
+        return 0
+
+    @contextlib.contextmanager
+    def stream(self, s):
+        before, self.current = self.current, int(s)
+        yield
+        self.current = before
+
+
+@pytest.mark.parametrize("current", [0, 0x1000])
+@pytest.mark.parametrize("stream", [0, 0x1000, 0x2000])
+def test_work_memory_is_allocated_on_the_calls_stream(monkeypatch, current, stream):
+    """A block of the current stream's may still be in use there when the call runs on its own stream."""
+    fake = _Torch(current)
+    monkeypatch.setattr(dz, "_torch", fake)
+    monkeypatch.setattr(dz, "_current_stream", lambda t: fake.current)
+    dz._work(types.SimpleNamespace(device="cuda:0"), 100, stream)
+    assert fake.blocks == [(100, stream)] and fake.current == current

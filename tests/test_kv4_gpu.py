@@ -474,6 +474,38 @@ def test_on_another_stream(dz):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("handle", [False, True])
+def test_work_memory_while_the_current_stream_is_busy(dz, handle):
+    """A call on a stream of its own takes no block that queued work of the current stream still uses, though its tensor is gone."""
+    k, v = _rows(410, 900, 4, 256), _rows(411, 900, 4, 256)
+    c = _cache(dz, k, v)
+    q = _normal(412, 2, 24, 256).cuda()
+    x, tokens = (_normal(413, 4, 30000) * 3).cuda(), torch.tensor([1, 2, 3, 4], dtype=torch.int32, device="cuda")
+    want, lwant = torch.empty_like(q), torch.empty(4, device="cuda")
+    c.attend_dev(q, want)
+    dz.logprobs_dev(x, tokens, lwant)
+    got, lgot = torch.zeros_like(q), torch.zeros(4, device="cuda")
+    sizes = (dz.lib().dz_kv4_attend_work_bytes(c._h, 24, 2), dz.lib().dz_logprobs_work_bytes(4, 30000, 0))
+    s, big = torch.cuda.Stream(), torch.ones(1 << 27, device="cuda")
+    for _ in range(3):
+        got.zero_()
+        lgot.zero_()
+        torch.cuda.synchronize()
+        for _ in range(40):  # some milliseconds
+            big.mul_(1.0)
+        kept = []
+        for n in sizes:
+            tmp = torch.full((n,), 7, dtype=torch.uint8, device="cuda")
+            kept.append(tmp.clone())
+            del tmp
+        on = s.cuda_stream if handle else s
+        c.attend_dev(q, got, stream=on)
+        dz.logprobs_dev(x, tokens, lgot, stream=on)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(lgot, lwant)
+        assert all(bool((t == 7).all()) for t in kept)
+
+
 def test_two_caches_at_once(dz):
     """Two caches on two streams do not touch each other's work."""
     q = _normal(500, 2, 24, 256).cuda()
