@@ -7,7 +7,6 @@
 
 #include "elem.h"
 #include "kv4.h"
-#include "q1_digits.h"
 
 struct dz_kv4 {
   dz::Kv4View v;
@@ -236,16 +235,6 @@ struct KeyWords {
     return (v | v >> 16) & 0xFFFFu;  // the four lanes of a row have a quarter each
   }
 };
-// f += K · Q^T of 16 rows of keys (a lane's words and scale bytes) and a digit of 16 queries, for part g of a lane's dims (32, or
-// 16 and zeros): the 4-bit values are the 16x16x128 instruction's operand as they stand, their bytes its block scales.
-template <int HD>
-__device__ __forceinline__ f32x4 digit_scores(const unsigned (&code)[HD / 32], unsigned scale, int g, const i32x8& q, int q_scale, f32x4 f) {
-  i32x8 k{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < (HD >= 128 ? 4 : 2); ++i) k[i] = (int)code[4 * g + i];
-  return g ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, f, 4, 2, 1, (int)scale, 0, q_scale)
-           : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, f, 4, 2, 0, (int)scale, 0, q_scale);
-}
 template <int HD>
 struct ValueWords {
   static constexpr int T = HD / 32;
@@ -340,65 +329,6 @@ struct QueryStage {
   }
 };
 
-// f32 query rows as digits (q1_digits.h: a block of 32 values to 2^-29 of its largest) for the 16x16x128 instruction, which runs
-// at four times the rate of the bf16 one: six digits take half the time of three bf16 parts, and the keys need no dequantising.
-// Of a row tile: [g][digit] the first 16 bytes of the lanes, then their last 8, then [g] their block scales.  Forming them
-// takes a wave about 650 instructions, ten times the bf16 parts': for calls of many rows.
-template <int HD>
-struct DigitTile {
-  static constexpr int G = KeyWords<HD>::G, kTail = G * kDigits * 1024, kScales = kTail + G * kDigits * 512, kBytes = kScales + G * 256;
-};
-template <int HD, int TILES, int NT>
-struct DigitStage {
-  using D = DigitTile<HD>;
-  static constexpr int G = D::G, W = HD >= 128 ? 32 : 16, N = (TILES * G * 64 + NT - 1) / NT;
-  float x[N][W];
-  __device__ __forceinline__ void load(const float* __restrict__ q, int64_t ldq, int head0, int grp, int row0, int rows, int tid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int u = tid + i * NT, lane = u & 63, g = (u >> 6) % G, tile = (u >> 6) / G;
-      const int rho = min(row0 + 16 * tile + (lane & 15), rows - 1);  // a row past the last is the last one again: not used
-      struct __attribute__((packed, aligned(4))) Raw {
-        float e[W];
-      };
-      const Raw r = *reinterpret_cast<const Raw*>(q + (size_t)(rho / grp) * ldq + (size_t)(head0 + rho % grp) * HD +
-                                                  (HD / 4) * (lane >> 4) + 32 * g);
-#pragma unroll
-      for (int j = 0; j < W; ++j) x[i][j] = r.e[j];
-    }
-  }
-  __device__ __forceinline__ void store(uint8_t* to, int tid) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int u = tid + i * NT, lane = u & 63, g = (u >> 6) % G, tile = (u >> 6) / G;
-      if (N * NT != TILES * G * 64 && u >= TILES * G * 64) break;
-      float v[32];  // pack_digits' element 2i is its argument 8 (i & 3) + (i >> 2), 2i + 1 the fourth after it
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int c = 8 * (j & 3) + (j >> 2);
-        v[c] = 2 * j < W ? x[i][2 * j < W ? 2 * j : 0] : 0.f;
-        v[c + 4] = 2 * j < W ? x[i][2 * j < W ? 2 * j + 1 : 0] : 0.f;
-      }
-      u32x6 d[kDigits];
-      const unsigned e = pack_digits(v, d);
-      uint8_t* p = to + tile * D::kBytes;
-#pragma unroll
-      for (int k = 0; k < kDigits; ++k) {
-        *reinterpret_cast<u32x4*>(p + (g * kDigits + k) * 1024 + lane * 16) = u32x4{d[k][0], d[k][1], d[k][2], d[k][3]};
-        *reinterpret_cast<u32x2*>(p + D::kTail + (g * kDigits + k) * 512 + lane * 8) = u32x2{d[k][4], d[k][5]};
-      }
-      *reinterpret_cast<unsigned*>(p + D::kScales + g * 256 + lane * 4) = e;
-    }
-  }
-};
-// Digit k of part g of a lane's dims.
-template <int HD>
-__device__ __forceinline__ i32x8 digit_operand(const uint8_t* tile, int g, int k, int lane) {
-  const u32x4 a = *reinterpret_cast<const u32x4*>(tile + (g * kDigits + k) * 1024 + lane * 16);
-  const u32x2 b = *reinterpret_cast<const u32x2*>(tile + DigitTile<HD>::kTail + (g * kDigits + k) * 512 + lane * 8);
-  return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], 0, 0};
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Where a call's results go: the output itself (nch = 1) or a record (m, l, o[HD]) per row and chunk of positions.
@@ -443,8 +373,8 @@ __device__ __forceinline__ float sum_over_lk(float x) {
 // Causal attention of the n·grp query rows of a key/value head on the matrix cores, in one pass with the running maximum m and
 // sum l of each row's softmax.  Scores as S^T = K · Q^T, the operand of the queries from LDS; lane (ln, lk) gets the scores of
 // row ln at positions 4lk + i and 16 + 4lk + i of the tile, which are, in that order, its part of the operand P of O += P · V.
-// Dequantising is exact, queries are sums of bf16 operands (Parts) or digits of the 4-bit instruction (attend_digits),
-// probabilities sums of bf16 operands: products are those of f32 values, and the sums f32.
+// Dequantising is exact, queries and probabilities are sums of bf16 operands (Parts): products are those of f32 values, and
+// the sums f32.
 //
 // A workgroup has RT tiles of 16 rows and PS waves for each, which take the chunk's tiles of 32 positions in turn, each a
 // tile ahead with its loads; their results meet in LDS at the end.  Two waves a SIMD, so that one's dequantising runs beside
@@ -452,15 +382,14 @@ __device__ __forceinline__ float sum_over_lk(float x) {
 //   RT = 1 (up to 192 rows)  bound by latency to about 16384 positions (one token behind 4096: 8.0 us and the merge's 2.7)
 //                            and by the cache's bytes beyond (262144: 62 us, 4.6 TB/s, of 285 MB)
 //   RT = 4                   bound by the vector instructions (of which a wave dequantises its values with about 190 a tile, 32
-//                            positions) and the matrix instructions (24 of 9.1 ns for scores by six digits, 48 of 6.7 ns for
-//                            three parts of P) that do not run beside each other well enough: 0.67 and 0.54 us of the 1.6 us
-//                            of a tile.  333 tokens behind 7000 positions, 59 GFLOP, 169 us; with three bf16 parts for the
-//                            queries, 96 matrix instructions and the keys' dequantising beside them, 206 us.
+//                            positions) and the matrix instructions (96 of 6.7 ns a tile: three parts of Q, three of P) that
+//                            do not run beside each other well enough: 1.7 us a tile.  333 tokens behind 7000 positions, 59
+//                            GFLOP, 186 us.  f32 queries as six 6-bit digits of the 16x16x128 instruction, which take the keys
+//                            as they stand, took 169 us, but hold a query to 2^-29 of the largest of each 32 dims: beside
+//                            an outlier that meets keys of 0 the other dims lose bits that an f32 product has.
 // Tiles with blocks that are not numbers, and calls that keep their scores, take loops of their own: in the common one
 // the bookkeeping cost 40 registers that it does not have.
 // Grid: row tiles x key/value heads x chunks; 64 RT PS threads.
-template <class E, int RT>
-constexpr bool attend_digits() { return RT == 4 && std::is_same<E, float>::value; }
 // Row tiles of a wave, and threads of a workgroup.  Two tiles share the values' dequantising, where registers hold two and the
 // other wave of the SIMD stays: 1024 tokens of 32 heads on 8 x 128 bf16 behind 8192 positions 290 us for 350, 333 tokens 121
 // for 190 (16-bit types).  f32 gains as much there but loses on short calls (300 tokens behind 3700 positions 52 us for 45);
@@ -475,7 +404,6 @@ __global__ __launch_bounds__((attend_threads<HD, E, RT, PS>()), 2) void kv4_atte
                                                                      E* __restrict__ out, int64_t ldo) {
   constexpr int T = HD / 32, QP = Parts<E>::q, PP = Parts<E>::p, QT = attend_wave_tiles<HD, E, RT>(),
                 NT = attend_threads<HD, E, RT, PS>();
-  constexpr bool kDig = attend_digits<E, RT>();
   extern __shared__ __align__(16) uint8_t smem[];
   u32x4* qs = reinterpret_cast<u32x4*>(smem);
   const int grp = nq / c.nkv, rows = n * grp, ntile = (rows + 16 * RT - 1) / (16 * RT);
@@ -504,7 +432,7 @@ __global__ __launch_bounds__((attend_threads<HD, E, RT, PS>()), 2) void kv4_atte
   const int p_first = pbeg + 32 * turn;
   KeyWords<HD> kw;
   ValueWords<HD> vw;
-  typename std::conditional<kDig, DigitStage<HD, RT, NT>, QueryStage<HD, E, RT, NT>>::type queries;
+  QueryStage<HD, E, RT, NT> queries;
   queries.load(q, ldq, g * grp, grp, row0, rows, (int)tid);
   // whether a tile of the chunk may hold blocks that are not numbers: such chunks take a loop of their own
   unsigned flag = 0;
@@ -513,8 +441,7 @@ __global__ __launch_bounds__((attend_threads<HD, E, RT, PS>()), 2) void kv4_atte
     kw.load(kc, ks, p_first, ln, lk);
     vw.load(vc, vs, p_first, (int)lane);
   }
-  if constexpr (kDig) queries.store(smem, (int)tid);
-  else queries.store(qs, (int)tid);
+  queries.store(qs, (int)tid);
   __syncthreads();
   f32x4 o[QT][2 * T];
   float m[QT], l[QT];
@@ -528,7 +455,7 @@ __global__ __launch_bounds__((attend_threads<HD, E, RT, PS>()), 2) void kv4_atte
   int first[T];  // first position seen whose value block t is not a number
 #pragma unroll
   for (int t = 0; t < T; ++t) first[t] = 0x7FFFFFFF;
-  unsigned qoff = kDig ? (unsigned)(rt * DigitTile<HD>::kBytes) : (unsigned)(rt * T * QP * 64) + lane;
+  unsigned qoff = (unsigned)(rt * T * QP * 64) + lane;
   auto tiles = [&](auto Odd, auto Keep) {
     for (int p0 = p_first; p0 < wend; p0 += step) {
       constexpr bool odd = decltype(Odd)::value;
@@ -538,59 +465,38 @@ __global__ __launch_bounds__((attend_threads<HD, E, RT, PS>()), 2) void kv4_atte
       f32x4 s[QT][2];
 #pragma unroll
       for (int u = 0; u < QT; ++u) s[u][0] = s[u][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (kDig) {
-        constexpr int G = DigitTile<HD>::G;
-        const uint8_t* qt = smem + qoff;
-        int qe[QT][G];
+      // matrix instructions of block b among the next block's dequantising
+      u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QT][QP];
 #pragma unroll
-        for (int u = 0; u < QT; ++u)
+      for (int u = 0; u < QT; ++u)
 #pragma unroll
-          for (int g2 = 0; g2 < G; ++g2)
-            qe[u][g2] = *reinterpret_cast<const int*>(qt + u * DigitTile<HD>::kBytes + DigitTile<HD>::kScales + g2 * 256 + lane * 4);
+        for (int k = 0; k < QP; ++k) qq[u][k] = qs[qoff + (u * T * QP + k) * 64];
 #pragma unroll
-        for (int k = kDigits - 1; k >= 0; --k)
-#pragma unroll
-          for (int g2 = 0; g2 < G; ++g2)
-#pragma unroll
-            for (int u = 0; u < QT; ++u) {
-              const i32x8 d = digit_operand<HD>(qt + u * DigitTile<HD>::kBytes, g2, k, (int)lane);
-              s[u][0] = digit_scores<HD>(kw.code[0], kw.scale[0], g2, d, qe[u][g2] - 5 * k, s[u][0]);
-              s[u][1] = digit_scores<HD>(kw.code[1], kw.scale[1], g2, d, qe[u][g2] - 5 * k, s[u][1]);
-            }
-      } else {
-        // matrix instructions of block b among the next block's dequantising
-        u32x4 k0 = kw.operand(0, 0), k1 = kw.operand(1, 0), qq[QT][QP];
-#pragma unroll
-        for (int u = 0; u < QT; ++u)
-#pragma unroll
-          for (int k = 0; k < QP; ++k) qq[u][k] = qs[qoff + (u * T * QP + k) * 64];
-#pragma unroll
-        for (int b = 0; b < T; ++b) {
-          u32x4 n0 = k0, n1 = k1, qn[QT][QP];
-          if (b + 1 < T) {
-#pragma unroll
-            for (int u = 0; u < QT; ++u)
-#pragma unroll
-              for (int k = 0; k < QP; ++k) qn[u][k] = qs[qoff + ((u * T + b + 1) * QP + k) * 64];
-            n0 = kw.operand(0, b + 1);
-            n1 = kw.operand(1, b + 1);
-          }
-#pragma unroll
-          for (int k = 0; k < QP; ++k)
-#pragma unroll
-            for (int u = 0; u < QT; ++u) {
-              s[u][0] = mfma(k0, qq[u][k], s[u][0]);
-              s[u][1] = mfma(k1, qq[u][k], s[u][1]);
-            }
-          interleave<2 * QP * QT, 10>();
-          __builtin_amdgcn_sched_barrier(0);
-          k0 = n0;
-          k1 = n1;
+      for (int b = 0; b < T; ++b) {
+        u32x4 n0 = k0, n1 = k1, qn[QT][QP];
+        if (b + 1 < T) {
 #pragma unroll
           for (int u = 0; u < QT; ++u)
 #pragma unroll
-            for (int k = 0; k < QP; ++k) qq[u][k] = qn[u][k];
+            for (int k = 0; k < QP; ++k) qn[u][k] = qs[qoff + ((u * T + b + 1) * QP + k) * 64];
+          n0 = kw.operand(0, b + 1);
+          n1 = kw.operand(1, b + 1);
         }
+#pragma unroll
+        for (int k = 0; k < QP; ++k)
+#pragma unroll
+          for (int u = 0; u < QT; ++u) {
+            s[u][0] = mfma(k0, qq[u][k], s[u][0]);
+            s[u][1] = mfma(k1, qq[u][k], s[u][1]);
+          }
+        interleave<2 * QP * QT, 10>();
+        __builtin_amdgcn_sched_barrier(0);
+        k0 = n0;
+        k1 = n1;
+#pragma unroll
+        for (int u = 0; u < QT; ++u)
+#pragma unroll
+          for (int k = 0; k < QP; ++k) qq[u][k] = qn[u][k];
       }
       unsigned b0 = 0, b1 = 0;
       if constexpr (odd) {
@@ -919,7 +825,7 @@ __global__ __launch_bounds__(256) void kv4_few_weights_kernel(const float* __res
 
 // Bytes of a row tile of the operands that the weights' pass takes ready.
 template <int HD, class E>
-constexpr int ready_bytes() { return std::is_same<E, float>::value ? DigitTile<HD>::kBytes : HD / 32 * Parts<E>::q * 1024; }
+constexpr int ready_bytes() { return HD / 32 * Parts<E>::q * 1024; }
 
 // The query rows of a key/value head as operands, a tile of 16 rows per workgroup: [kv head][row tile].  500 tiles of f32
 // rows 9 us.
@@ -929,10 +835,9 @@ __global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q,
                                                         uint8_t* __restrict__ split) {
   const int g = blockIdx.y, grp = nq / nkv;
   uint8_t* to = split + ((size_t)g * gridDim.x + blockIdx.x) * ready_bytes<HD, E>();
-  typename std::conditional<std::is_same<E, float>::value, DigitStage<HD, 1, 256>, QueryStage<HD, E, 1, 256>>::type queries;
+  QueryStage<HD, E, 1, 256> queries;
   queries.load(q, ldq, g * grp, grp, 16 * (int)blockIdx.x, n * grp, (int)threadIdx.x);
-  if constexpr (std::is_same<E, float>::value) queries.store(to, (int)threadIdx.x);
-  else queries.store(reinterpret_cast<u32x4*>(to), (int)threadIdx.x);
+  queries.store(reinterpret_cast<u32x4*>(to), (int)threadIdx.x);
 }
 
 // weights[g][r] += Σ over the group's query rows ρ of exp(s_ρr - m_ρ) / l_ρ: a wave holds the operands of 16·PT rows of keys and
@@ -941,8 +846,8 @@ __global__ __launch_bounds__(256) void kv4_split_kernel(const E* __restrict__ q,
 // READY: the queries come as operands (kv4_split_kernel), the next tile's requested ahead and LDS in two halves, one
 // barrier a tile, and the row tiles may be spread over gridDim.z workgroups whose sums kv4_join_weights_kernel adds; else
 // the workgroup forms them (few rows, where a launch more would cost more).
-// Bound by the matrix instructions (48 of 9.1 ns a wave and tile with f32 queries as digits and PT = 4) and the vector ones
-// (about 350, 0.7 us), which add up to the 2.3 us that a tile of two waves a SIMD takes; a tile's exponentials among the next
+// Bound by the matrix instructions (96 of 6.7 ns a wave and tile with f32 queries and PT = 4) and the vector ones (about
+// 350, 0.7 us), which add up to the 2.9 us that a tile of two waves a SIMD takes; a tile's exponentials among the next
 // one's matrix instructions measured the same.
 // Grid (ceil(len / 64PT), nkv, parts), 256 threads.
 template <int HD, class E, int PT, bool READY>
@@ -950,16 +855,14 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
                                                              float scale, const u32x4* __restrict__ split,
                                                              const float2* __restrict__ stats, float* __restrict__ weights,
                                                              int64_t ldw, float* __restrict__ parts) {
-  constexpr bool kDig = READY && std::is_same<E, float>::value;
-  constexpr int T = HD / 32, QP = Parts<E>::q, TILE = (READY ? ready_bytes<HD, E>() : T * QP * 1024) / 16, N = (TILE + 255) / 256;
+  constexpr int T = HD / 32, QP = Parts<E>::q, TILE = T * QP * 64, N = (TILE + 255) / 256;
   __shared__ u32x4 qs[(READY ? 2 : 1) * TILE];
   const int g = blockIdx.y, grp = nq / c.nkv, rows = n * grp, before = len - n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int ln = lane & 15, lk = lane >> 4;
   const int pblk = (int)blockIdx.x * 64 * PT, pw = pblk + 16 * PT * w;  // the workgroup's and the wave's first position
   const uint8_t *kc = c.kc + g * c.code_head(), *ks = c.ks + g * c.scale_head();
-  u32x4 kop[kDig ? 1 : PT][T];
-  unsigned kcode[kDig ? PT : 1][T], kscale[kDig ? PT : 1];
+  u32x4 kop[PT][T];
   unsigned nan[PT];
 #pragma unroll
   for (int u = 0; u < PT; u += (PT == 1 ? 1 : 2)) {
@@ -968,16 +871,8 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     const int r = pw + 16 * u, base = r < len ? r & ~31 : 0;
     kw.load(kc, ks, base, ln, lk);
     const int h0 = r < len ? (r >> 4) & 1 : 0;
-    if constexpr (kDig) {
 #pragma unroll
-      for (int h = 0; h < (PT == 1 ? 1 : 2); ++h) {
-        kscale[u + h] = PT == 1 && h0 ? kw.scale[1] : kw.scale[h];
-#pragma unroll
-        for (int b = 0; b < T; ++b) kcode[u + h][b] = PT == 1 && h0 ? kw.code[1][b] : kw.code[h][b];
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < (kDig ? 0 : T); ++b) {
+    for (int b = 0; b < T; ++b) {
       if constexpr (PT == 1) {
         kop[u][b] = h0 ? kw.operand(1, b) : kw.operand(0, b);
       } else {
@@ -1040,30 +935,14 @@ __global__ __launch_bounds__(256, 1) void kv4_weights_kernel(Kv4View c, int len,
     f32x4 s[PT];
 #pragma unroll
     for (int u = 0; u < PT; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if constexpr (kDig) {
-      constexpr int G = DigitTile<HD>::G;
-      const uint8_t* qd = reinterpret_cast<const uint8_t*>(qt);
-      int qe[G];
 #pragma unroll
-      for (int g2 = 0; g2 < G; ++g2) qe[g2] = *reinterpret_cast<const int*>(qd + DigitTile<HD>::kScales + g2 * 256 + lane * 4);
+    for (int b = 0; b < T; ++b)
 #pragma unroll
-      for (int k = kDigits - 1; k >= 0; --k)
+      for (int k = 0; k < QP; ++k) {
+        const u32x4 qq = qt[(b * QP + k) * 64 + lane];
 #pragma unroll
-        for (int g2 = 0; g2 < G; ++g2) {
-          const i32x8 d = digit_operand<HD>(qd, g2, k, lane);
-#pragma unroll
-          for (int u = 0; u < PT; ++u) s[u] = digit_scores<HD>(kcode[u], kscale[u], g2, d, qe[g2] - 5 * k, s[u]);
-        }
-    } else {
-#pragma unroll
-      for (int b = 0; b < T; ++b)
-#pragma unroll
-        for (int k = 0; k < QP; ++k) {
-          const u32x4 qq = qt[(b * QP + k) * 64 + lane];
-#pragma unroll
-          for (int u = 0; u < PT; ++u) s[u] = mfma(kop[u][b], qq, s[u]);
-        }
-    }
+        for (int u = 0; u < PT; ++u) s[u] = mfma(kop[u][b], qq, s[u]);
+      }
     const float inv = 1.f / st.y;
     if (any_nan) {
 #pragma unroll
@@ -1118,10 +997,15 @@ __global__ __launch_bounds__(256) void kv4_join_weights_kernel(const float* __re
 
 // The form of the kernel that a call takes: row tiles of a workgroup (rt), and the waves of a row tile (ps).  Four row tiles
 // read the cache once between them; up to 192 rows one tile a workgroup, each with its own pass over the cache but more
-// waves on the same chunk, is faster (24 heads on 4 behind 8192 positions: 48 rows 19.5 against 24.0 us, 192 rows
-// 35.8 against 41.0, 384 rows 64.2 against 59.0).  It takes eight waves, or four while 256 workgroups of four
-// have no more than a tile each: fewer results to join (one token: 10.4 against 12.1 us at 4096 positions, 16.5
-// against 14.8 at 16384).
+// waves on the same chunk, is faster.  Behind 8192 positions, one tile against four, us:
+//   rows            48           192          288          384
+//   24/4 x 256 f32  17.7 : 24.5  34.6 : 42.0  44.5 : 52.9  57.8 : 60.7
+//   32/8 x 128 bf16 14.6 : 18.9  30.9 : 33.0  43.5 : 42.7  47.2 : 48.8
+//   16/4 x 64 bf16   9.6 : 12.7  15.1 : 18.7  19.2 : 22.5  23.7 : 24.8
+// With one key/value head (8/1 x 256 f32: 24.0 : 31.9 at 384 rows) it would still be ahead beyond the line, whose work memory
+// and cache traffic grow with the rows.  It takes eight waves, or four while 256 workgroups of four have no more than a tile
+// each: fewer results to join (one token, four against eight: 24/4 x 256 f32 10.8 : 12.2 us at 4096 positions, 14.6 : 15.1 at
+// 16384, 18.3 : 18.1 at 32768; 8/1 x 128 f16 8.2 : 8.9 at 4096, 12.7 : 11.1 at 32768).
 struct AttendForm {
   int rt, ps;
 };
@@ -1154,12 +1038,18 @@ static int attend_chunks(int n, int n_head, int nkv, bool pairs, int len) {
   return best;
 }
 
-// From this many tiles of 16 query rows on the weights' pass takes its queries as operands formed once (attention and pass of
-// 5 tiles 25.7 against 22.3 us behind 600 positions, 66.2 against 67.6 behind 32768; of 8 tiles 27.1 against 28.1, 87.7
-// against 93.5; of 12 28.9 against 35.4).
+// From this many tiles of 16 query rows on the weights' pass takes its queries as operands formed once.  Attention and pass, formed
+// once against by every workgroup, us:
+//   rows                   80           96           128          192
+//   24/4 x 256 f32   600   24.9 : 22.5  25.4 : 24.0  26.3 : 27.9  28.3 : 35.0
+//                   8192   39.6 : 35.2  42.6 : 39.2  44.3 : 44.2  55.6 : 60.2
+//   32/8 x 128 bf16  600   19.9 : 16.1  20.2 : 16.9  20.6 : 18.8  22.7 : 22.5
+//                   8192   32.5 : 29.5  34.2 : 31.8  36.6 : 35.6  47.5 : 48.8
+//   8/1 x 256 f32   8192   27.4 : 24.9  27.9 : 26.7  29.0 : 31.0  32.6 : 38.4
 constexpr int kKv4SplitTiles = 8;
-// It has 4 tiles of 16 positions a wave then, and its query rows over as many workgroups as make up this number (333 tokens,
-// the pass alone: 26 us behind 600 positions and 72 behind 7333; each with all the rows: 110 and 129).
+// It has 4 tiles of 16 positions a wave then, and its query rows over as many workgroups as make up this number (attention and
+// pass of 2000 rows behind 2000 and 7333 positions: 24/4 x 256 f32 106 and 276 us, with all the rows in each workgroup 291
+// and 408; 16/4 x 64 bf16 46 and 100, 137 and 168; 8/1 x 128 f16 38 and 60, 161 and 181).
 constexpr int kKv4WeightGroups = 512, kKv4WeightTiles = 4;
 
 size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
@@ -1168,8 +1058,7 @@ size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
   const int tiles = (n * (n_head / c.nkv) + 15) / 16;
   if (tiles == 1) return (rows * sizeof(float2) + 15) / 16 * 16 + rec + rows * (size_t)c.cap * sizeof(float);
   // over the records; the f32 queries' are the largest
-  const size_t ready = c.hd == 256 ? DigitTile<256>::kBytes : DigitTile<128>::kBytes;
-  static_assert(ready_bytes<256, __half>() <= DigitTile<256>::kBytes && DigitTile<64>::kBytes <= DigitTile<128>::kBytes);
+  const size_t ready = (size_t)(c.hd / 32) * Parts<float>::q * 1024;
   const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * c.nkv * ready + kKv4WeightGroups * 64 * kKv4WeightTiles * sizeof(float) : 0;
   return (rows * sizeof(float2) + 15) / 16 * 16 + std::max(rec, split);
 }
@@ -1177,7 +1066,7 @@ size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
 // Dynamic LDS of a workgroup for a call of `rows` rows a key/value head.
 template <int HD, class E, int RT, int PS>
 constexpr size_t attend_lds(int rows) {
-  const size_t queries = (size_t)RT * (attend_digits<E, RT>() ? DigitTile<HD>::kBytes : HD / 32 * Parts<E>::q * 1024);
+  const size_t queries = (size_t)RT * (HD / 32 * Parts<E>::q * 1024);
   const size_t join = RT == 1 ? (size_t)PS * (128 + (rows < 16 ? rows : 16) * (HD + 8) * 4) : (size_t)(RT * PS / 2) * (HD / 32 * 2 * 1024 + 512);
   return queries > join ? queries : join;
 }

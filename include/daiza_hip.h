@@ -176,8 +176,8 @@ int dz_kv4_read_dev(const dz_kv4* c, int start, int n, float* k, float* v, void*
  * Causal attention of n queries over the cache, whose newest n rows are the queries' own: query i sees the rows
  * [0, len - n + i].  n_head is a multiple of kv_heads, query head h reads key/value head h / (n_head / kv_heads)
  * (attention.rs:149-203).  out[i][h] = sum_j softmax_j(scale * q[i][h] . K[j]) V[j]; q and out are of `type`, scores,
- * softmax statistics and sums f32 (f32 queries of more than about 100 rows a key/value head are held to 2^-29 of the largest of
- * each 32 dims, others exactly).  What a query does not see (an infinity or a NaN of a later row) does not reach it.
+ * softmax statistics and sums f32; queries are held exactly, whatever their number and type.  What a query does not see (an
+ * infinity or a NaN of a later row) does not reach it.
  * With `weights` (f32 [kv_heads] rows of ldw >= len elements, NULL: none), weights[g][j] += the sum of
  * query j's softmax weights over all queries and the heads of group g, in a fixed order.
  * `work` is device memory of dz_kv4_attend_work_bytes(c, n_head, n) bytes, 16-byte aligned, that no other work uses

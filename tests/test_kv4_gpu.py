@@ -181,6 +181,25 @@ def test_attend_queries_of_uneven_size(dz, n, hd):
     assert bool(((w.cpu().double() - ww).abs() <= wb + 4 * held.amax() * ww + 2.0 ** -24 * ww).all())
 
 
+@pytest.mark.parametrize("n", [1, 30, 70])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attend_f32_queries_beside_outliers(dz, n, hd):
+    """One dim in every 32 a million times the others, whose keys are held as 0: the other dims' bits count as in any f32 product,
+    by one query and by many, in the outputs and in the weights."""
+    k, v = _rows(59, 150, 1, hd), _rows(63, 150, 1, hd)
+    k[:, :, 7::32] *= 1e-6
+    q = _normal(64, n, 4, hd)
+    q[:, :, 7::32] *= 2.0 ** 20
+    ks, vs = ref.stored(k), ref.stored(v)
+    assert bool((ks[:, :, 7::32] == 0).all())
+    c = _cache(dz, k, v)
+    out, w = torch.empty(n, 4, hd, device="cuda"), torch.zeros(1, 150, device="cuda")
+    c.attend_dev(q.cuda(), out, weights=w)
+    want, ww, bound, wb = ref.attend(q, ks, vs)
+    assert bool(((out.cpu().double() - want).abs() <= bound + 2.0 ** -24 * want.abs()).all())
+    assert bool(((w.cpu().double() - ww).abs() <= wb + 2.0 ** -24 * ww).all())
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_query_that_is_not_a_number_among_many(dz, value, hd):
