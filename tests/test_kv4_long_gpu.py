@@ -1,0 +1,109 @@
+"""Long caches, many rows and large vocabularies, where calls take other forms of the kernels than the short ones of
+test_kv4_gpu.py and test_logprobs_gpu.py, against the same 64-bit plain forms (kv4_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import kv4_ref as ref
+from test_kv4_gpu import TYPES, _cache, _check_attend, _check_evict, _normal, _rows, _same
+from test_logprobs_gpu import _check, _logits
+
+pytestmark = pytest.mark.gpu
+
+
+# Eight waves on a row tile (beyond 32768 positions times key/value heads and row tiles), and chunks by the dozen: at one
+# key/value head 20000 and 40000 positions go in 157 chunks, of four and of eight waves.
+@pytest.mark.parametrize("nq,nkv,hd,length,n", [(24, 4, 256, 9000, 1), (24, 4, 256, 9000, 2), (24, 4, 256, 9001, 8), (2, 1, 64, 20000, 1),
+                                                (2, 1, 64, 40000, 1), (7, 1, 128, 33000, 3), (16, 8, 128, 4500, 7)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_long(dz, nq, nkv, hd, length, n, dtype):
+    _check_attend(dz, nq, nkv, hd, length, n, dtype, True)
+
+
+# 17 to 112 query rows: the weights' pass has two tiles of 16 positions a wave from 400 blocks of 64 positions and heads on, and
+# four from 800.
+@pytest.mark.parametrize("nq,nkv,hd,length,n", [(16, 8, 64, 3300, 9), (16, 8, 64, 3271, 56), (16, 8, 64, 6500, 20), (8, 4, 128, 6410, 13),
+                                                (8, 4, 64, 12801, 50), (16, 8, 256, 3300, 20), (8, 8, 256, 6405, 17)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_weights_of_few_tokens_behind_many_rows(dz, nq, nkv, hd, length, n, dtype):
+    _check_attend(dz, nq, nkv, hd, length, n, dtype, True)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,length,n,at", [(24, 4, 256, 9000, 8, 8996), (24, 4, 256, 9000, 1, 31), (2, 1, 64, 40000, 3, 39998),
+                                                   (16, 8, 64, 3300, 20, 3290), (16, 8, 64, 6500, 20, 6485), (8, 4, 128, 6410, 13, 6397)])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_later_rows_stay_out_of_long_calls(dz, nq, nkv, hd, length, n, at, where):
+    """A row with a NaN: queries before it are as without it, bit for bit, those that see it get NaN, and the weights of other
+    heads' rows and, of a value, all weights are untouched."""
+    k, v = _rows(80, length, nkv, hd), _rows(81, length, nkv, hd)
+    q = _normal(82, n, nq, hd).cuda()
+    got = []
+    for bad in (False, True):
+        if bad:
+            (k if where == "k" else v)[at, 0, 37] = math.nan
+        c = _cache(dz, k, v)
+        out, w = torch.empty_like(q), torch.zeros(nkv, length, device="cuda")
+        c.attend_dev(q, out, weights=w)
+        got.append((out.cpu(), w.cpu()))
+    (want, ww), (out, w) = got
+    first, grp = max(0, at - (length - n)), nq // nkv
+    assert torch.equal(out[:first], want[:first]) and torch.equal(out[:, grp:], want[:, grp:]) and torch.equal(w[1:], ww[1:])
+    if where == "k":
+        assert bool(torch.isnan(out[first:, :grp]).all())
+        # every row that a query with a NaN sees gets its share of it; the first such query sees the rows up to `seen`
+        seen = length - n + first + 1
+        assert bool(torch.isnan(w[0, :seen]).all())
+    else:
+        assert bool(torch.isnan(out[first:, :grp, 32:64]).all()) and torch.equal(out[..., :32], want[..., :32])
+        assert torch.equal(w, ww)
+
+
+# More than 32768 rows to choose from: the keys are read anew for each pass instead of staying in registers.
+@pytest.mark.parametrize("kind", ["spread", "equal", "zeros", "special"])
+@pytest.mark.parametrize("nkv,length,keep,recent", [(2, 32769, 1, 0), (1, 32868, 32868, 99), (1, 32869, 20000, 100), (2, 40001, 10000, 256),
+                                                    (1, 100000, 33333, 0), (1, 100000, 99999, 64)])
+def test_evict_long(dz, kind, nkv, length, keep, recent):
+    g = torch.Generator().manual_seed(length + keep)
+    w = torch.exp(torch.randn(nkv, length, generator=g) * 3)
+    if kind == "equal":
+        w[:] = 0.75
+    elif kind == "zeros":
+        w = torch.where(torch.rand(w.shape, generator=g) < 0.95, torch.zeros_like(w), w)
+        w[0, ::3] = -0.0
+    elif kind == "special":
+        r = torch.rand(w.shape, generator=g)
+        w = torch.where(r < 0.4, torch.full_like(w, math.nan), torch.where(r < 0.5, torch.full_like(w, math.inf), w))
+        w = torch.where((r > 0.6) & (r < 0.9), torch.floor(w), w)
+    _check_evict(dz, w, keep, recent, 64)
+
+
+# More than 1024 groups of 256 logits: they are looked through in batches.
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab,top", [(262144, 20), (262145, 20), (300001, 64), (600000, 3)])
+def test_large_vocabularies(dz, dtype, vocab, top):
+    _check(dz, *_logits(vocab, 2, vocab, dtype), top)
+
+
+@pytest.mark.parametrize("kind", ["equal", "rising", "falling", "last", "masked"])
+def test_orders_over_large_vocabularies(dz, kind):
+    vocab = 300001
+    i = torch.arange(vocab, dtype=torch.float32)
+    x = {"equal": torch.full((vocab,), 0.5), "rising": i * 1e-4, "falling": -i * 1e-4, "last": torch.where(i > vocab - 30, 4.0, 0.0),
+         "masked": torch.where(i < 270000, -math.inf, 1.0)}[kind].reshape(1, -1)
+    if kind == "masked":
+        x[0, 270005:] = -math.inf
+    _check(dz, x, torch.tensor([270001], dtype=torch.int32), 40)
+
+
+def test_more_rows_than_a_launch_takes(dz):
+    _check(dz, *_logits(9, 70000, 7), 2)
+
+
+def test_rows_in_and_out_of_a_long_cache(dz):
+    n, nkv, hd = 70001, 1, 64
+    k, v = _rows(90, n, nkv, hd), _rows(91, n, nkv, hd)
+    c = _cache(dz, k, v)
+    gk, gv = (torch.empty(nkv, n, hd, device="cuda") for _ in range(2))
+    c.read_dev(0, gk, gv)
+    assert _same(gk.cpu().double(), ref.stored(k)) and _same(gv.cpu().double(), ref.stored(v))
