@@ -464,14 +464,14 @@ class Context:
     """ModelState + ForwardContext (forward.rs:32-131) on the device.
 
     kv4: the key/value cache in 4 bits (dz_ctx_create_kv4), for kv_rows rows (0: max_ctx); track: with the attention weight
-    that each row receives, for kv_evict."""
+    that each row receives, for kv_evict; track=2 counts the drafts that verify_commit keeps too."""
 
     def __init__(self, model, kv4=False, kv_rows=0, track=False):
         self.model = model
         self.cfg = model.cfg
         h = _vp()
         if kv4:
-            _check(lib().dz_ctx_create_kv4(model._h, int(kv_rows), int(bool(track)), ctypes.byref(h)))
+            _check(lib().dz_ctx_create_kv4(model._h, int(kv_rows), int(track), ctypes.byref(h)))
         elif kv_rows or track:
             raise DaizaError(DZ_ERR_UNSUPPORTED, "kv_rows and track need kv4")
         else:

@@ -107,12 +107,14 @@ struct dz_ctx {
     // verify records per DeltaNet layer: conv inputs [kv][qkvd] and the scan's rollback record
     int kv_cap = 0;
     dz::DnRecords recs{};
+    float* vq = nullptr;      // [attention layer][kv_cap][n_head · head_dim]: a verify's queries (kv4.drafts)
     int pending = 0;          // tokens of the last verify forward (0: none); their ids are in `ids`
   } bt;
   // key/value cache in 4 bits (dz_ctx_create_kv4), in place of kv: every attention layer holds the rows of
   // pos_host - evicted positions
   struct {
     bool on = false, track = false;
+    bool drafts = false;              // track: a verify's commit adds the weights of the drafts that it keeps
     int rows = 0;                     // capacity
     std::vector<dz::Kv4View> layer;   // per attention layer
     std::vector<float*> w;            // per attention layer: weights [nkv][cap] (track)
@@ -1379,6 +1381,7 @@ static int bt_reserve_verify(dz_ctx* x, int k) {
   if ((rc = alloc_t(A, &r.x, lk * qkvd)) || (rc = alloc_t(A, &r.decay, lk * c.ssm_v_heads)) || (rc = alloc_t(A, &r.d, lk * inner)) ||
       (rc = alloc_t(A, &r.k, lk * kdim)))
     return rc;
+  if (x->kv4.drafts && (rc = alloc_t(A, &x->bt.vq, (size_t)x->m->n_attn * k * c.n_head * c.head_dim))) return rc;
   r.cap = k;
   x->bt.kv_cap = k;
   return DZ_OK;
@@ -1572,9 +1575,10 @@ static int bt_forward(dz_ctx* x, const uint32_t* ids, int n, int out_rows, bool 
         if ((rc = bt_gemm(x, l.out_proj, x->bt.gy, inner, n, nullptr, x->bt.h, H, 1))) return rc;
       }
     } else if (x->kv4.on) {
-      // a verify's drafts may be dropped again: only forwards that are kept add to the weights
+      // a verify's drafts may be dropped again: only forwards that are kept add to the weights (see bt_verify_commit)
       const ProjRows proj{x->bt.yin, ld_in};
-      if ((rc = kv4_attention(x, l, proj, p0, n, x->bt.qb, x->bt.gate, x->bt.gy, x->kv4.track && !verify, s))) return rc;
+      float* q = verify && x->kv4.drafts ? x->bt.vq + (size_t)l.kind_idx * x->bt.kv_cap * qd : x->bt.qb;
+      if ((rc = kv4_attention(x, l, proj, p0, n, q, x->bt.gate, x->bt.gy, x->kv4.track && !verify, s))) return rc;
       if ((rc = bt_gemm(x, l.out_proj, x->bt.gy, qd, n, nullptr, x->bt.h, H, 1, few ? &gd : nullptr))) return rc;
     } else {
       float* kc = x->kv + (size_t)l.kind_idx * 2 * kvsz;
@@ -1669,10 +1673,23 @@ static int bt_verify_commit(dz_ctx* x, int a) {
   const int64_t hd = c.ssm_state, kdim = (int64_t)c.ssm_k_heads * hd, inner = (int64_t)c.ssm_v_heads * hd;
   const int64_t qkvd = 2 * kdim + inner;
   const int p0 = x->pos_host;
+  // (its work memory may be larger than that of all k drafts: few rows keep their scores)
+  if (x->kv4.drafts && m->n_attn)
+    if (int rc = x->kv4.work.reserve(kv4_attend_work(x->kv4.layer[0], (int)c.n_head, a))) return rc;
   if (m->n_ssm)
     DZ_HIP_CHECK(launch(bt_commit_kernel, dim3((unsigned)(4 * c.ssm_v_heads + (qkvd + 255) / 256), (unsigned)m->n_ssm), dim3(256),
                         x->s, x->ssm_state, x->conv, (const int*)x->ring_base_dev, p0, x->bt.recs, a, (int)c.ssm_k_heads,
                         (int)c.ssm_v_heads, qkvd));
+  // the weights of the drafts that stay: their queries once more over the rows that they see, as a forward of them alone
+  // (the outputs go to a buffer that nothing reads)
+  const int row = p0 - x->kv4.evicted;
+  const int64_t qd = (int64_t)c.n_head * c.head_dim;
+  for (size_t i = 0; x->kv4.drafts && i < x->kv4.layer.size(); ++i) {
+    const Kv4View& v = x->kv4.layer[i];
+    if (int rc = kv4_attend(v, row + a, x->bt.vq + i * (size_t)x->bt.kv_cap * qd, qd, DZ_F32, (int)c.n_head, a, 1.0f, x->kv4.w[i],
+                            v.cap, x->bt.gy, qd, x->kv4.work.ptr, x->s, nullptr))
+      return rc;
+  }
   const int rc = bt_finish(x, a, p0, a - 1);
   if (rc) return rc;
   DZ_HIP_CHECK(hipStreamSynchronize(x->s));
@@ -1764,7 +1781,7 @@ static int check_logprobs(const dz_ctx* x, int top, const void* targets, const v
 }  // namespace dz
 
 // A context; kv4_rows > 0: with its key/value cache in 4 bits, for that many rows.
-static int ctx_create(dz_model* m, int kv4_rows, bool track, dz_ctx** out) {
+static int ctx_create(dz_model* m, int kv4_rows, int track, dz_ctx** out) {
   int rc = ensure_device();
   if (rc) return rc;
   if ((rc = prepare_gemv_kernels()) || (kv4_rows && (rc = prepare_kv4_kernels()))) return rc;
@@ -1773,6 +1790,7 @@ static int ctx_create(dz_model* m, int kv4_rows, bool track, dz_ctx** out) {
   const dz_config& c = m->cfg;
   x->kv4.on = kv4_rows > 0;
   x->kv4.track = kv4_rows > 0 && track;
+  x->kv4.drafts = kv4_rows > 0 && track == 2;
   x->kv4.rows = kv4_rows;
   auto fail = [&](int code) { ctx_release(x); return code; };
   hipError_t e = hipStreamCreateWithFlags(&x->s, hipStreamNonBlocking);
@@ -1840,14 +1858,14 @@ extern "C" {
 
 int dz_ctx_create(dz_model* m, dz_ctx** out) {
   if (!m || !out) return set_error(DZ_ERR_MODEL, "null argument");
-  return ctx_create(m, 0, false, out);
+  return ctx_create(m, 0, 0, out);
 }
 
 int dz_ctx_create_kv4(dz_model* m, int kv_rows, int track, dz_ctx** out) {
   if (!m || !out) return set_error(DZ_ERR_MODEL, "null argument");
   if (kv_rows < 0 || kv_rows > m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "4-bit cache of %d rows (max_ctx %d)", kv_rows, m->cfg.max_ctx);
   try {
-    return ctx_create(m, kv_rows ? kv_rows : m->cfg.max_ctx, track != 0, out);
+    return ctx_create(m, kv_rows ? kv_rows : m->cfg.max_ctx, track, out);
   } catch (...) {  // an allocation on the host
     return set_error(DZ_ERR_MODEL, "out of memory");
   }

@@ -272,7 +272,11 @@ int dz_model_weight_bytes(const dz_model* m, uint64_t* q1_bytes);
  * 4 bits lose.  dz_ctx_get_kv reads what the rows stand for, dz_ctx_set_kv rounds to it; dz_ctx_copy_state
  * needs contexts of one kind.  The reference has no such cache.
  * track != 0: the context also sums the attention weight that each cached row receives (over the heads of a key/value
- * head's group) in every forward that is kept, starting from 0 when the row is written; a verify adds none.
+ * head's group) in every forward, starting from 0 when the row is written.  A verify adds none, as its drafts may be
+ * dropped; with track == 2 its commit adds what the drafts that are kept gave, as if they alone had been forwarded (their attention is
+ * formed a second time then), otherwise the commit adds none either and rows that only accepted drafts attended to are the
+ * first to be evicted.  What dropped tokens gave (dz_kv_truncate, dz_ctx_set_pos) stays in the rows that remain, and tokens
+ * forwarded again add again.
  */
 int dz_ctx_create_kv4(dz_model* m, int kv_rows, int track, dz_ctx** out);
 /* Eviction by accumulated attention weight on a context that tracks it: every attention layer keeps, per key/value head,

@@ -357,3 +357,72 @@ def test_non_finite_row_of_a_context(dz, oracle):
     assert np.isnan(a.forward_single_token(3)[1]).all()
     a.kv_truncate(40)
     assert np.array_equal(a.forward_single_token(3)[1], want)
+
+
+@pytest.mark.parametrize("k,a", [(5, 2), (3, 2), (1, 1), (8, 8), (4, 0), (40, 30)])
+def test_accepted_drafts_count_in_the_weights(dz, oracle, k, a):
+    """track=2: verify and commit leave the weights that a forward of the accepted drafts alone leaves, and the same eviction."""
+    cfg, om, model, x = _setup(dz, oracle, track=2, kv_rows=150)
+    y = dz.Context(model, kv4=True, kv_rows=150, track=True)
+    ids = np.random.default_rng(20).integers(0, cfg.vocab, 100)
+    x.forward_batch(ids[:50])
+    x.kv_evict(40, 8)  # rows and positions differ
+    y.copy_state_from(x)
+    before = {l: x.kv_weights(l) for l in _attn(cfg)}
+    x.verify_forward(ids[50:50 + k])
+    for l in _attn(cfg):
+        assert np.array_equal(x.kv_weights(l), before[l])
+    x.verify_commit(a)
+    if a:
+        y.forward_batch(ids[50:50 + a])
+    assert x.pos == y.pos == 50 + a
+    for l in _attn(cfg):
+        wx, wy = x.kv_weights(l), y.kv_weights(l)
+        assert wx.shape == wy.shape == (cfg.n_head_kv, 40 + a)
+        # sums of a x (heads of a group) probabilities of attentions that agree to the bar
+        assert np.abs(wx - wy).max() <= a * (cfg.n_head // cfg.n_head_kv) * BAR
+        total = a * cfg.n_head // cfg.n_head_kv
+        assert np.allclose(wx.sum(1) - before[l].sum(1), total, atol=1e-4 * max(1, total))
+    # k and a tokens take their products in forms that round in other orders
+    assert normwise_rel(x.forward_single_token(3)[1], y.forward_single_token(3)[1]) < BAR
+    z = dz.Context(model, kv4=True, kv_rows=150, track=True)  # without it the commit adds none
+    z.forward_batch(ids[:50])
+    z.verify_forward(ids[50:50 + k])
+    w = {l: z.kv_weights(l) for l in _attn(cfg)}
+    z.verify_commit(a)
+    for l in _attn(cfg):
+        assert np.array_equal(z.kv_weights(l)[:, :50], w[l]) and not z.kv_weights(l)[:, 50:].any()
+
+
+def test_speculative_steps_count_in_the_weights(dz, oracle):
+    """dz_spec_verify on a track=2 context: every forwarded token's attention is in the weights once."""
+    cfg, om, model, x = _setup(dz, oracle, track=2)
+    ids = np.random.default_rng(21).integers(0, cfg.vocab, 30)
+    t = int(np.argmax(x.forward_batch(ids)))
+    y = dz.Context(model, kv4=True)
+    y.forward_batch(ids)
+    greedy = y.decode_greedy(t, 6)
+    draft = np.append([t], greedy[:3]).astype(np.uint32)
+    draft[-1] = (draft[-1] + 1) % cfg.vocab  # three right ones and a wrong one
+    n, bonus = x.spec_verify(draft, None, dz.SamplingParams(0.0, 0, 1.0), dz.LcgRng(1))[:2]
+    assert n == 3 and bonus == greedy[2] and x.pos == 33
+    grp = cfg.n_head // cfg.n_head_kv
+    for l in _attn(cfg):
+        assert np.allclose(x.kv_weights(l).sum(1), 33 * grp, atol=1e-4 * 33 * grp)
+
+
+def test_weights_after_going_back(dz, oracle):
+    """What dropped tokens gave stays in the rows that remain; forwarded again, they give it again and their rows start from 0."""
+    cfg, om, model, x = _setup(dz, oracle, n_layers=1, full_attn_interval=1)
+    ids = np.random.default_rng(22).integers(0, cfg.vocab, 52)
+    x.forward_batch(ids[:40])
+    w0 = x.kv_weights(0)
+    x.forward_batch(ids[40:])
+    w1 = x.kv_weights(0)
+    x.kv_truncate(40)
+    assert np.array_equal(x.kv_weights(0), w1[:, :40])
+    x.forward_batch(ids[40:])
+    w2 = x.kv_weights(0)
+    # an attention layer alone: the same tokens at the same positions give the same; two f32 additions of sums up to 52 x group
+    assert np.allclose(w2[:, :40] - w1[:, :40], w1[:, :40] - w0, atol=2 * 52 * (cfg.n_head // cfg.n_head_kv) * 2.0 ** -24)
+    assert np.array_equal(w2[:, 40:], w1[:, 40:])
