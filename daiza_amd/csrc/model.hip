@@ -509,6 +509,13 @@ static int launch_attention(int grp, dim3 grid, const AttnArgs& a, hipStream_t s
   });
 }
 
+// Work memory for the attention of n tokens on a 4-bit cache.  Called before a forward's first launch, for a forward that fails
+// further on leaves DeltaNet layers a token ahead.
+static int kv4_reserve(dz_ctx* x, int n) {
+  if (x->kv4.layer.empty()) return DZ_OK;
+  return x->kv4.work.reserve(kv4_attend_work(x->kv4.layer[0], (int)x->m->cfg.n_head, n));
+}
+
 // Attention of n tokens at positions pos .. of a context whose cache is in 4 bits, from their in-projection: its rows into
 // the cache, then the gated outputs -> out[n][n_head · head_dim].
 template <class Src>
@@ -518,7 +525,6 @@ static int kv4_attention(dz_ctx* x, const LayerDev& l, const Src& src, int pos, 
   const Kv4View& v = x->kv4.layer[(size_t)l.kind_idx];
   float* w = x->kv4.track ? x->kv4.w[(size_t)l.kind_idx] : nullptr;
   const int row = pos - x->kv4.evicted;
-  if (int rc = x->kv4.work.reserve(kv4_attend_work(v, (int)c.n_head, n))) return rc;
   hipLaunchKernelGGL(kv4_prep_kernel<Src>, dim3((unsigned)n, (unsigned)(c.n_head + c.n_head_kv)), dim3(256), 0, s, src, (int)c.n_head,
                      (int)c.n_head_kv, (const float*)l.q_norm, (const float*)l.k_norm, c.rms_eps, (const float*)x->rope,
                      (int)c.rope_dim, pos, row, q, gate, v, w, (int64_t)v.cap);
@@ -824,6 +830,7 @@ static int ctx_run(dz_ctx* x, int n) {
     return set_error(DZ_ERR_TENSOR, "context full: pos %d + %d > max_ctx %d", x->pos_host, n, x->m->cfg.max_ctx);
   if (int rc = kv4_room(x, n)) return rc;
   if (x->kv4.on) {
+    if (int rc = kv4_reserve(x, 1)) return rc;
     // the rows that a token's attention reads size its launches: no graph
     for (int i = 0; i < n; ++i)
       if (int rc = enqueue_token(x, x->s, x->pos_host + i)) return rc;
@@ -1491,7 +1498,10 @@ static int bt_forward(dz_ctx* x, const uint32_t* ids, int n, int out_rows, bool 
   hipStream_t s = x->s;
   int rc;
   if ((rc = bt_reserve(x, n)) || (rc = bt_reserve_logits(x, out_rows))) return rc;
-  if (verify && (rc = bt_reserve_verify(x, n))) return rc;
+  if ((verify && (rc = bt_reserve_verify(x, n))) || (rc = kv4_reserve(x, n))) return rc;
+  if (!verify && n >= kScanMinTokens && m->n_ssm &&
+      (rc = x->bt.chunk.reserve(chunk_prep_floats(n, (int)c.ssm_k_heads, (int)c.ssm_v_heads) * sizeof(float))))
+    return rc;
   for (int i = 0; i < n; ++i)
     if (ids[i] >= (uint32_t)c.vocab) return set_error(DZ_ERR_TENSOR, "token id %u >= vocab %d", ids[i], c.vocab);
   FewIds fi{};
@@ -1547,7 +1557,6 @@ static int bt_forward(dz_ctx* x, const uint32_t* ids, int n, int out_rows, bool 
       float* state = x->ssm_state + (size_t)si * c.ssm_v_heads * hd * hd;
       const int nkh = (int)c.ssm_k_heads, nvh = (int)c.ssm_v_heads;
       if (!verify && n >= kScanMinTokens) {
-        if ((rc = x->bt.chunk.reserve(chunk_prep_floats(n, nkh, nvh) * sizeof(float)))) return rc;
         const ChunkPrep cp = chunk_prep_carve(static_cast<float*>(x->bt.chunk.ptr), n, nkh, nvh);
         DZ_HIP_CHECK(launch(bt_chunk_prep_kernel, dim3((unsigned)nvh, (unsigned)((n + kScanC - 1) / kScanC)), dim3(256), s,
                             (const float*)x->bt.yin, ld_in, (const float*)x->bt.cout, qkvd, (const float*)x->bt.qk, n, nkh,
@@ -1674,8 +1683,8 @@ static int bt_verify_commit(dz_ctx* x, int a) {
   const int64_t qkvd = 2 * kdim + inner;
   const int p0 = x->pos_host;
   // (its work memory may be larger than that of all k drafts: few rows keep their scores)
-  if (x->kv4.drafts && m->n_attn)
-    if (int rc = x->kv4.work.reserve(kv4_attend_work(x->kv4.layer[0], (int)c.n_head, a))) return rc;
+  if (x->kv4.drafts)
+    if (int rc = kv4_reserve(x, a)) return rc;
   if (m->n_ssm)
     DZ_HIP_CHECK(launch(bt_commit_kernel, dim3((unsigned)(4 * c.ssm_v_heads + (qkvd + 255) / 256), (unsigned)m->n_ssm), dim3(256),
                         x->s, x->ssm_state, x->conv, (const int*)x->ring_base_dev, p0, x->bt.recs, a, (int)c.ssm_k_heads,
@@ -1749,13 +1758,19 @@ static int bt_prefill(dz_ctx* x, const uint32_t* ids, int n, float* last_logits,
   return DZ_OK;
 }
 
+// Bytes on the device for the log probabilities of n rows: the work memory, then targets and results.
+static size_t ctx_logprobs_bytes(const dz_ctx* x, int n, int top, size_t* work) {
+  *work = (logprobs_work(n, (int)x->m->cfg.vocab, top) + 15) / 16 * 16;
+  return *work + ((size_t)3 * n + 2 * (size_t)n * top) * 4;
+}
 // Log probabilities of n rows of logits on the device, targets and results in host arrays (dz_forward_logprobs); enqueued,
 // the caller waits.
 static int ctx_logprobs(dz_ctx* x, const float* logits, int n, const int32_t* targets, int top, float* logp, float* entropy,
                         int32_t* top_ids, float* top_logp) {
   const int V = (int)x->m->cfg.vocab;
-  const size_t work = (logprobs_work(n, V, top) + 15) / 16 * 16, nt = (size_t)n * top;
-  if (int rc = x->bt.logp.reserve(work + ((size_t)3 * n + 2 * nt) * 4)) return rc;
+  const size_t nt = (size_t)n * top;
+  size_t work;
+  if (int rc = x->bt.logp.reserve(ctx_logprobs_bytes(x, n, top, &work))) return rc;
   uint8_t* base = static_cast<uint8_t*>(x->bt.logp.ptr);
   int32_t* tok = reinterpret_cast<int32_t*>(base + work);
   float *lp = reinterpret_cast<float*>(tok + n), *en = lp + n, *tl = en + n;
@@ -1840,7 +1855,8 @@ static int ctx_create(dz_model* m, int kv4_rows, int track, dz_ctx** out) {
       if (e4 != hipSuccess) return fail(set_error(DZ_ERR_DEVICE, "hipMemsetAsync: %s", hipGetErrorString(e4)));
       if ((rc = alloc_t(A, &x->kv4.kept, (size_t)nkv * cap))) return fail(rc);
     }
-    if ((rc = alloc_t(A, &x->kv4.q, (size_t)c.n_head * c.head_dim)) || (rc = alloc_t(A, &x->kv4.gate, (size_t)c.n_head * c.head_dim)))
+    if ((rc = alloc_t(A, &x->kv4.q, (size_t)c.n_head * c.head_dim)) || (rc = alloc_t(A, &x->kv4.gate, (size_t)c.n_head * c.head_dim)) ||
+        (rc = kv4_reserve(x, 1)))
       return fail(rc);
   }
   x->ring_base.assign((size_t)m->n_ssm, 0);
@@ -2320,6 +2336,7 @@ int dz_ctx_mixer_step_dev(dz_ctx* x, int layer, const float* h_dev, float* h_out
   if (layer < 0 || layer >= x->m->cfg.n_layers) return set_error(DZ_ERR_TENSOR, "layer %d out of range", layer);
   if (x->pos_host >= x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "context full");
   if (int rc0 = kv4_room(x, 1)) return rc0;
+  if (int rc0 = kv4_reserve(x, 1)) return rc0;
   const dz_config& c = x->m->cfg;
   int64_t ld_in, ld_h, ld_gu;
   int th, to, tf;
@@ -2348,6 +2365,7 @@ int dz_ctx_mixer_step(dz_ctx* x, int layer, float* h) {
   if (layer < 0 || layer >= x->m->cfg.n_layers) return set_error(DZ_ERR_TENSOR, "layer %d out of range", layer);
   if (x->pos_host >= x->m->cfg.max_ctx) return set_error(DZ_ERR_TENSOR, "context full");
   if (int rc0 = kv4_room(x, 1)) return rc0;
+  if (int rc0 = kv4_reserve(x, 1)) return rc0;
   const dz_config& c = x->m->cfg;
   int64_t ld_in, ld_h, ld_gu;
   int th, to, tf;
@@ -2386,8 +2404,9 @@ int dz_forward_logprobs(dz_ctx* x, const uint32_t* ids, const int32_t* targets, 
   auto run = [&]() -> int {
     for (int i0 = 0; i0 < n; i0 += kChunk) {
       const int k = std::min(kChunk, n - i0);
-      int rc = bt_forward(x, ids + i0, k, k, false);
-      if (rc || (rc = bt_finish(x, k, x->pos_host, k - 1))) return rc;
+      size_t work;
+      int rc = x->bt.logp.reserve(ctx_logprobs_bytes(x, k, top, &work));  // before the tokens are forwarded
+      if (rc || (rc = bt_forward(x, ids + i0, k, k, false)) || (rc = bt_finish(x, k, x->pos_host, k - 1))) return rc;
       const size_t t0 = (size_t)i0 * top;
       if ((rc = ctx_logprobs(x, x->bt.logits, k, targets ? targets + i0 : nullptr, top, logp ? logp + i0 : nullptr,
                              entropy ? entropy + i0 : nullptr, top_ids + t0, top_logp ? top_logp + t0 : nullptr)))

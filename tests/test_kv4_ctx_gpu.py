@@ -426,3 +426,22 @@ def test_weights_after_going_back(dz, oracle):
     # an attention layer alone: the same tokens at the same positions give the same; two f32 additions of sums up to 52 x group
     assert np.allclose(w2[:, :40] - w1[:, :40], w1[:, :40] - w0, atol=2 * 52 * (cfg.n_head // cfg.n_head_kv) * 2.0 ** -24)
     assert np.array_equal(w2[:, 40:], w1[:, 40:])
+
+
+def test_a_token_allocates_nothing(dz, oracle):
+    """The work memory of a token's attention, which keeps its scores for the weights (16 MB here), is there before the first
+    token: a failed allocation between its layers would leave some of them a token ahead."""
+    shape = dict(n_layers=2, full_attn_interval=2, max_ctx=1 << 20, rope_dim=16)
+    cfg, om, model, small = _setup(dz, oracle, kv_rows=64, **shape)
+    ctx = dz.Context(model, kv4=True, track=True)
+    for layer in range(2):  # what the runtime keeps for the kernels' first launches
+        small.mixer_step(layer, np.zeros(cfg.hidden, np.float32))
+    small.reset()
+    small.forward_single_token(3)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    ctx.forward_single_token(3)
+    ctx.decode_greedy(5, 3)
+    ctx.mixer_step(1, np.zeros(cfg.hidden, np.float32))
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] == before
