@@ -181,6 +181,7 @@ _MODEL_PROTOS = {
     "dz_kv4_append_dev": ([_vp, _vp, _i64, _vp, _i64, ctypes.c_int, ctypes.c_int, _vp], ctypes.c_int),
     "dz_kv4_read_dev": ([_vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp], ctypes.c_int),
     "dz_kv4_attend_work_bytes": ([_vp, ctypes.c_int, ctypes.c_int], ctypes.c_size_t),
+    "dz_kv4_attend_only_work_bytes": ([_vp, ctypes.c_int, ctypes.c_int], ctypes.c_size_t),
     "dz_kv4_attend_dev": ([_vp, _vp, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp, _i64, _vp, _i64, _vp,
                            _vp], ctypes.c_int),
     "dz_kv4_evict_dev": ([_vp, _vp, _i64, ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, _vp], ctypes.c_int),
@@ -809,7 +810,8 @@ class Kv4Cache:
             if weights.shape[1] < len(self):
                 raise DaizaError(DZ_ERR_TENSOR, "weights of %d rows, %d held" % (weights.shape[1], len(self)))
         s, L = _call_stream(q, stream), lib()
-        w = _work(q, L.dz_kv4_attend_work_bytes(self._h, heads, n), s)
+        size = L.dz_kv4_attend_only_work_bytes if wp is None else L.dz_kv4_attend_work_bytes
+        w = _work(q, size(self._h, heads, n), s)
         _check(L.dz_kv4_attend_dev(self._h, qp, ldq, ty, heads, n, self.head_dim ** -0.5 if scale is None else float(scale), wp, ldw,
                                    op, ldo, w.data_ptr(), s))
 

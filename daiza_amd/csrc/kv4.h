@@ -92,7 +92,8 @@ __device__ __forceinline__ float kv4_scale(unsigned byte) {
 int kv4_append(const Kv4View& c, int row0, const void* k, int64_t ldk, const void* v, int64_t ldv, int type, int n, hipStream_t s);
 int kv4_read(const Kv4View& c, int start, int n, float* k, float* v, hipStream_t s);
 int prepare_kv4_kernels();
-size_t kv4_attend_work(const Kv4View& c, int n_head, int n);
+// weights: for calls that add to the rows' weights.
+size_t kv4_attend_work(const Kv4View& c, int n_head, int n, bool weights);
 // gate: see AttendOut (f32 [n][n_head][head_dim]).
 int kv4_attend(const Kv4View& c, int len, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                int64_t ldw, void* out, int64_t ldo, void* work, hipStream_t s, const float* gate);

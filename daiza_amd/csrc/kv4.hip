@@ -1052,15 +1052,17 @@ constexpr int kKv4SplitTiles = 8;
 // and 408; 16/4 x 64 bf16 46 and 100, 137 and 168; 8/1 x 128 f16 38 and 60, 161 and 181).
 constexpr int kKv4WeightGroups = 512, kKv4WeightTiles = 4;
 
-size_t kv4_attend_work(const Kv4View& c, int n_head, int n) {
+size_t kv4_attend_work(const Kv4View& c, int n_head, int n, bool weights) {
   const size_t rows = (size_t)n * n_head, nch = (size_t)attend_chunks(n, n_head, c.nkv, c.hd <= 128, 0);
   const size_t rec = nch > 1 ? (rows * nch * (size_t)(2 + c.hd) * sizeof(float) + 15) / 16 * 16 : 0;
   const int tiles = (n * (n_head / c.nkv) + 15) / 16;
-  if (tiles == 1) return (rows * sizeof(float2) + 15) / 16 * 16 + rec + rows * (size_t)c.cap * sizeof(float);
+  const size_t stats = (rows * sizeof(float2) + 15) / 16 * 16;
+  if (!weights) return stats + rec;
+  if (tiles == 1) return stats + rec + rows * (size_t)c.cap * sizeof(float);  // the scores
   // over the records; the f32 queries' are the largest
   const size_t ready = (size_t)(c.hd / 32) * Parts<float>::q * 1024;
   const size_t split = tiles >= kKv4SplitTiles ? (size_t)tiles * c.nkv * ready + kKv4WeightGroups * 64 * kKv4WeightTiles * sizeof(float) : 0;
-  return (rows * sizeof(float2) + 15) / 16 * 16 + std::max(rec, split);
+  return stats + std::max(rec, split);
 }
 
 // Dynamic LDS of a workgroup for a call of `rows` rows a key/value head.
@@ -1480,10 +1482,12 @@ int dz_kv4_read_dev(const dz_kv4* c, int start, int n, float* k, float* v, void*
   return kv4_read(c->v, start, n, k, v, static_cast<hipStream_t>(stream));
 }
 
-size_t dz_kv4_attend_work_bytes(const dz_kv4* c, int n_head, int n) {
+static size_t attend_work_bytes(const dz_kv4* c, int n_head, int n, bool weights) {
   if (!c || n_head < 1 || n < 1 || n_head % c->v.nkv || (int64_t)n * n_head > 1 << 30) return 0;  // refused calls
-  return kv4_attend_work(c->v, n_head, n);
+  return kv4_attend_work(c->v, n_head, n, weights);
 }
+size_t dz_kv4_attend_work_bytes(const dz_kv4* c, int n_head, int n) { return attend_work_bytes(c, n_head, n, true); }
+size_t dz_kv4_attend_only_work_bytes(const dz_kv4* c, int n_head, int n) { return attend_work_bytes(c, n_head, n, false); }
 
 int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                       int64_t ldw, void* out, int64_t ldo, void* work, void* stream) {

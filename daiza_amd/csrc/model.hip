@@ -513,7 +513,7 @@ static int launch_attention(int grp, dim3 grid, const AttnArgs& a, hipStream_t s
 // further on leaves DeltaNet layers a token ahead.
 static int kv4_reserve(dz_ctx* x, int n) {
   if (x->kv4.layer.empty()) return DZ_OK;
-  return x->kv4.work.reserve(kv4_attend_work(x->kv4.layer[0], (int)x->m->cfg.n_head, n));
+  return x->kv4.work.reserve(kv4_attend_work(x->kv4.layer[0], (int)x->m->cfg.n_head, n, x->kv4.track));
 }
 
 // Attention of n tokens at positions pos .. of a context whose cache is in 4 bits, from their in-projection: its rows into

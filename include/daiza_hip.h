@@ -180,10 +180,13 @@ int dz_kv4_read_dev(const dz_kv4* c, int start, int n, float* k, float* v, void*
  * infinity or a NaN of a later row) does not reach it.
  * With `weights` (f32 [kv_heads] rows of ldw >= len elements, NULL: none), weights[g][j] += the sum of
  * query j's softmax weights over all queries and the heads of group g, in a fixed order.
- * `work` is device memory of dz_kv4_attend_work_bytes(c, n_head, n) bytes, 16-byte aligned, that no other work uses
- * until the call has run (a captured call: until its last replay has); the size does not depend on the rows held.
+ * `work` is device memory, 16-byte aligned, that no other work uses until the call has run (a captured call: until its
+ * last replay has): dz_kv4_attend_work_bytes(c, n_head, n) bytes, or dz_kv4_attend_only_work_bytes(c, n_head, n) without
+ * `weights` (with them, calls of up to 16 query rows a key/value head keep their scores, 4 bytes a query row and row of the
+ * capacity).  The sizes do not depend on the rows held.
  */
 size_t dz_kv4_attend_work_bytes(const dz_kv4* c, int n_head, int n);
+size_t dz_kv4_attend_only_work_bytes(const dz_kv4* c, int n_head, int n);
 int dz_kv4_attend_dev(const dz_kv4* c, const void* q, int64_t ldq, int type, int n_head, int n, float scale, float* weights,
                       int64_t ldw, void* out, int64_t ldo, void* work, void* stream);
 

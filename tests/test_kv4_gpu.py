@@ -493,6 +493,43 @@ def test_on_another_stream(dz):
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_work_memory_of_calls_without_weights(dz):
+    """A call that adds to no weights has no use for its scores, 25 MB of a token's 24 heads at 262144 rows."""
+    c = dz.Kv4Cache(4, 256, 262144)
+    x = _rows(420, 40, 4, 256).cuda()
+    c.append_dev(x, x)
+    q = _normal(421, 1, 24, 256).cuda()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    c.attend_dev(q, out)
+    assert torch.cuda.max_memory_allocated() - before < 8 << 20
+
+
+@pytest.mark.parametrize("nq,nkv,hd,length,n,dtype", [(24, 4, 256, 5000, 1, "f32"), (24, 4, 256, 2000, 2, "f32"), (6, 1, 256, 40, 3, "f32"),
+                                                      (24, 4, 256, 900, 21, "f32"), (8, 2, 128, 3000, 80, "bf16"),
+                                                      (8, 1, 64, 20000, 1, "f16"), (4, 4, 64, 600, 200, "f32")])
+@pytest.mark.parametrize("weights", [False, True])
+def test_work_memory_is_enough(dz, nq, nkv, hd, length, n, dtype, weights):
+    """The sizes that the library gives hold what calls write: nothing behind them changes."""
+    c = _cache(dz, _rows(422, length, nkv, hd), _rows(423, length, nkv, hd))
+    q = _normal(424, n, nq, hd).to(TYPES[dtype]).cuda()
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    ww, w = (torch.zeros(nkv, length, device="cuda") for _ in range(2))
+    c.attend_dev(q, want, weights=ww if weights else None)
+    L = dz.lib()
+    size = (L.dz_kv4_attend_work_bytes if weights else L.dz_kv4_attend_only_work_bytes)(c._h, nq, n)
+    work = torch.full((size + (1 << 24),), 0xA5, dtype=torch.uint8, device="cuda")
+    rc = L.dz_kv4_attend_dev(c._h, q.data_ptr(), nq * hd, {"f32": 0, "f16": 1, "bf16": 30}[dtype], nq, n, hd ** -0.5,
+                             w.data_ptr() if weights else None, length, out.data_ptr(), nq * hd, work.data_ptr(),
+                             torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == dz.DZ_OK and torch.equal(out, want) and torch.equal(w, ww if weights else torch.zeros_like(w))
+    assert bool((work[size:] == 0xA5).all())
+
+
 @pytest.mark.parametrize("handle", [False, True])
 def test_work_memory_while_the_current_stream_is_busy(dz, handle):
     """A call on a stream of its own takes no block that queued work of the current stream still uses, though its tensor is gone."""
@@ -504,7 +541,7 @@ def test_work_memory_while_the_current_stream_is_busy(dz, handle):
     c.attend_dev(q, want)
     dz.logprobs_dev(x, tokens, lwant)
     got, lgot = torch.zeros_like(q), torch.zeros(4, device="cuda")
-    sizes = (dz.lib().dz_kv4_attend_work_bytes(c._h, 24, 2), dz.lib().dz_logprobs_work_bytes(4, 30000, 0))
+    sizes = (dz.lib().dz_kv4_attend_only_work_bytes(c._h, 24, 2), dz.lib().dz_logprobs_work_bytes(4, 30000, 0))
     s, big = torch.cuda.Stream(), torch.ones(1 << 27, device="cuda")
     for _ in range(3):
         got.zero_()
