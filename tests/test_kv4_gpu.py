@@ -200,6 +200,28 @@ def test_attend_f32_queries_beside_outliers(dz, n, hd):
     assert bool(((w.cpu().double() - ww).abs() <= wb + 2.0 ** -24 * ww).all())
 
 
+@pytest.mark.parametrize("n,nkv", [(512, 4), (8, 256)])
+def test_attend_errors_have_no_sign(dz, n, nkv):
+    """The relative errors of a million positive f16 outputs average out, by many rows a head and by few.
+
+    An output's rounding is off by up to 2^-11 to either side, so the mean of N = 2^20 of them stays under
+    2^-10 sqrt(ln(2 / 1e-9) / 2N) = 3.1e-6 but for one run in 1e9 (Hoeffding); the f32 evaluation gets 16 half steps, 2^-20."""
+    nq, hd, length = 4 * nkv, 128, 600
+    k, v = _rows(65, length, nkv, hd), _rows(66, length, nkv, hd).abs() + 0.1
+    q = _normal(67, n, nq, hd).half().cuda()
+    c = _cache(dz, k, v)
+    out = torch.empty_like(q)
+    c.attend_dev(q, out)
+    ks, vs, grp = ref.stored(k).cuda(), ref.stored(v).cuda(), nq // nkv
+    hidden = torch.arange(length, device="cuda")[None] > torch.arange(length - n, length, device="cuda")[:, None]
+    mean = torch.zeros((), dtype=torch.float64, device="cuda")
+    for h in range(nq):
+        s = (q[:, h].double() @ ks[h // grp].t().contiguous()) * hd ** -0.5
+        want = torch.softmax(s.masked_fill(hidden, -math.inf), 1) @ vs[h // grp]
+        mean += ((out[:, h].double() - want) / want).sum()
+    assert out.numel() == 2 ** 20 and abs(mean.item() / out.numel()) < 3.1e-6 + 2.0 ** -20, mean.item() / out.numel()
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_query_that_is_not_a_number_among_many(dz, value, hd):
