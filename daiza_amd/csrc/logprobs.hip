@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kLpJoin) void logprobs_join_kernel(const E* __restr
   LogitSums s{-INFINITY, 0.f, 0.f};
   if (tid < parts) s = sums[row * parts + tid];
   const int groups = (vocab + kLpStep - 1) / kLpStep * kLpGroups;
-  gmax += row * (size_t)groups;
+  if (top) gmax += row * (size_t)groups;
   float held[kHeld], gm = -INFINITY;  // the groups tid + 256 i of the first 1024, and the largest of all of the thread's
   if (top && tid < 256) {
 #pragma unroll
@@ -354,13 +354,21 @@ int logprobs(const void* logits, int64_t ld, int type, int n, int vocab, const i
     using E = std::remove_pointer_t<decltype(e)>;
     const E* x = static_cast<const E*>(logits);
     // rows beyond the grid's second dimension go in further launches
-    for (int r0 = 0; r0 < n; r0 += 65535) {
+    for (int r0 = 0; r0 < n; r0 += std::min(65535, n - r0)) {
       logprobs_kernel<E><<<dim3((unsigned)parts, (unsigned)std::min(65535, n - r0)), 64, 0, s>>>(
           x + (size_t)r0 * ld, ld, vocab, per, sums + (size_t)r0 * parts, top ? gmax + r0 * groups : nullptr);
       DZ_HIP_CHECK(hipGetLastError());
     }
-    logprobs_join_kernel<E><<<(unsigned)n, kLpJoin, 0, s>>>(x, ld, vocab, parts, top, sums, gmax, tokens, logp, entropy, top_ids, top_logp);
-    DZ_HIP_CHECK(hipGetLastError());
+    // nor does a launch have 2^32 threads
+    constexpr int kRows = 1 << 22;
+    for (int r0 = 0; r0 < n; r0 += std::min(kRows, n - r0)) {
+      const size_t t0 = (size_t)r0 * top;
+      logprobs_join_kernel<E><<<(unsigned)std::min(kRows, n - r0), kLpJoin, 0, s>>>(
+          x + (size_t)r0 * ld, ld, vocab, parts, top, sums + (size_t)r0 * parts, top ? gmax + r0 * groups : nullptr,
+          logp ? tokens + r0 : nullptr, logp ? logp + r0 : nullptr, entropy ? entropy + r0 : nullptr, top ? top_ids + t0 : nullptr,
+          top_logp ? top_logp + t0 : nullptr);
+      DZ_HIP_CHECK(hipGetLastError());
+    }
     return DZ_OK;
   });
 }

@@ -100,6 +100,24 @@ def test_more_rows_than_a_launch_takes(dz):
     _check(dz, *_logits(9, 70000, 7), 2)
 
 
+def test_eight_million_rows(dz):
+    """More rows than a launch of the join has threads for: every row against torch's own log softmax in 64 bits."""
+    n = (1 << 23) + 77
+    x = torch.randn(n, 3, generator=torch.Generator().manual_seed(10)).cuda()
+    tokens = (torch.arange(n, device="cuda") % 3).to(torch.int32)
+    lp, ent = torch.full((n,), 9.0, device="cuda"), torch.full((n,), 9.0, device="cuda")
+    ids, tl = torch.full((n, 1), -1, dtype=torch.int32, device="cuda"), torch.full((n, 1), 9.0, device="cuda")
+    dz.logprobs_dev(x, tokens, lp, ent, ids, tl)
+    y = x.double()
+    want = y - torch.logsumexp(y, 1, keepdim=True)
+    best, at = want.max(1)
+    # three terms and a logarithm in f32: the bounds of kv4_ref.logprobs at a vocabulary of 3, |log p| and the entropy under 16
+    u = 2.0 ** -24
+    assert ((lp.double() - want.gather(1, tokens.long()[:, None])[:, 0]).abs() <= 11 * u + 4 * u * 18).all()
+    assert ((tl[:, 0].double() - best).abs() <= 11 * u + 4 * u * 18).all() and torch.equal(ids[:, 0].long(), at)
+    assert ((ent.double() + (want.exp() * want).sum(1)).abs() <= 2 * 11 * u * 17 + 8 * u * 2).all()
+
+
 def test_rows_in_and_out_of_a_long_cache(dz):
     n, nkv, hd = 70001, 1, 64
     k, v = _rows(90, n, nkv, hd), _rows(91, n, nkv, hd)
