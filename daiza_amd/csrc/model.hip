@@ -1384,6 +1384,7 @@ static int bt_reserve_verify(dz_ctx* x, int k) {
   DnRecords& r = x->bt.recs;
   const size_t lk = (size_t)x->m->n_ssm * k;
   auto& A = x->bt.allocs;
+  x->bt.kv_cap = 0;  // until all of them are there
   int rc;
   if ((rc = alloc_t(A, &r.x, lk * qkvd)) || (rc = alloc_t(A, &r.decay, lk * c.ssm_v_heads)) || (rc = alloc_t(A, &r.d, lk * inner)) ||
       (rc = alloc_t(A, &r.k, lk * kdim)))
