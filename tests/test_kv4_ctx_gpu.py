@@ -445,3 +445,22 @@ def test_a_token_allocates_nothing(dz, oracle):
     ctx.mixer_step(1, np.zeros(cfg.hidden, np.float32))
     torch.cuda.synchronize()
     assert torch.cuda.mem_get_info()[0] == before
+
+
+def test_small_caches_and_empty_evictions(dz, oracle):
+    """One row at a time, evictions that leave nothing or take nothing, and going on after each."""
+    cfg, om, model, x = _setup(dz, oracle, kv_rows=1)
+    a, n = _attn(cfg)[0], cfg.n_head // cfg.n_head_kv
+    lg = x.forward_single_token(3)[1]
+    assert np.allclose(x.kv_weights(a), n, atol=n * 2.0 ** -22)
+    with pytest.raises(dz.DaizaError, match="full"):
+        x.forward_single_token(4)
+    assert x.kv_evict(1, 1).tolist() == [[[0]] * cfg.n_head_kv] * len(_attn(cfg))  # all stay
+    assert x.kv_evict(0, 0).shape == (len(_attn(cfg)), cfg.n_head_kv, 0) and x.kv_len(a) == 0 and x.pos == 1
+    for t in (4, 5, 6):  # each token sees itself alone
+        x.forward_single_token(t)
+        assert np.allclose(x.kv_weights(a), n, atol=n * 2.0 ** -22) and x.kv_len(a) == 1
+        x.kv_evict(0, 0)
+    assert x.pos == 4
+    x.reset()
+    assert np.array_equal(x.forward_single_token(3)[1], lg)

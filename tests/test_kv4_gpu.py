@@ -584,6 +584,45 @@ def test_work_memory_while_the_current_stream_is_busy(dz, handle):
         assert all(bool((t == 7).all()) for t in kept)
 
 
+@pytest.mark.parametrize("handle", [False, True])
+def test_captured_on_a_forked_stream(dz, handle):
+    """A call given another stream of the capture, forked from the capturing one and joined again, replays with memory of the
+    graph's own."""
+    k, v = _rows(430, 900, 4, 256), _rows(431, 900, 4, 256)
+    c = _cache(dz, k, v)
+    q, x = torch.zeros(2, 24, 256, device="cuda"), torch.zeros(3, 30000, device="cuda")
+    tokens = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+    out, w, lp = torch.empty_like(q), torch.zeros(4, 900, device="cuda"), torch.empty(3, device="cuda")
+    ids, tl = torch.empty(3, 9, dtype=torch.int32, device="cuda"), torch.empty(3, 9, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(stream):
+        c.attend_dev(q, out, weights=w, stream=stream)
+        dz.logprobs_dev(x, tokens, lp, None, ids, tl, stream=stream)
+
+    step(None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        step(side.cuda_stream if handle else side)
+        torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        q.copy_(_normal(440 + i, 2, 24, 256))
+        x.copy_(_normal(450 + i, 3, 30000))
+        w.zero_()
+        junk = [torch.full((1 << 22,), 3.0, device="cuda") for _ in range(8)]  # whatever is free is written to
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (out, w, lp, ids, tl)]
+        w.zero_()
+        step(None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (out, w, lp, ids, tl))), i
+        del junk
+
+
 def test_two_caches_at_once(dz):
     """Two caches on two streams do not touch each other's work."""
     q = _normal(500, 2, 24, 256).cuda()

@@ -100,6 +100,77 @@ def test_more_rows_than_a_launch_takes(dz):
     _check(dz, *_logits(9, 70000, 7), 2)
 
 
+def test_codes_past_32_bits(dz):
+    """34 million rows of 128 bytes of codes: rows of zeros, on which every score is 0, and a few others at either end of them."""
+    n, hd, nq = (1 << 25) + (1 << 20), 256, 6
+    c = dz.Kv4Cache(1, hd, n + 8)
+    k, v = _rows(92, 8, 1, hd), _rows(93, 8, 1, hd)
+    c.append_dev(k[:3].cuda(), v[:3].cuda())
+    zeros = torch.zeros(n, 1, hd, dtype=torch.bfloat16, device="cuda")
+    c.append_dev(zeros, zeros)
+    del zeros
+    c.append_dev(k[3:].cuda(), v[3:].cuda())
+    ks, vs = ref.stored(k)[0], ref.stored(v)[0]
+    gk, gv = (torch.empty(1, 6, hd, device="cuda") for _ in range(2))
+    c.read_dev(n + 2, gk, gv)
+    assert torch.equal(gk[0, 1:].cpu().double(), ks[3:]) and torch.equal(gv[0, 1:].cpu().double(), vs[3:])
+    assert not gk[0, 0].any() and not gv[0, 0].any()
+    q = _normal(94, 2, nq, hd) * 8.0  # the last rows' scores against millions of zeros
+    out, w = torch.empty(2, nq, hd, device="cuda"), torch.zeros(1, n + 8, device="cuda")
+    c.attend_dev(q.cuda(), out, weights=w)
+    s = (q.double() @ ks.T) / math.sqrt(hd)  # [2][heads][8]
+    s[0, :, 7] = -math.inf
+    m = s.amax(2, keepdim=True).clamp(min=0)
+    p, z0 = torch.exp(s - m), torch.exp(-m[..., 0])
+    z = p.sum(2) + n * z0
+    want = (p @ vs) / z[..., None]
+    # f32 sums of 34 million terms in 256 chunks of eight waves with 8 terms a tile and lane: partial sums of at most
+    # 34e6 / 2048 / 32 = 520 tiles' totals, joined over waves and chunks, each addition 2^-24; scores and exponentials as
+    # in kv4_ref.attend (hd + 4 and 16 units on scores of at most |s| + |m|)
+    u = 2.0 ** -24
+    terms = (q.double().abs() @ ks.abs().T).amax(2) / math.sqrt(hd)
+    rel = (520 + 8 + 8 + 256 + 16) * u + 2 * (hd + 4) * u * terms
+    assert bool(((out.cpu().double() - want).abs() <= rel[..., None] * ((p @ vs.abs()) / z[..., None]) + u * want.abs()).all())
+    ww, got = (p / z[..., None]).sum((0, 1)), w[0].cpu().double()
+    ends = torch.cat([got[:3], got[-5:]])
+    assert bool(((ends - ww).abs() <= rel.max() * ww + 12 * u * ww).all())
+    each = (z0 / z).sum()
+    assert bool(((got[3:-5] - each).abs() <= (rel.max() + 12 * u) * each).all())
+    # the three best of all but the newest two rows
+    small = dz.Kv4Cache(1, hd, 5)
+    kept, dw = torch.empty(1, 5, dtype=torch.int32, device="cuda"), torch.empty(1, 5, device="cuda")
+    c.evict_dev(small, 5, 2, w, dw, kept)
+    order = torch.sort(w[0, :-2], descending=True, stable=True).indices[:3].sort().values
+    assert torch.equal(kept[0].cpu().long(), torch.cat([order.cpu(), torch.tensor([n + 6, n + 7])]))
+    rk = torch.empty(1, 5, hd, device="cuda")
+    small.read_dev(0, rk)
+    assert torch.equal(rk[0, 3:].cpu().double(), ks[6:]) and torch.equal(dw[0], w[0, kept[0].long()])
+
+
+def test_logits_past_32_bits(dz):
+    """9000 rows of 248320 bf16 logits are 2^31 elements and more: the last rows by themselves give the same."""
+    n, vocab = 9000, 248320
+    x = torch.randn(64, vocab, generator=torch.Generator().manual_seed(12)).bfloat16().cuda()
+    big = torch.empty(n, vocab, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, n, 64):
+        big[i:i + 64] = x[:min(64, n - i)].roll(i // 64, 1)
+    tokens = (torch.arange(n, device="cuda") * 27).to(torch.int32)
+
+    def run(x, t):
+        out = [torch.empty(x.shape[0], device="cuda"), torch.empty(x.shape[0], device="cuda"),
+               torch.empty(x.shape[0], 5, dtype=torch.int32, device="cuda"), torch.empty(x.shape[0], 5, device="cuda")]
+        dz.logprobs_dev(x, t, *out)
+        return out
+
+    whole = run(big, tokens)
+    _check(dz, big[-2:].clone(), tokens[-2:].cpu(), 5)
+    for r in (0, 4000, 8640, n - 100):
+        part = run(big[r:r + 100].clone(), tokens[r:r + 100].clone())
+        # more parts of a row with fewer rows: sums in another order
+        assert torch.equal(whole[2][r:r + 100], part[2])
+        assert all(torch.allclose(whole[i][r:r + 100], part[i], rtol=0, atol=1e-4) for i in (0, 1, 3))
+
+
 def test_eight_million_rows(dz):
     """More rows than a launch of the join has threads for: every row against torch's own log softmax in 64 bits."""
     n = (1 << 23) + 77
