@@ -392,7 +392,7 @@ __device__ __forceinline__ float sum_over_lk(float x) {
 //   RT = 4                   bound by the vector instructions (of which a wave dequantises its values with about 190 a tile, 32
 //                            positions) and the matrix instructions (96 of 6.7 ns a tile: three parts of Q, three of P) that
 //                            do not run beside each other well enough: 1.7 us a tile.  333 tokens behind 7000 positions, 59
-//                            GFLOP, 186 us.  f32 queries as six 6-bit digits of the 16x16x128 instruction, which take the keys
+//                            GFLOP, 182 to 190 us.  f32 queries as six 6-bit digits of the 16x16x128 instruction, which take the keys
 //                            as they stand, took 169 us, but hold a query to 2^-29 of the largest of each 32 dims: beside
 //                            an outlier that meets keys of 0 the other dims lose bits that an f32 product has.
 // Tiles with blocks that are not numbers, and calls that keep their scores, take loops of their own: in the common one

@@ -271,7 +271,9 @@ int dz_model_weight_bytes(const dz_model* m, uint64_t* q1_bytes);
 /*
  * A context whose attention layers hold their keys and values in 4 bits (dz_kv4 above, 1088 instead of 8192 bytes a position
  * and layer at the 27B shape), for kv_rows rows (0: max_ctx; fewer than max_ctx with eviction).  Every call on
- * contexts works on it, by the per-kernel path (dz_ctx_token_kernel is 0); results differ from an f32 context's by what
+ * contexts works on it, by the per-kernel path without its graph (dz_ctx_token_kernel is 0): at the 27B shape single tokens
+ * are slower than on an f32 context up to about twenty thousand positions (394 against 526 tok/s at 1024, 373 against 456 at 8192,
+ * 360 against 314 at 32768); n-token forwards and verifies are not.  Results differ from an f32 context's by what
  * 4 bits lose.  dz_ctx_get_kv reads what the rows stand for, dz_ctx_set_kv rounds to it; dz_ctx_copy_state
  * needs contexts of one kind.  The reference has no such cache.
  * track != 0: the context also sums the attention weight that each cached row receives (over the heads of a key/value
