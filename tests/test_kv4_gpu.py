@@ -260,6 +260,22 @@ def test_attend_strided_and_scaled(dz):
     assert bool((got[:, :2] == 3).all()) and bool((got[:, 514:] == 3).all())
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 9, 120])
+def test_attend_at_odd_addresses(dz, dtype, n):
+    """16-bit queries and outputs out of wider arrays, two bytes off any alignment, by one tile of rows a workgroup and by four."""
+    k, v = _rows(34, 300, 2, 128), _rows(35, 300, 2, 128)
+    c = _cache(dz, k, v)
+    q = _normal(36, n, 4, 128).to(TYPES[dtype])
+    want, w0, w1 = torch.empty(n, 4, 128, dtype=TYPES[dtype], device="cuda"), *(torch.zeros(2, 300, device="cuda") for _ in range(2))
+    c.attend_dev(q.cuda(), want, weights=w0)
+    src, dst = (torch.full((n, 4 * 128 + 7), 3.0, dtype=TYPES[dtype], device="cuda") for _ in range(2))
+    src[:, 1:513] = q.flatten(1).cuda()
+    c.attend_dev(src[:, 1:513].unflatten(1, (4, 128)), dst[:, 3:515].unflatten(1, (4, 128)), weights=w1)
+    assert torch.equal(dst[:, 3:515].unflatten(1, (4, 128)), want) and torch.equal(w0, w1)
+    assert bool((dst[:, :3] == 3).all()) and bool((dst[:, 515:] == 3).all())
+
+
 @pytest.mark.parametrize("nq,nkv,hd,length,n,at", [(6, 1, 256, 70, 20, 60), (4, 2, 128, 300, 120, 200), (2, 1, 64, 40, 40, 0),
                                                    (6, 1, 256, 700, 5, 697), (24, 4, 256, 40, 1, 12)])
 @pytest.mark.parametrize("where", ["k", "v"])
