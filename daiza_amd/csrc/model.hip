@@ -1690,6 +1690,8 @@ static int bt_verify_commit(dz_ctx* x, int a) {
     DZ_HIP_CHECK(launch(bt_commit_kernel, dim3((unsigned)(4 * c.ssm_v_heads + (qkvd + 255) / 256), (unsigned)m->n_ssm), dim3(256),
                         x->s, x->ssm_state, x->conv, (const int*)x->ring_base_dev, p0, x->bt.recs, a, (int)c.ssm_k_heads,
                         (int)c.ssm_v_heads, qkvd));
+  const int rc = bt_finish(x, a, p0, a - 1);
+  if (rc) return rc;
   // the weights of the drafts that stay: their queries once more over the rows that they see, as a forward of them alone
   // (the outputs go to a buffer that nothing reads)
   const int row = p0 - x->kv4.evicted;
@@ -1700,8 +1702,6 @@ static int bt_verify_commit(dz_ctx* x, int a) {
                             v.cap, x->bt.gy, qd, x->kv4.work.ptr, x->s, nullptr))
       return rc;
   }
-  const int rc = bt_finish(x, a, p0, a - 1);
-  if (rc) return rc;
   DZ_HIP_CHECK(hipStreamSynchronize(x->s));
   return DZ_OK;
 }
